@@ -7,7 +7,9 @@ set -euo pipefail
 here="$(cd "$(dirname "$0")" && pwd)"
 out="$here/../lib"
 mkdir -p "$out"
-flags="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -shared"
+# no packed f32 arithmetic (v_pk_add/mul/fma_f32) anywhere: the compiler makes it of plain float code by itself,
+# and some of its forms have given wrong results on this GPU.  The host pass warns that it does not know the feature.
+flags="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -shared -Xclang -target-feature -Xclang -packed-fp32-ops"
 if [ "${1:-}" = "--stamps" ]; then
   hipcc $flags -DARTMIPS_DIAG -DARTMIPS_STAMPS_BUILD -o "$out/libartmips_stamps.so" "$here/artmips.hip"
   echo "built $out/libartmips_stamps.so"
