@@ -1,0 +1,362 @@
+// libartread.so — operators that read the passages a search found (include/artread.h).  gfx950 only.
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdarg.h>
+#include <stdint.h>
+#include <stdio.h>
+#include <string.h>
+
+#include "../../include/artread.h"
+#include "artread_attend.h"
+#include "artread_embed.h"
+
+static thread_local char g_read_err[512] = "";
+
+static int read_fail(int code, const char* fmt, ...) {
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(g_read_err, sizeof(g_read_err), fmt, ap);
+    va_end(ap);
+    return code;
+}
+
+#define READ_HIP(expr)                                                                          \
+    do {                                                                                        \
+        hipError_t e__ = (expr);                                                                \
+        if (e__ != hipSuccess)                                                                  \
+            return read_fail(ARTREAD_ERR_HIP, "%s failed: %s (%s:%d)", #expr, hipGetErrorString(e__), \
+                             __FILE__, __LINE__);                                               \
+    } while (0)
+#define READ_ARG(cond, ...)                                          \
+    do {                                                             \
+        if (!(cond)) return read_fail(ARTREAD_ERR_ARG, __VA_ARGS__); \
+    } while (0)
+
+struct ReadDeviceGuard {
+    int prev = -1, dev;
+    hipError_t err = hipSuccess;
+    explicit ReadDeviceGuard(int d) : dev(d) {
+        err = hipGetDevice(&prev);
+        if (err == hipSuccess && prev != dev) err = hipSetDevice(dev);
+    }
+    ~ReadDeviceGuard() {
+        if (prev >= 0 && prev != dev) (void)hipSetDevice(prev);
+    }
+};
+
+extern "C" const char* artread_last_error(void) { return g_read_err; }
+
+static constexpr int64_t kLimit = (int64_t)1 << 31;
+static int elem_bytes(int dtype) { return dtype == ARTREAD_F32 ? 4 : 2; }
+static bool aligned(const void* p, uint64_t to) { return ((uintptr_t)p) % to == 0; }
+static int64_t round_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
+
+// ---- embedding ------------------------------------------------------------------------------------
+static int check_tokens(const void* tokens, int token_bytes, const int32_t* lengths, int64_t n, int64_t len,
+                        int64_t vocab, int64_t dim, int64_t vocab_base, Tokens* T) {
+    READ_ARG(tokens, "tokens is NULL");
+    READ_ARG(token_bytes == 4 || token_bytes == 8, "token_bytes must be 4 or 8 (got %d)", token_bytes);
+    READ_ARG(n >= 1 && len >= 1 && n < kLimit && len < kLimit && n * len < kLimit,
+             "n %lld x len %lld must be in [1, 2^31)", (long long)n, (long long)len);
+    READ_ARG(vocab >= 1 && vocab < kLimit, "vocab %lld must be in [1, 2^31)", (long long)vocab);
+    READ_ARG(dim >= 1 && dim <= (1 << 20), "dim %lld must be in [1, 2^20]", (long long)dim);
+    T->tokens = tokens;
+    T->lengths = lengths;
+    T->len = (uint32_t)len;
+    T->inv_len = len == 1 ? 0xffffffffu : (uint32_t)(((uint64_t)1 << 32) / (uint64_t)len);
+    T->vocab = vocab;
+    T->vocab_base = vocab_base;
+    T->positions = n * len;
+    return 0;
+}
+
+template <typename TT, typename OT, typename IDX, int EPV>
+static void launch_embed(const void* table, int64_t stride, const Tokens& T, float scale, void* out, int dim,
+                         hipStream_t st) {
+    const int cpr = dim / EPV, rpp = cpr < 256 ? 256 / cpr : 1;
+    const int threads = cpr < 256 ? (int)round_up((int64_t)cpr * rpp, 64) : 256;
+    const int64_t want = (T.positions + (int64_t)rpp * 8 - 1) / ((int64_t)rpp * 8);
+    const unsigned grid = (unsigned)(want < (1 << 22) ? want : (1 << 22));
+    hipLaunchKernelGGL((embed_kernel<TT, OT, IDX, EPV>), dim3(grid), dim3(threads), 0, st, (const TT*)table, stride, T,
+                       scale, (OT*)out, dim, cpr, rpp);
+}
+
+template <typename TT, typename OT>
+static void embed_any(const void* table, int64_t stride, const Tokens& T, int token_bytes, float scale, void* out,
+                      int dim, hipStream_t st) {
+    constexpr int W = 16 / sizeof(OT);
+    const bool wide = dim % W == 0 && stride % (16 / (int)sizeof(TT)) == 0 && aligned(table, 16) && aligned(out, 16);
+    if (token_bytes == 4) {
+        if (wide) launch_embed<TT, OT, int32_t, W>(table, stride, T, scale, out, dim, st);
+        else launch_embed<TT, OT, int32_t, 1>(table, stride, T, scale, out, dim, st);
+    } else {
+        if (wide) launch_embed<TT, OT, int64_t, W>(table, stride, T, scale, out, dim, st);
+        else launch_embed<TT, OT, int64_t, 1>(table, stride, T, scale, out, dim, st);
+    }
+}
+
+extern "C" int artread_embed(int device, const void* table, int table_dtype, int64_t vocab, int64_t dim,
+                             int64_t table_stride, const void* tokens, int token_bytes, const int32_t* lengths,
+                             int64_t n, int64_t len, int64_t vocab_base, float scale, void* out, int out_dtype,
+                             void* stream) {
+    Tokens T;
+    const int rc = check_tokens(tokens, token_bytes, lengths, n, len, vocab, dim, vocab_base, &T);
+    if (rc) return rc;
+    READ_ARG(table && out, "table or out is NULL");
+    READ_ARG(table_stride >= dim || vocab == 1, "table_stride %lld is below dim %lld", (long long)table_stride,
+             (long long)dim);
+    READ_ARG(table_dtype >= 0 && table_dtype <= 2 && out_dtype >= 0 && out_dtype <= 2, "unknown element type");
+    READ_ARG(out_dtype == table_dtype || table_dtype == ARTREAD_F32,
+             "out must have the table's type, or f16 / bf16 of an f32 table");
+    READ_ARG(aligned(table, elem_bytes(table_dtype)) && aligned(out, elem_bytes(out_dtype)), "misaligned pointer");
+    READ_ARG(isfinite(scale), "scale must be finite");
+    ReadDeviceGuard g(device);
+    READ_HIP(g.err);
+    hipStream_t st = (hipStream_t)stream;
+    if (table_dtype == ARTREAD_F16) embed_any<f16, f16>(table, table_stride, T, token_bytes, scale, out, (int)dim, st);
+    else if (table_dtype == ARTREAD_BF16) embed_any<bf16, bf16>(table, table_stride, T, token_bytes, scale, out, (int)dim, st);
+    else if (out_dtype == ARTREAD_F16) embed_any<float, f16>(table, table_stride, T, token_bytes, scale, out, (int)dim, st);
+    else if (out_dtype == ARTREAD_BF16) embed_any<float, bf16>(table, table_stride, T, token_bytes, scale, out, (int)dim, st);
+    else embed_any<float, float>(table, table_stride, T, token_bytes, scale, out, (int)dim, st);
+    READ_HIP(hipGetLastError());
+    return 0;
+}
+
+// Sort digits of at most nine bits, at most 256 chunks of at least 4,096 positions.
+static SortPlan sort_plan(int64_t vocab, int64_t positions) {
+    SortPlan P;
+    int bits = 1;
+    while (bits < 31 && ((int64_t)1 << bits) < vocab) ++bits;
+    P.passes = (bits + 8) / 9;
+    P.bits = (bits + P.passes - 1) / P.passes;
+    P.chunk = round_up((positions + 255) / 256, 256);
+    if (P.chunk < 4096) P.chunk = 4096;
+    P.blocks = (int)((positions + P.chunk - 1) / P.chunk);
+    return P;
+}
+
+// Workers of 64 positions where there are enough positions for them to fill the chip, fewer down to 8.
+static int sum_run(int64_t positions) {
+    int run = 64;
+    while (run > 8 && positions / run < 4096) run >>= 1;
+    return run;
+}
+
+struct GradSpace {   // byte offsets into the workspace
+    int64_t meta, counts, used, pairs0, pairs1, chain_end, partial, total;
+    int64_t pad_dim;
+    int run;
+};
+static GradSpace grad_space(int64_t vocab, int64_t dim, int64_t positions) {
+    const SortPlan P = sort_plan(vocab, positions);
+    GradSpace s;
+    int64_t at = 0;
+    auto take = [&](int64_t bytes) {
+        const int64_t here = at;
+        at += round_up(bytes, 256);
+        return here;
+    };
+    s.run = sum_run(positions);
+    s.pad_dim = round_up(dim, 4);
+    s.meta = take(sizeof(SortMeta));
+    s.counts = take((int64_t)P.blocks * (1 << P.bits) * 4);
+    s.used = take(round_up(vocab, 16));
+    s.pairs0 = take(positions * 8);
+    s.pairs1 = P.passes > 1 ? take(positions * 8) : s.pairs0;
+    s.chain_end = take(vocab * 4);
+    s.partial = take((positions + s.run - 1) / s.run * 2 * s.pad_dim * 4);
+    s.total = at;
+    return s;
+}
+
+extern "C" int64_t artread_embed_grad_workspace(int64_t vocab, int64_t dim, int64_t n, int64_t len) {
+    if (n < 1 || len < 1 || n >= kLimit || len >= kLimit || n * len >= kLimit || vocab < 1 || vocab >= kLimit ||
+        dim < 1 || dim > (1 << 20))
+        return read_fail(ARTREAD_ERR_ARG, "sizes out of range");
+    return grad_space(vocab, dim, n * len).total;
+}
+
+template <typename GT, typename OT, int EPV>
+static void launch_grad_sums(const void* grad, const Pair* sorted, const SortMeta* meta, const uint8_t* used,
+                             const Tokens& T, float scale, void* table, int dim, const GradSpace& s, float* partial,
+                             int32_t* chain_end, hipStream_t st) {
+    SumPlan S;
+    S.run = s.run;
+    S.cpr = dim / EPV;
+    S.rpp = S.cpr < 256 ? 256 / S.cpr : 1;
+    S.pad_dim = s.pad_dim;
+    S.workers = (T.positions + s.run - 1) / s.run;
+    S.sum_groups = (S.workers + S.rpp - 1) / S.rpp;
+    const int threads = S.cpr < 256 ? (int)round_up((int64_t)S.cpr * S.rpp, 64) : 256;
+    int64_t clear = (T.vocab + S.rpp * 4 - 1) / (S.rpp * 4);
+    if (clear > 16384) clear = 16384;
+    hipLaunchKernelGGL((grad_sum_kernel<GT, OT, EPV>), dim3((unsigned)(S.sum_groups + clear)), dim3(threads), 0, st,
+                       (const GT*)grad, sorted, meta, used, T.vocab, scale, (OT*)table, dim, S, partial, chain_end);
+    const unsigned jx = (unsigned)(S.workers < 4096 ? S.workers : 4096);
+    hipLaunchKernelGGL((grad_join_kernel<OT>), dim3(jx, (unsigned)((dim + 63) / 64)), dim3(256), 0, st, sorted, meta,
+                       scale, (OT*)table, dim, S, partial, chain_end);
+}
+
+template <typename GT, typename OT>
+static void grad_sums(const void* grad, const Pair* sorted, const SortMeta* meta, const uint8_t* used, const Tokens& T,
+                      float scale, void* table, int dim, const GradSpace& s, float* partial, int32_t* chain_end,
+                      hipStream_t st) {
+    constexpr int W = 16 / sizeof(GT);
+    if (dim % W == 0 && aligned(grad, 16) && aligned(table, 16))
+        launch_grad_sums<GT, OT, W>(grad, sorted, meta, used, T, scale, table, dim, s, partial, chain_end, st);
+    else
+        launch_grad_sums<GT, OT, 1>(grad, sorted, meta, used, T, scale, table, dim, s, partial, chain_end, st);
+}
+
+template <typename IDX>
+static const Pair* sort_tokens(const Tokens& T, char* ws, const GradSpace& s, hipStream_t st) {
+    const SortPlan P = sort_plan(T.vocab, T.positions);
+    SortMeta* meta = (SortMeta*)(ws + s.meta);
+    uint32_t* counts = (uint32_t*)(ws + s.counts);
+    uint8_t* used = (uint8_t*)(ws + s.used);
+    Pair* pairs[2] = {(Pair*)(ws + s.pairs0), (Pair*)(ws + s.pairs1)};
+    const dim3 grid((unsigned)P.blocks), block(256);
+    for (int pass = 0; pass < P.passes; ++pass) {
+        const int shift = pass * P.bits;
+        const Pair* in = pairs[(pass + 1) & 1];
+        if (pass == 0) {
+            hipLaunchKernelGGL((sort_count_kernel<IDX, true>), grid, block, 0, st, T, in, meta, P, shift, counts, used);
+            hipLaunchKernelGGL((sort_place_kernel<IDX, true>), grid, block, 0, st, T, in, meta, P, shift, counts,
+                               pairs[0], used);
+        } else {
+            hipLaunchKernelGGL((sort_count_kernel<IDX, false>), grid, block, 0, st, T, in, meta, P, shift, counts, used);
+            hipLaunchKernelGGL((sort_place_kernel<IDX, false>), grid, block, 0, st, T, in, meta, P, shift, counts,
+                               pairs[pass & 1], used);
+        }
+    }
+    return pairs[(P.passes - 1) & 1];
+}
+
+extern "C" int artread_embed_grad(int device, const void* grad_out, int grad_dtype, const void* tokens, int token_bytes,
+                                  const int32_t* lengths, int64_t n, int64_t len, int64_t vocab, int64_t dim,
+                                  int64_t vocab_base, float scale, void* grad_table, int table_dtype, void* workspace,
+                                  int64_t workspace_bytes, void* stream) {
+    Tokens T;
+    const int rc = check_tokens(tokens, token_bytes, lengths, n, len, vocab, dim, vocab_base, &T);
+    if (rc) return rc;
+    READ_ARG(grad_out && grad_table && workspace, "grad_out, grad_table or workspace is NULL");
+    READ_ARG(grad_dtype >= 0 && grad_dtype <= 2 && table_dtype >= 0 && table_dtype <= 2, "unknown element type");
+    READ_ARG(table_dtype == grad_dtype || table_dtype == ARTREAD_F32, "grad_table must have grad_out's type, or f32");
+    READ_ARG(aligned(grad_out, elem_bytes(grad_dtype)) && aligned(grad_table, elem_bytes(table_dtype)),
+             "misaligned pointer");
+    READ_ARG(isfinite(scale), "scale must be finite");
+    const GradSpace s = grad_space(vocab, dim, T.positions);
+    READ_ARG(aligned(workspace, 16) && workspace_bytes >= s.total, "workspace of %lld bytes, %lld needed, 16-byte aligned",
+             (long long)workspace_bytes, (long long)s.total);
+    ReadDeviceGuard g(device);
+    READ_HIP(g.err);
+    hipStream_t st = (hipStream_t)stream;
+    char* ws = (char*)workspace;
+    const Pair* sorted = token_bytes == 4 ? sort_tokens<int32_t>(T, ws, s, st) : sort_tokens<int64_t>(T, ws, s, st);
+    READ_HIP(hipGetLastError());
+    const SortMeta* meta = (const SortMeta*)(ws + s.meta);
+    const uint8_t* used = (const uint8_t*)(ws + s.used);
+    float* partial = (float*)(ws + s.partial);
+    int32_t* ends = (int32_t*)(ws + s.chain_end);
+#define SUMS(GT, OT) grad_sums<GT, OT>(grad_out, sorted, meta, used, T, scale, grad_table, (int)dim, s, partial, ends, st)
+    if (grad_dtype == ARTREAD_F32) SUMS(float, float);
+    else if (grad_dtype == ARTREAD_F16 && table_dtype == ARTREAD_F16) SUMS(f16, f16);
+    else if (grad_dtype == ARTREAD_F16) SUMS(f16, float);
+    else if (table_dtype == ARTREAD_BF16) SUMS(bf16, bf16);
+    else SUMS(bf16, float);
+#undef SUMS
+    READ_HIP(hipGetLastError());
+    return 0;
+}
+
+// ---- attention ------------------------------------------------------------------------------------
+static int check_attend(const artread_attend_t* a) {
+    READ_ARG(a, "arguments are NULL");
+    READ_ARG(a->dtype == ARTREAD_F16 || a->dtype == ARTREAD_BF16, "attention takes f16 or bf16");
+    READ_ARG(a->batch >= 1 && a->rows >= 1 && a->passages >= 1 && a->len >= 1 && a->heads >= 1 && a->kv_heads >= 1,
+             "batch, rows, passages, len and heads must be positive");
+    READ_ARG(a->heads % a->kv_heads == 0, "%lld heads cannot share %lld key heads", (long long)a->heads,
+             (long long)a->kv_heads);
+    READ_ARG(a->dim >= 8 && a->dim <= 128 && a->dim % 8 == 0, "dim %lld must be a multiple of 8 up to 128",
+             (long long)a->dim);
+    const int64_t sizes[6] = {a->batch, a->rows, a->passages, a->len, a->heads, a->kv_heads};
+    for (int i = 0; i < 6; ++i) READ_ARG(sizes[i] < kLimit, "sizes must be below 2^31");
+    READ_ARG((double)a->batch * a->rows * a->heads < (double)kLimit &&
+                 (double)a->batch * a->passages * a->len * a->kv_heads < (double)kLimit,
+             "q and k hold at most 2^31 - 1 rows each");
+    READ_ARG(isfinite(a->scale), "scale must be finite");
+    const int64_t strides[11] = {a->q_batch, a->q_row, a->q_head, a->k_batch, a->k_passage, a->k_row,
+                                 a->k_head, a->v_batch, a->v_passage, a->v_row, a->v_head};
+    for (int i = 0; i < 11; ++i)
+        READ_ARG(strides[i] >= 0 && strides[i] % 8 == 0 && strides[i] < kLimit,
+                 "strides must be multiples of 8 in [0, 2^31)");
+    return 0;
+}
+static int check_attend_call(const artread_attend_t* a) {
+    const int rc = check_attend(a);
+    if (rc) return rc;
+    READ_ARG(a->q && a->k && a->v && a->out, "q, k, v or out is NULL");
+    READ_ARG(aligned(a->rest, 16), "rest must be 16-byte aligned");
+    READ_ARG(aligned(a->q, 16) && aligned(a->k, 16) && aligned(a->v, 16) && aligned(a->out, 16),
+             "q, k, v and out must be 16-byte aligned");
+    return 0;
+}
+static unsigned grid_of(int64_t items) { return (unsigned)(items < (1 << 22) ? items : (1 << 22)); }
+
+extern "C" int64_t artread_attend_workspace(const artread_attend_t* a) {
+    const int rc = check_attend(a);
+    return rc ? rc : 0;
+}
+
+extern "C" int artread_attend(int device, const artread_attend_t* a, void* workspace, int64_t workspace_bytes,
+                              void* stream) {
+    const int rc = check_attend_call(a);
+    if (rc) return rc;
+    (void)workspace;
+    (void)workspace_bytes;
+    ReadDeviceGuard g(device);
+    READ_HIP(g.err);
+    hipStream_t st = (hipStream_t)stream;
+    const dim3 grid(grid_of(a->batch * a->rows * a->heads));
+    if (a->dtype == ARTREAD_F16) hipLaunchKernelGGL(attend_simple_kernel<f16>, grid, dim3(64), 0, st, *a);
+    else hipLaunchKernelGGL(attend_simple_kernel<bf16>, grid, dim3(64), 0, st, *a);
+    READ_HIP(hipGetLastError());
+    return 0;
+}
+
+extern "C" int64_t artread_attend_grad_workspace(const artread_attend_t* a) {
+    const int rc = check_attend(a);
+    if (rc) return rc;
+    return round_up(a->batch * a->heads * a->rows * 4, 256);
+}
+
+extern "C" int artread_attend_grad(int device, const artread_attend_t* a, const artread_attend_grads_t* gr,
+                                   void* workspace, int64_t workspace_bytes, void* stream) {
+    const int rc = check_attend_call(a);
+    if (rc) return rc;
+    READ_ARG(gr && a->lse && gr->grad_out && gr->grad_q && gr->grad_k && gr->grad_v, "a pointer is NULL");
+    const int64_t strides[3] = {gr->g_batch, gr->g_row, gr->g_head};
+    for (int i = 0; i < 3; ++i)
+        READ_ARG(strides[i] >= 0 && strides[i] % 8 == 0 && strides[i] < kLimit,
+                 "strides must be multiples of 8 in [0, 2^31)");
+    READ_ARG(aligned(gr->grad_out, 16) && aligned(gr->grad_q, 16) && aligned(gr->grad_k, 16) && aligned(gr->grad_v, 16),
+             "gradients must be 16-byte aligned");
+    const int64_t need = artread_attend_grad_workspace(a);
+    READ_ARG(workspace && aligned(workspace, 16) && workspace_bytes >= need,
+             "workspace of %lld bytes, %lld needed, 16-byte aligned", (long long)workspace_bytes, (long long)need);
+    ReadDeviceGuard g(device);
+    READ_HIP(g.err);
+    hipStream_t st = (hipStream_t)stream;
+    float* delta = (float*)workspace;
+    const dim3 gq(grid_of(a->batch * a->rows * a->heads));
+    const dim3 gk(grid_of(a->batch * a->passages * a->len * a->kv_heads));
+    if (a->dtype == ARTREAD_F16) {
+        hipLaunchKernelGGL(attend_grad_q_simple_kernel<f16>, gq, dim3(64), 0, st, *a, *gr, delta);
+        hipLaunchKernelGGL(attend_grad_kv_simple_kernel<f16>, gk, dim3(64), 0, st, *a, *gr, delta);
+    } else {
+        hipLaunchKernelGGL(attend_grad_q_simple_kernel<bf16>, gq, dim3(64), 0, st, *a, *gr, delta);
+        hipLaunchKernelGGL(attend_grad_kv_simple_kernel<bf16>, gk, dim3(64), 0, st, *a, *gr, delta);
+    }
+    READ_HIP(hipGetLastError());
+    return 0;
+}

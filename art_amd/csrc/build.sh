@@ -20,6 +20,8 @@ hipcc $flags -DARTMIPS_DIAG -o "$out/libartmips_diag.so" "$here/artmips.hip" &
 diag_pid=$!
 hipcc $flags -o "$out/libarttok.so" "$here/arttok.hip" &
 tok_pid=$!
+hipcc $flags -o "$out/libartread.so" "$here/artread.hip" &
+read_pid=$!
 if [ "${1:-}" = "--asm" ]; then
   tmp="${2:-/tmp/artmips_asm}"
   mkdir -p "$tmp"
@@ -30,4 +32,5 @@ else
 fi
 wait $diag_pid
 wait $tok_pid
-echo "built $out/libartmips.so $out/libartmips_diag.so $out/libarttok.so"
+wait $read_pid
+echo "built $out/libartmips.so $out/libartmips_diag.so $out/libarttok.so $out/libartread.so"

@@ -239,6 +239,17 @@ class DeviceTokenStore(object):
                                          ctypes.c_void_p(torch.cuda.current_stream(ids.device).cuda_stream)))
         return tokens.view(tuple(ids.shape) + (max_len,)), lens.view(tuple(ids.shape))
 
+    def embed(self, ids, table, max_len=None, scale=1.0, vocab_base=0, out_dtype=None):
+        """The tokens of `ids` as rows of `table` [vocab, dim] on the store's device: ``gather`` and then
+        ``art_amd.reader.embed_tokens``.  Returns (states [..., max_len, dim], lengths [...] int32), zeros
+        behind an item's length and for an id outside the dataset (length -1).  Differentiable in `table`."""
+        from .reader import embed_tokens
+
+        if table.device != ids.device:
+            raise ValueError("table is on %s, the store on cuda:%d" % (table.device, self.device))
+        tokens, lens = self.gather(ids, max_len=max_len)
+        return embed_tokens(tokens, table, lens, scale=scale, vocab_base=vocab_base, out_dtype=out_dtype), lens
+
     def info(self):
         a, b, c = ctypes.c_int64(), ctypes.c_int64(), ctypes.c_int64()
         _tcheck(_tok().arttok_info(self._h, ctypes.byref(a), ctypes.byref(b), ctypes.byref(c)))
