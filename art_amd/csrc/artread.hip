@@ -8,6 +8,7 @@
 
 #include "../../include/artread.h"
 #include "artread_attend.h"
+#include "artread_attend_grad.h"
 #include "artread_embed.h"
 
 static thread_local char g_read_err[512] = "";
@@ -303,23 +304,88 @@ static int check_attend_call(const artread_attend_t* a) {
 }
 static unsigned grid_of(int64_t items) { return (unsigned)(items < (1 << 22) ? items : (1 << 22)); }
 
+// How a forward call runs.  Up to 32 rows (64 at 64 columns) of a key head are one wave's, which streams the
+// keys; more share their tiles of keys in a workgroup.
+struct AttendShape {
+    bool stream;
+    int qb;
+    AttendPlan plan;
+    Partials partials(void* ws, const artread_attend_t* a) const {
+        Partials W;
+        W.rows = a->batch * a->kv_heads * plan.row_count;
+        W.o = (float*)ws;
+        W.ml = (float2*)((char*)ws + round_up(plan.splits * W.rows * a->dim * 4, 256));
+        return W;
+    }
+    int64_t bytes(const artread_attend_t* a) const {
+        const int64_t rows = a->batch * a->kv_heads * plan.row_count;
+        return plan.splits > 1 ? round_up(plan.splits * rows * a->dim * 4, 256) + round_up(plan.splits * rows * 8, 256) : 0;
+    }
+};
+static void plan_scale(AttendPlan* P, float scale) {
+    P->c = scale == 0.0f ? 1.0f : fabsf(scale) * kLog2e;
+    P->q_and = scale == 0.0f ? 0u : 0xffffffffu;
+    P->q_xor = scale < 0.0f ? 0x80008000u : 0u;
+}
+static AttendShape attend_shape(const artread_attend_t* a) {
+    AttendShape S;
+    AttendPlan& P = S.plan;
+    P.share = (int)(a->heads / a->kv_heads);
+    P.row_count = a->rows * P.share;
+    S.stream = P.row_count <= (a->dim <= 64 ? 64 : 32);
+    S.qb = S.stream && P.row_count > 32 ? 2 : 1;
+    const int block = (S.stream ? 32 : 128) * S.qb, keys = S.stream ? 32 : 64;
+    P.row_blocks = (P.row_count + block - 1) / block;
+    P.items = a->batch * a->kv_heads * P.row_blocks;
+    const int64_t tiles = a->passages * ((a->len + keys - 1) / keys);
+    int64_t want = ((S.stream ? 4096 : 512) + P.items - 1) / P.items, most = tiles / (S.stream ? 2 : 4);
+    want = want < most ? want : most;
+    P.splits = (int)(want < 1 ? 1 : (want < 256 ? want : 256));
+    plan_scale(&P, a->scale);
+    return S;
+}
+
 extern "C" int64_t artread_attend_workspace(const artread_attend_t* a) {
     const int rc = check_attend(a);
-    return rc ? rc : 0;
+    return rc ? rc : attend_shape(a).bytes(a);
+}
+
+template <typename T, int DP>
+static void launch_attend(const artread_attend_t* a, const AttendShape& S, const Partials& W, hipStream_t st) {
+    const int64_t parts = S.plan.items * S.plan.splits;
+    if (S.stream) {
+        const dim3 grid(grid_of((parts + 3) / 4));
+        if (S.qb == 1) hipLaunchKernelGGL((attend_stream_kernel<T, DP, 1>), grid, dim3(256), 0, st, *a, S.plan, W);
+        else if constexpr (DP == 64) hipLaunchKernelGGL((attend_stream_kernel<T, DP, 2>), grid, dim3(256), 0, st, *a, S.plan, W);
+    } else {
+        const dim3 grid(grid_of(round_up(parts, 8)));
+        hipLaunchKernelGGL((attend_tile_kernel<T, DP, 1>), grid, dim3(256), 0, st, *a, S.plan, W);
+    }
+    if (S.plan.splits > 8)
+        hipLaunchKernelGGL((attend_join_kernel<T, 8>), dim3(grid_of(W.rows)), dim3(256), 0, st, *a, S.plan, W);
+    else if (S.plan.splits > 1)
+        hipLaunchKernelGGL((attend_join_kernel<T, 1>), dim3(grid_of((W.rows + 7) / 8)), dim3(256), 0, st, *a, S.plan, W);
 }
 
 extern "C" int artread_attend(int device, const artread_attend_t* a, void* workspace, int64_t workspace_bytes,
                               void* stream) {
     const int rc = check_attend_call(a);
     if (rc) return rc;
-    (void)workspace;
-    (void)workspace_bytes;
+    const AttendShape S = attend_shape(a);
+    const int64_t need = S.bytes(a);
+    READ_ARG(need == 0 || (workspace && aligned(workspace, 16) && workspace_bytes >= need),
+             "workspace of %lld bytes, %lld needed, 16-byte aligned", (long long)workspace_bytes, (long long)need);
+    const Partials W = S.partials(workspace, a);
     ReadDeviceGuard g(device);
     READ_HIP(g.err);
     hipStream_t st = (hipStream_t)stream;
-    const dim3 grid(grid_of(a->batch * a->rows * a->heads));
-    if (a->dtype == ARTREAD_F16) hipLaunchKernelGGL(attend_simple_kernel<f16>, grid, dim3(64), 0, st, *a);
-    else hipLaunchKernelGGL(attend_simple_kernel<bf16>, grid, dim3(64), 0, st, *a);
+    if (a->dtype == ARTREAD_F16) {
+        if (a->dim <= 64) launch_attend<f16, 64>(a, S, W, st);
+        else launch_attend<f16, 128>(a, S, W, st);
+    } else {
+        if (a->dim <= 64) launch_attend<bf16, 64>(a, S, W, st);
+        else launch_attend<bf16, 128>(a, S, W, st);
+    }
     READ_HIP(hipGetLastError());
     return 0;
 }

@@ -1,205 +1,507 @@
 // Attention of query rows to the states of their passages, and its gradient (include/artread.h).
 // Included by artread.hip only.
+//
+// The rows of one batch entry that read one key head (rows x the heads that share it) are numbered r, query
+// position major; a workgroup or wave takes a block of them.  All products are 32x32x16 MFMAs:
+//   lane l of A holds row l & 31, of B column l & 31, both 8 consecutive k at 8 * (l >> 5);
+//   lane l of C holds column l & 31 and, in element i, row 8 * (i >> 2) + 4 * (l >> 5) + (i & 3).
+// Scores are computed as S^T = K Q^T, so a lane owns one query row and the softmax of a row is arithmetic
+// inside two lanes.  The weights P^T then lie where the next product wants its B operand, if its k index runs
+// over the keys in C's order; V^T as the A operand follows that order through the transposing LDS read
+// (ds_read_b64_tr_b16: four rows of the tile as four consecutive k).  So no weight ever crosses lanes.
 #pragma once
 #include "artread_common.h"
 
-// One wave per query row (b, t, h).  Scores of 64 keys at a time, one per lane, then the wave turns: a lane
-// owns the columns lane and lane + 64 and adds the 64 weighted value rows.  The running maximum m and sum l
-// of the softmax are kept in 32 bits.
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
 
-__device__ __forceinline__ float wave_max(float x) {
-    for (int o = 32; o; o >>= 1) x = fmaxf(x, __shfl_xor(x, o));
-    return x;
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+template <typename T>
+struct Mma;
+template <>
+struct Mma<f16> {
+    typedef f16 V8 __attribute__((ext_vector_type(8)));
+    static __device__ __forceinline__ f32x16 mul(V8 a, V8 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+    }
+    // Weights of a softmax keep 2^10 beside them while they are f16: the smallest normal f16 is 2^-14, so a weight
+    // of one key among tens of thousands would else lose bits.  Sums carry the same factor, and it cancels.
+    static constexpr float kWeightLog2 = 10.0f;
+};
+template <>
+struct Mma<bf16> {
+    typedef bf16 V8 __attribute__((ext_vector_type(8)));
+    static __device__ __forceinline__ f32x16 mul(V8 a, V8 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    }
+    static constexpr float kWeightLog2 = 0.0f;   // the exponent of f32
+};
+
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// ---- the problem as the kernels see it --------------------------------------------------------------
+struct AttendPlan {
+    int64_t row_count;    // rows x share
+    int64_t row_blocks;   // blocks of rows per (batch entry, key head)
+    int64_t items;        // batch x kv_heads x row_blocks
+    int share;
+    int splits;           // parts the keys of an item are dealt to
+    float c;              // |scale| * log2(e)
+    uint32_t q_and, q_xor;   // scale's sign (and zero) applied to the bits of q: c stays positive
+};
+
+// Deals the tiles of KT keys of a batch entry's passages to `splits` walkers, one after the other; a passage's
+// last tile may be short, the next passage starts a new tile.  Lengths are held 64 passages at a time, one per
+// lane.  All of it is uniform over the wave.
+template <int KT>
+struct Walk {
+    const int32_t* lengths;
+    int passages, len, p, n, j0, step;
+    int held;
+    __device__ __forceinline__ void hold() {
+        const int i = p + (int)(threadIdx.x & 63);
+        int x = len;
+        if (lengths) x = i < passages ? lengths[i] : 0;
+        held = x < 0 ? 0 : (x < len ? x : len);
+    }
+    __device__ __forceinline__ void start(const artread_attend_t& A, int64_t b, int split, int splits) {
+        lengths = A.lengths ? A.lengths + b * A.passages : nullptr;
+        passages = (int)A.passages;
+        len = (int)A.len;
+        p = 0;
+        hold();
+        n = uniform(held);
+        j0 = split * KT;
+        step = splits * KT;
+    }
+    // false: no tile left; else passage p, first key j0, n keys in the passage
+    __device__ __forceinline__ bool settle() {
+        while (j0 >= n) {
+            j0 -= (n + KT - 1) / KT * KT;
+            if (++p >= passages) return false;
+            if ((p & 63) == 0) hold();
+            n = __builtin_amdgcn_readlane(held, p & 63);
+        }
+        return true;
+    }
+    __device__ __forceinline__ void advance() { j0 += step; }
+};
+
+// 16-byte pieces of rows: zero behind `dim` and for rows that are not there
+template <typename T>
+__device__ __forceinline__ typename Mma<T>::V8 load8(const T* p, bool ok) {
+    typename Mma<T>::V8 v = {};
+    if (ok) v = *(const typename Mma<T>::V8*)p;
+    return v;
 }
-__device__ __forceinline__ float wave_sum(float x) {
-    for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o);
-    return x;
+
+// ---- LDS tiles of DP columns --------------------------------------------------------------------------
+// 16-byte chunks of a row are permuted by the row's number.  `key` order: 32 lanes that read the same chunk of 32
+// rows (A operands) meet every bank once; `value` order: the four rows x 64 bytes that half a wave's transposing
+// read touches do.
+template <int DP>
+__device__ __forceinline__ int key_chunk(int row, int chunk) {
+    return DP == 128 ? chunk ^ (row & 15) : chunk ^ ((row >> 1) & 7);
 }
-__device__ __forceinline__ int valid_of(const artread_attend_t& A, int64_t b, int64_t p) {
-    if (!A.lengths) return (int)A.len;
-    const int n = A.lengths[b * A.passages + p];
-    return n < 0 ? 0 : (n < A.len ? n : (int)A.len);
+template <int DP>
+__device__ __forceinline__ int value_chunk(int row, int chunk) {
+    return DP == 128 ? chunk ^ ((row & 3) << 2) : chunk ^ (((row >> 1) & 1) << 2);
+}
+// A operand rows r0 + (l & 31), columns 16 * s + 8 * (l >> 5)..
+template <typename T, int DP>
+__device__ __forceinline__ typename Mma<T>::V8 lds_rows(const T* tile, int row, int s, int half) {
+    return *(const typename Mma<T>::V8*)(tile + row * DP + key_chunk<DP>(row, 2 * s + half) * 8);
+}
+// A operand of the transposed tile: columns 32 * db + (l & 31), k over rows r0 + {4 half + 0..3, 8 + 4 half + 0..3}
+template <typename T, int DP>
+__device__ __forceinline__ typename Mma<T>::V8 lds_columns(const T* tile, int r0, int db, int lane) {
+    union {
+        s16x4 h[2];
+        typename Mma<T>::V8 v;
+    } u;
+    const int i = lane & 15, half = lane >> 5, col = 32 * db + (lane & 16) + 4 * (i & 3);
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+        const int row = r0 + 8 * x + 4 * half + (i >> 2);
+        const T* p = tile + row * DP + value_chunk<DP>(row, col >> 3) * 8 + (col & 7);
+        u.h[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
+    }
+    return u.v;
+}
+
+// ---- softmax over one tile ----------------------------------------------------------------------------
+__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
+
+// scores of NB x 32 keys of one row per lane pair -> weights; m, l are the running maximum (of scores x c) and the
+// lane's own part of the sum, `o` the accumulators that a new maximum rescales
+template <typename T, int NB, int NO>
+__device__ __forceinline__ void softmax_tile(f32x16 (&s)[NB], float c, int left, int half, float& m, float& l,
+                                             f32x16 (&o)[NO]) {
+    if (left < NB * 32) {
+#pragma unroll
+        for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (32 * kb + 8 * (i >> 2) + 4 * half + (i & 3) >= left) s[kb][i] = -INFINITY;
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[kb][i]);
+    top = fmaxf(top, other_half(top)) * c;
+    if (__any(top > m)) {
+        const float m1 = fmaxf(m, top);
+        const float f = m1 == -INFINITY ? 1.0f : exp2f(m - m1);
+        m = m1;
+        l *= f;
+#pragma unroll
+        for (int x = 0; x < NO; ++x)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[x][i] *= f;
+    }
+    const float base = (m == -INFINITY ? 0.0f : m) - Mma<T>::kWeightLog2;
+#pragma unroll
+    for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            s[kb][i] = __builtin_amdgcn_exp2f(fmaf(s[kb][i], c, -base));
+            l += s[kb][i];
+        }
 }
 
 template <typename T>
-__global__ __launch_bounds__(64) void attend_simple_kernel(artread_attend_t A) {
-    __shared__ float qs[128], ps[64];
-    const int lane = threadIdx.x, dim = (int)A.dim;
-    const int64_t total = A.batch * A.rows * A.heads;
-    for (int64_t w = blockIdx.x; w < total; w += gridDim.x) {
-        const int64_t h = w % A.heads, t = w / A.heads % A.rows, b = w / A.heads / A.rows;
-        const int64_t kh = h / (A.heads / A.kv_heads);
-        const T* q = (const T*)A.q + b * A.q_batch + t * A.q_row + h * A.q_head;
-        __syncthreads();
-        for (int d = lane; d < 128; d += 64) qs[d] = d < dim ? to_f32(q[d]) : 0.0f;
-        __syncthreads();
-        float m = -INFINITY, l = 0.0f, o0 = 0.0f, o1 = 0.0f;
-        for (int64_t p = 0; p < A.passages; ++p) {
-            const int n = valid_of(A, b, p);
-            const T* k = (const T*)A.k + b * A.k_batch + p * A.k_passage + kh * A.k_head;
-            const T* v = (const T*)A.v + b * A.v_batch + p * A.v_passage + kh * A.v_head;
-            for (int j0 = 0; j0 < n; j0 += 64) {
-                float s = -INFINITY;
-                if (j0 + lane < n) {
-                    s = 0.0f;
-                    for (int d = 0; d < dim; ++d) s += qs[d] * to_f32(k[(int64_t)(j0 + lane) * A.k_row + d]);
-                    s *= A.scale;
-                }
-                const float m1 = fmaxf(m, wave_max(s));
-                const float m_use = m1 == -INFINITY ? 0.0f : m1;
-                const float e = exp2f((s - m_use) * kLog2e), f = exp2f((m - m_use) * kLog2e);
-                l = l * f + wave_sum(e);
-                m = m1;
-                __syncthreads();
-                ps[lane] = e;
-                __syncthreads();
-                o0 *= f;
-                o1 *= f;
-                const int c = n - j0 < 64 ? n - j0 : 64;
-                for (int j = 0; j < c; ++j) {
-                    const T* vr = v + (int64_t)(j0 + j) * A.v_row;
-                    if (lane < dim) o0 += ps[j] * to_f32(vr[lane]);
-                    if (lane + 64 < dim) o1 += ps[j] * to_f32(vr[lane + 64]);
+__device__ __forceinline__ typename Mma<T>::V8 weights8(const f32x16& s, int ks) {
+    typename Mma<T>::V8 p;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) p[e] = (T)s[8 * ks + e];   // rounded once, to nearest
+    return p;
+}
+
+// ---- what a block of rows leaves ----------------------------------------------------------------------
+// One split: the rows themselves.  Several: accumulators, maximum and sum of every row for the join.
+struct Partials {
+    float* o;      // [splits][all rows][dim]
+    float2* ml;    // [splits][all rows]
+    int64_t rows;  // batch x kv_heads x row_count
+};
+
+template <typename T>
+__device__ __forceinline__ void finish_row4(const artread_attend_t& A, int64_t at, int d, const float* o) {
+    Vec<T, 4> w, e;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+        w.x[x] = (T)o[x];
+        e.x[x] = (T)(o[x] - (float)w.x[x]);
+    }
+    store_vec<T, 4>((T*)A.out + at + d, w);
+    if (A.rest) store_vec<T, 4>((T*)A.rest + at + d, e);
+}
+
+__device__ __forceinline__ float log_sum(float m, float l, float weight_log2) {
+    return l == 0.0f ? -INFINITY : (m - weight_log2) * kLn2 + logf(l);
+}
+
+template <typename T, int DP>
+__device__ __forceinline__ void finish_rows(const artread_attend_t& A, const AttendPlan& P, const Partials& W, int64_t b,
+                                            int64_t kh, int64_t r, int split, int half, float m, float l,
+                                            f32x16 (&o)[DP / 32]) {
+    l += other_half(l);
+    if (r >= P.row_count) return;
+    const int dim = (int)A.dim;
+    if (P.splits > 1) {
+        const int64_t at = split * W.rows + (b * A.kv_heads + kh) * P.row_count + r;
+        if (half == 0) W.ml[at] = make_float2(m, l);
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const int d = 32 * db + 8 * x + 4 * half;
+                if (d < dim) *(float4*)(W.o + at * dim + d) = make_float4(o[db][4 * x], o[db][4 * x + 1], o[db][4 * x + 2], o[db][4 * x + 3]);
+            }
+        return;
+    }
+    const int64_t t = r / P.share, h = kh * P.share + r % P.share;
+    const int64_t at = ((b * A.rows + t) * A.heads + h) * dim;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;   // no key: zeros
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const int d = 32 * db + 8 * x + 4 * half;
+            const float y[4] = {o[db][4 * x] * inv, o[db][4 * x + 1] * inv, o[db][4 * x + 2] * inv, o[db][4 * x + 3] * inv};
+            if (d < dim) finish_row4<T>(A, at, d, y);
+        }
+    if (A.lse && half == 0) A.lse[(b * A.heads + h) * A.rows + t] = log_sum(m, l, Mma<T>::kWeightLog2);
+}
+
+// Joins the splits of a row: 32 lanes of four columns each, G groups of lanes that take every G-th split side by
+// side.  G is 1 for a few splits (eight rows a workgroup) and 8 for many (one row a workgroup: the sum over 256
+// splits is then 32 steps long).  The groups' sums are added in a fixed order.
+template <typename T, int G>
+__global__ __launch_bounds__(256) void attend_join_kernel(artread_attend_t A, AttendPlan P, Partials W) {
+    __shared__ float part[8][32][5];
+    const int lane = threadIdx.x & 31, d = lane * 4, group = threadIdx.x >> 5;
+    const int mine = G == 1 ? 0 : group;
+    for (int64_t R0 = (int64_t)blockIdx.x * (8 / G); R0 < W.rows; R0 += (int64_t)gridDim.x * (8 / G)) {
+        const int64_t R = G == 1 ? R0 + group : R0;
+        const bool there = R < W.rows;
+        float m = -INFINITY, l = 0.0f, o[4] = {0, 0, 0, 0};
+        if (there) {
+            for (int s = lane; s < P.splits; s += 32) m = fmaxf(m, W.ml[s * W.rows + R].x);
+            for (int x = 16; x; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
+            const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll 4
+            for (int s = mine; s < P.splits; s += G) {
+                const float2 ml = W.ml[s * W.rows + R];   // a split without keys: -inf, 0 and zeros
+                const float f = exp2f(ml.x - base);
+                l += f * ml.y;
+                if (d < (int)A.dim) {
+                    const float4 x = *(const float4*)(W.o + (s * W.rows + R) * A.dim + d);
+                    o[0] += f * x.x;
+                    o[1] += f * x.y;
+                    o[2] += f * x.z;
+                    o[3] += f * x.w;
                 }
             }
         }
-        const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
-        T* out = (T*)A.out + w * dim;
-        if (lane < dim) out[lane] = from_f32<T>(o0 * inv);
-        if (lane + 64 < dim) out[lane + 64] = from_f32<T>(o1 * inv);
-        if (A.rest) {
-            T* rest = (T*)A.rest + w * dim;
-            if (lane < dim) rest[lane] = from_f32<T>(o0 * inv - to_f32(from_f32<T>(o0 * inv)));
-            if (lane + 64 < dim) rest[lane + 64] = from_f32<T>(o1 * inv - to_f32(from_f32<T>(o1 * inv)));
+        if (G > 1) {
+            part[group][lane][0] = l;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) part[group][lane][1 + x] = o[x];
+            __syncthreads();
+            l = o[0] = o[1] = o[2] = o[3] = 0.0f;
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                l += part[g][lane][0];
+#pragma unroll
+                for (int x = 0; x < 4; ++x) o[x] += part[g][lane][1 + x];
+            }
+            __syncthreads();
         }
-        if (A.lse && lane == 0) A.lse[(b * A.heads + h) * A.rows + t] = l == 0.0f ? -INFINITY : m + logf(l);
+        if (!there || (G > 1 && group != 0)) continue;
+        const int64_t r = R % P.row_count, bk = R / P.row_count, kh = bk % A.kv_heads, b = bk / A.kv_heads;
+        const int64_t t = r / P.share, h = kh * P.share + r % P.share;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) o[x] *= inv;
+        if (d < (int)A.dim) finish_row4<T>(A, ((b * A.rows + t) * A.heads + h) * A.dim, d, o);
+        if (A.lse && lane == 0) A.lse[(b * A.heads + h) * A.rows + t] = log_sum(m, l, Mma<T>::kWeightLog2);
     }
 }
 
-// delta[b, h, t] = grad_out . out, and grad_q: one wave per query row
-template <typename T>
-__global__ __launch_bounds__(64) void attend_grad_q_simple_kernel(artread_attend_t A, artread_attend_grads_t G,
-                                                                  float* __restrict__ delta) {
-    __shared__ float qs[128], gs[128], ps[64];
-    const int lane = threadIdx.x, dim = (int)A.dim;
-    const int64_t total = A.batch * A.rows * A.heads;
-    for (int64_t w = blockIdx.x; w < total; w += gridDim.x) {
-        const int64_t h = w % A.heads, t = w / A.heads % A.rows, b = w / A.heads / A.rows;
-        const int64_t kh = h / (A.heads / A.kv_heads);
-        const T* q = (const T*)A.q + b * A.q_batch + t * A.q_row + h * A.q_head;
-        const T* g = (const T*)G.grad_out + b * G.g_batch + t * G.g_row + h * G.g_head;
-        const T* out = (const T*)A.out + w * dim;
-        __syncthreads();
-        float dl = 0.0f;
-        for (int d = lane; d < 128; d += 64) {
-            qs[d] = d < dim ? to_f32(q[d]) : 0.0f;
-            gs[d] = d < dim ? to_f32(g[d]) : 0.0f;
-            if (d < dim) dl += gs[d] * (to_f32(out[d]) + (A.rest ? to_f32(((const T*)A.rest + w * dim)[d]) : 0.0f));
-        }
-        dl = wave_sum(dl);
-        const int64_t at = (b * A.heads + h) * A.rows + t;
-        if (lane == 0) delta[at] = dl;
-        const float lse = A.lse[at];
-        __syncthreads();
-        float o0 = 0.0f, o1 = 0.0f;
-        for (int64_t p = 0; p < A.passages; ++p) {
-            const int n = valid_of(A, b, p);
-            const T* k = (const T*)A.k + b * A.k_batch + p * A.k_passage + kh * A.k_head;
-            const T* v = (const T*)A.v + b * A.v_batch + p * A.v_passage + kh * A.v_head;
-            for (int j0 = 0; j0 < n; j0 += 64) {
-                float ds = 0.0f;
-                if (j0 + lane < n) {
-                    float s = 0.0f, dp = 0.0f;
-                    for (int d = 0; d < dim; ++d) {
-                        s += qs[d] * to_f32(k[(int64_t)(j0 + lane) * A.k_row + d]);
-                        dp += gs[d] * to_f32(v[(int64_t)(j0 + lane) * A.v_row + d]);
-                    }
-                    ds = exp2f((s * A.scale - lse) * kLog2e) * (dp - dl);
-                }
-                __syncthreads();
-                ps[lane] = ds;
-                __syncthreads();
-                const int c = n - j0 < 64 ? n - j0 : 64;
-                for (int j = 0; j < c; ++j) {
-                    const T* kr = k + (int64_t)(j0 + j) * A.k_row;
-                    if (lane < dim) o0 += ps[j] * to_f32(kr[lane]);
-                    if (lane + 64 < dim) o1 += ps[j] * to_f32(kr[lane + 64]);
-                }
-            }
-        }
-        T* gq = (T*)G.grad_q + w * dim;
-        if (lane < dim) gq[lane] = from_f32<T>(o0 * A.scale);
-        if (lane + 64 < dim) gq[lane + 64] = from_f32<T>(o1 * A.scale);
+// Q^T operand of a row block: row r, all columns, in registers for the whole walk
+template <typename T, int DP>
+__device__ __forceinline__ void load_q(const artread_attend_t& A, const AttendPlan& P, const T* base, int64_t s_batch,
+                                       int64_t s_row, int64_t s_head, int64_t b, int64_t kh, int64_t r, int half,
+                                       uint32_t q_and, uint32_t q_xor, typename Mma<T>::V8 (&q)[DP / 16]) {
+    const int64_t t = r / P.share, h = kh * P.share + r % P.share;
+    const T* src = base + b * s_batch + t * s_row + h * s_head;
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s) {
+        const int d = 16 * s + 8 * half;
+        union {
+            typename Mma<T>::V8 v;
+            uint32_t u[4];
+        } x;
+        x.v = load8<T>(src + d, r < P.row_count && d < (int)A.dim);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x.u[e] = (x.u[e] & q_and) ^ q_xor;
+        q[s] = x.v;
     }
 }
 
-// grad_k and grad_v: one wave per key (b, p, j, kh) over all rows of the heads that share it
-template <typename T>
-__global__ __launch_bounds__(64) void attend_grad_kv_simple_kernel(artread_attend_t A, artread_attend_grads_t G,
-                                                                   const float* __restrict__ delta) {
-    __shared__ float ks[128], vs[128], ps[64], es[64];
-    const int lane = threadIdx.x, dim = (int)A.dim;
-    const int64_t share = A.heads / A.kv_heads, rows = A.rows * share;
-    const int64_t total = A.batch * A.passages * A.len * A.kv_heads;
-    for (int64_t w = blockIdx.x; w < total; w += gridDim.x) {
-        const int64_t kh = w % A.kv_heads, j = w / A.kv_heads % A.len, p = w / A.kv_heads / A.len % A.passages;
-        const int64_t b = w / A.kv_heads / A.len / A.passages;
-        T* gk = (T*)G.grad_k + w * dim;
-        T* gv = (T*)G.grad_v + w * dim;
-        float k0 = 0.0f, k1 = 0.0f, v0 = 0.0f, v1 = 0.0f;
-        if (j < valid_of(A, b, p)) {
-            const T* k = (const T*)A.k + b * A.k_batch + p * A.k_passage + j * A.k_row + kh * A.k_head;
-            const T* v = (const T*)A.v + b * A.v_batch + p * A.v_passage + j * A.v_row + kh * A.v_head;
-            __syncthreads();
-            for (int d = lane; d < 128; d += 64) {
-                ks[d] = d < dim ? to_f32(k[d]) : 0.0f;
-                vs[d] = d < dim ? to_f32(v[d]) : 0.0f;
+// ---- few rows: one wave walks its tiles alone ----------------------------------------------------------
+// QB x 32 rows per wave, 32 keys per tile.  Every key and value is read once, so this is bound by HBM: K goes
+// straight from memory into the A operand, V through a tile of LDS of the wave's own for the transposing read,
+// the next tile's loads are in flight while this one is worked on, and no wave waits for another.
+template <typename T, int DP, int QB>
+__global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void attend_stream_kernel(artread_attend_t A, AttendPlan P, Partials W) {
+    __shared__ __attribute__((aligned(16))) T tiles[4][32 * DP];
+    typedef typename Mma<T>::V8 V8;
+    const int lane = threadIdx.x & 63, half = lane >> 5, wave = uniform(threadIdx.x >> 6);
+    T* tile = tiles[wave];
+    const int dim = (int)A.dim;
+    const int64_t waves = P.items * P.splits;
+    for (int64_t w = (int64_t)blockIdx.x * 4 + wave; w < waves; w += (int64_t)gridDim.x * 4) {
+        const int split = (int)(w % P.splits);
+        const int64_t item = w / P.splits, rb = item % P.row_blocks, bk = item / P.row_blocks;
+        const int64_t kh = bk % A.kv_heads, b = bk / A.kv_heads, r0 = rb * 32 * QB + (lane & 31);
+        V8 q[QB][DP / 16];
+        f32x16 o[QB][DP / 32];
+        float m[QB], l[QB];
+#pragma unroll
+        for (int x = 0; x < QB; ++x) {
+            load_q<T, DP>(A, P, (const T*)A.q, A.q_batch, A.q_row, A.q_head, b, kh, r0 + 32 * x, half, P.q_and, P.q_xor, q[x]);
+            m[x] = -INFINITY;
+            l[x] = 0.0f;
+#pragma unroll
+            for (int db = 0; db < DP / 32; ++db) o[x][db] = f32x16{};
+        }
+        const T* kbase = (const T*)A.k + b * A.k_batch + kh * A.k_head + (int64_t)(lane & 31) * A.k_row + 8 * half;
+        // V: 8 or 16 lanes per row
+        constexpr int CH = DP / 8, VR = 64 / CH, VN = 32 / VR;
+        const int vrow = lane / CH, vchunk = lane % CH;
+        const T* vbase = (const T*)A.v + b * A.v_batch + kh * A.v_head + (int64_t)vrow * A.v_row + 8 * vchunk;
+        V8 kr[DP / 16], vr[VN];
+        Walk<32> walk;
+        walk.start(A, b, split, P.splits);
+        auto load = [&]() {
+            const int left = walk.n - walk.j0;
+            const T* kp = kbase + walk.p * A.k_passage + walk.j0 * A.k_row;
+            const T* vp = vbase + walk.p * A.v_passage + walk.j0 * A.v_row;
+#pragma unroll
+            for (int s = 0; s < DP / 16; ++s) kr[s] = load8<T>(kp + 16 * s, (lane & 31) < left && 16 * s + 8 * half < dim);
+#pragma unroll
+            for (int x = 0; x < VN; ++x) vr[x] = load8<T>(vp + (int64_t)x * VR * A.v_row, vrow + x * VR < left && 8 * vchunk < dim);
+        };
+        bool more = walk.settle();
+        if (more) load();
+        while (more) {
+            const int left = walk.n - walk.j0;
+            f32x16 s[QB][1];
+#pragma unroll
+            for (int x = 0; x < QB; ++x) s[x][0] = f32x16{};
+#pragma unroll
+            for (int k = 0; k < DP / 16; ++k)
+#pragma unroll
+                for (int x = 0; x < QB; ++x) s[x][0] = Mma<T>::mul(kr[k], q[x][k], s[x][0]);
+#pragma unroll
+            for (int x = 0; x < VN; ++x) {
+                const int row = vrow + x * VR;
+                *(V8*)(tile + row * DP + value_chunk<DP>(row, vchunk) * 8) = vr[x];
             }
-            __syncthreads();
-            for (int64_t r0 = 0; r0 < rows; r0 += 64) {
-                float e = 0.0f, ds = 0.0f;
-                const int64_t r = r0 + lane;
-                if (r < rows) {
-                    const int64_t t = r / share, h = kh * share + r % share;
-                    const T* q = (const T*)A.q + b * A.q_batch + t * A.q_row + h * A.q_head;
-                    const T* g = (const T*)G.grad_out + b * G.g_batch + t * G.g_row + h * G.g_head;
-                    float s = 0.0f, dp = 0.0f;
-                    for (int d = 0; d < dim; ++d) {
-                        s += ks[d] * to_f32(q[d]);
-                        dp += vs[d] * to_f32(g[d]);
-                    }
-                    const int64_t at = (b * A.heads + h) * A.rows + t;
-                    e = exp2f((s * A.scale - A.lse[at]) * kLog2e);
-                    ds = e * (dp - delta[at]);
-                }
-                __syncthreads();
-                ps[lane] = e;
-                es[lane] = ds;
-                __syncthreads();
-                const int c = rows - r0 < 64 ? (int)(rows - r0) : 64;
-                for (int i = 0; i < c; ++i) {
-                    const int64_t t = (r0 + i) / share, h = kh * share + (r0 + i) % share;
-                    const T* q = (const T*)A.q + b * A.q_batch + t * A.q_row + h * A.q_head;
-                    const T* g = (const T*)G.grad_out + b * G.g_batch + t * G.g_row + h * G.g_head;
-                    if (lane < dim) {
-                        k0 += es[i] * to_f32(q[lane]);
-                        v0 += ps[i] * to_f32(g[lane]);
-                    }
-                    if (lane + 64 < dim) {
-                        k1 += es[i] * to_f32(q[lane + 64]);
-                        v1 += ps[i] * to_f32(g[lane + 64]);
-                    }
+            walk.advance();
+            more = walk.settle();
+            if (more) load();
+#pragma unroll
+            for (int x = 0; x < QB; ++x) softmax_tile<T, 1, DP / 32>(s[x], P.c, left, half, m[x], l[x], o[x]);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // the tile is written: LDS keeps a wave's order
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                V8 pw[QB];
+#pragma unroll
+                for (int x = 0; x < QB; ++x) pw[x] = weights8<T>(s[x][0], ks);
+#pragma unroll
+                for (int db = 0; db < DP / 32; ++db) {
+                    const V8 vt = lds_columns<T, DP>(tile, 16 * ks, db, lane);
+#pragma unroll
+                    for (int x = 0; x < QB; ++x) o[x][db] = Mma<T>::mul(vt, pw[x], o[x][db]);
                 }
             }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
-        if (lane < dim) {
-            gk[lane] = from_f32<T>(k0 * A.scale);
-            gv[lane] = from_f32<T>(v0);
+#pragma unroll
+        for (int x = 0; x < QB; ++x) finish_rows<T, DP>(A, P, W, b, kh, r0 + 32 * x, split, half, m[x], l[x], o[x]);
+    }
+}
+
+// ---- many rows: four waves share the tiles --------------------------------------------------------------
+// 128 * QB rows per workgroup, 64 keys per tile; K and V tiles are double-buffered in LDS, one barrier per tile.
+// Workgroups of one (batch entry, key head) sit on one XCD, whose L2 then serves its states.
+__device__ __forceinline__ int64_t xcd_item(int64_t id, int64_t items) {
+    const int64_t per = (items + 7) / 8;
+    return (id & 7) * per + (id >> 3);
+}
+
+template <typename T, int DP, int QB>
+__global__ __launch_bounds__(256, QB == 1 ? 2 : 1) void attend_tile_kernel(artread_attend_t A, AttendPlan P, Partials W) {
+    __shared__ __attribute__((aligned(16))) T ktile[2][64 * DP];
+    __shared__ __attribute__((aligned(16))) T vtile[2][64 * DP];
+    typedef typename Mma<T>::V8 V8;
+    const int lane = threadIdx.x & 63, half = lane >> 5, wave = uniform(threadIdx.x >> 6);
+    const int dim = (int)A.dim;
+    const int64_t total = P.items * P.splits;
+    for (int64_t id = blockIdx.x; id < (total + 7) / 8 * 8; id += gridDim.x) {
+        const int64_t w = xcd_item(id, total);
+        if (w >= total) continue;
+        const int64_t rb = w % P.row_blocks, rest = w / P.row_blocks;
+        const int split = (int)(rest % P.splits);
+        const int64_t bk = rest / P.splits, kh = bk % A.kv_heads, b = bk / A.kv_heads;
+        const int64_t r0 = (rb * 4 + wave) * 32 * QB + (lane & 31);
+        V8 q[QB][DP / 16];
+        f32x16 o[QB][DP / 32];
+        float m[QB], l[QB];
+#pragma unroll
+        for (int x = 0; x < QB; ++x) {
+            load_q<T, DP>(A, P, (const T*)A.q, A.q_batch, A.q_row, A.q_head, b, kh, r0 + 32 * x, half, P.q_and, P.q_xor, q[x]);
+            m[x] = -INFINITY;
+            l[x] = 0.0f;
+#pragma unroll
+            for (int db = 0; db < DP / 32; ++db) o[x][db] = f32x16{};
         }
-        if (lane + 64 < dim) {
-            gk[lane + 64] = from_f32<T>(k1 * A.scale);
-            gv[lane + 64] = from_f32<T>(v1);
+        constexpr int CH = DP / 8, TR = 256 / CH, TN = 64 / TR;   // threads per row, rows side by side, steps
+        const int trow = threadIdx.x / CH, tchunk = threadIdx.x % CH;
+        const T* kbase = (const T*)A.k + b * A.k_batch + kh * A.k_head + (int64_t)trow * A.k_row + 8 * tchunk;
+        const T* vbase = (const T*)A.v + b * A.v_batch + kh * A.v_head + (int64_t)trow * A.v_row + 8 * tchunk;
+        V8 kr[TN], vr[TN];
+        Walk<64> walk;
+        walk.start(A, b, split, P.splits);
+        auto load = [&]() {
+            const int left = walk.n - walk.j0;
+            const T* kp = kbase + walk.p * A.k_passage + walk.j0 * A.k_row;
+            const T* vp = vbase + walk.p * A.v_passage + walk.j0 * A.v_row;
+#pragma unroll
+            for (int x = 0; x < TN; ++x) {
+                const bool ok = trow + x * TR < left && 8 * tchunk < dim;
+                kr[x] = load8<T>(kp + (int64_t)x * TR * A.k_row, ok);
+                vr[x] = load8<T>(vp + (int64_t)x * TR * A.v_row, ok);
+            }
+        };
+        auto put = [&](int buf) {
+#pragma unroll
+            for (int x = 0; x < TN; ++x) {
+                const int row = trow + x * TR;
+                *(V8*)(ktile[buf] + row * DP + key_chunk<DP>(row, tchunk) * 8) = kr[x];
+                *(V8*)(vtile[buf] + row * DP + value_chunk<DP>(row, tchunk) * 8) = vr[x];
+            }
+        };
+        bool more = walk.settle();
+        if (more) {
+            load();
+            put(0);
         }
+        __syncthreads();
+        int buf = 0;
+        while (more) {
+            const int left = walk.n - walk.j0;
+            walk.advance();
+            more = walk.settle();
+            if (more) load();
+            const T* kt = ktile[buf];
+            const T* vt = vtile[buf];
+            f32x16 s[QB][2];
+#pragma unroll
+            for (int x = 0; x < QB; ++x) s[x][0] = s[x][1] = f32x16{};
+#pragma unroll
+            for (int k = 0; k < DP / 16; ++k)
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb) {
+                    const V8 a = lds_rows<T, DP>(kt, 32 * kb + (lane & 31), k, half);
+#pragma unroll
+                    for (int x = 0; x < QB; ++x) s[x][kb] = Mma<T>::mul(a, q[x][k], s[x][kb]);
+                }
+#pragma unroll
+            for (int x = 0; x < QB; ++x) softmax_tile<T, 2, DP / 32>(s[x], P.c, left, half, m[x], l[x], o[x]);
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) {
+                V8 pw[QB];
+#pragma unroll
+                for (int x = 0; x < QB; ++x) pw[x] = weights8<T>(s[x][ks >> 1], ks & 1);
+#pragma unroll
+                for (int db = 0; db < DP / 32; ++db) {
+                    const V8 a = lds_columns<T, DP>(vt, 16 * ks, db, lane);
+#pragma unroll
+                    for (int x = 0; x < QB; ++x) o[x][db] = Mma<T>::mul(a, pw[x], o[x][db]);
+                }
+            }
+            if (more) put(buf ^ 1);
+            __syncthreads();
+            buf ^= 1;
+        }
+#pragma unroll
+        for (int x = 0; x < QB; ++x) finish_rows<T, DP>(A, P, W, b, kh, r0 + 32 * x, split, half, m[x], l[x], o[x]);
     }
 }
