@@ -322,8 +322,9 @@ struct AttendShape {
         return plan.splits > 1 ? round_up(plan.splits * rows * a->dim * 4, 256) + round_up(plan.splits * rows * 8, 256) : 0;
     }
 };
-static void plan_scale(AttendPlan* P, float scale) {
+static void plan_scale(AttendPlan* P, float scale, int dtype) {
     P->c = scale == 0.0f ? 1.0f : fabsf(scale) * kLog2e;
+    P->unweight = dtype == ARTREAD_F16 ? exp2f(-Mma<f16>::kWeightLog2) : 1.0f;
     P->q_and = scale == 0.0f ? 0u : 0xffffffffu;
     P->q_xor = scale < 0.0f ? 0x80008000u : 0u;
 }
@@ -341,7 +342,7 @@ static AttendShape attend_shape(const artread_attend_t* a) {
     int64_t want = ((S.stream ? 4096 : 512) + P.items - 1) / P.items, most = tiles / (S.stream ? 2 : 4);
     want = want < most ? want : most;
     P.splits = (int)(want < 1 ? 1 : (want < 256 ? want : 256));
-    plan_scale(&P, a->scale);
+    plan_scale(&P, a->scale, a->dtype);
     return S;
 }
 
@@ -390,10 +391,76 @@ extern "C" int artread_attend(int device, const artread_attend_t* a, void* works
     return 0;
 }
 
+// How a gradient call runs: a walk over the keys for dQ and one over the rows for dK and dV, either of them split
+// where its workgroups would not fill the chip.
+struct GradShape {
+    bool narrow;           // dQ: one wave of 32 rows per workgroup, else four
+    AttendPlan q, kv;
+    int64_t all_q, all_k;  // elements
+    int64_t stats, part;   // byte offsets; the two walks run one after the other and share their parts
+    int64_t total;
+};
+static GradShape grad_shape(const artread_attend_t* a) {
+    GradShape S;
+    AttendPlan& Q = S.q;
+    Q.share = (int)(a->heads / a->kv_heads);
+    Q.row_count = a->rows * Q.share;
+    plan_scale(&Q, a->scale, a->dtype);
+    S.kv = Q;
+    S.narrow = Q.row_count <= 64;
+    const int block = S.narrow ? 32 : 128, keys = S.narrow ? 32 : 64;
+    Q.row_blocks = (Q.row_count + block - 1) / block;
+    Q.items = a->batch * a->kv_heads * Q.row_blocks;
+    int64_t want = ((S.narrow ? 2048 : 512) + Q.items - 1) / Q.items;
+    int64_t most = a->passages * ((a->len + keys - 1) / keys) / 4;
+    want = want < most ? want : most;
+    Q.splits = (int)(want < 1 ? 1 : (want < 64 ? want : 64));
+    AttendPlan& K = S.kv;
+    K.row_blocks = 1;
+    K.items = a->batch * a->passages * ((a->len + 127) / 128) * a->kv_heads;
+    want = (512 + K.items - 1) / K.items;
+    most = (K.row_count + 31) / 32 / 4;
+    want = want < most ? want : most;
+    K.splits = (int)(want < 1 ? 1 : (want < 64 ? want : 64));
+    S.all_q = a->batch * a->rows * a->heads * a->dim;
+    S.all_k = a->batch * a->passages * a->len * a->kv_heads * a->dim;
+    S.stats = 0;
+    S.part = round_up(a->batch * a->kv_heads * Q.row_count * (int64_t)sizeof(RowStat), 256);
+    const int64_t pq = Q.splits > 1 ? Q.splits * S.all_q * 4 : 0, pk = K.splits > 1 ? K.splits * 2 * S.all_k * 4 : 0;
+    S.total = S.part + round_up(pq > pk ? pq : pk, 256);
+    return S;
+}
+
 extern "C" int64_t artread_attend_grad_workspace(const artread_attend_t* a) {
     const int rc = check_attend(a);
-    if (rc) return rc;
-    return round_up(a->batch * a->heads * a->rows * 4, 256);
+    return rc ? rc : grad_shape(a).total;
+}
+
+template <typename T>
+static void launch_sum(const float* part, int64_t stride, int splits, void* out, int64_t n, hipStream_t st) {
+    hipLaunchKernelGGL((attend_sum_kernel<T>), dim3(grid_of((n + 1023) / 1024)), dim3(256), 0, st, part, stride, splits,
+                       (T*)out, n);
+}
+
+template <typename T, int DP>
+static void launch_attend_grad(const artread_attend_t* a, const artread_attend_grads_t* g, const GradShape& S, void* ws,
+                               hipStream_t st) {
+    RowStat* stats = (RowStat*)((char*)ws + S.stats);
+    float* part = (float*)((char*)ws + S.part);
+    const int64_t rows = a->batch * a->kv_heads * S.q.row_count;
+    hipLaunchKernelGGL((attend_delta_kernel<T>), dim3(grid_of((rows + 15) / 16)), dim3(256), 0, st, *a, *g, S.q, rows, stats);
+    const dim3 gq(grid_of(round_up(S.q.items * S.q.splits, 8)));
+    if (S.narrow)
+        hipLaunchKernelGGL((attend_grad_q_kernel<T, DP, 1, 1>), gq, dim3(64), 0, st, *a, *g, S.q, stats, part);
+    else
+        hipLaunchKernelGGL((attend_grad_q_kernel<T, DP, 4, 2>), gq, dim3(256), 0, st, *a, *g, S.q, stats, part);
+    if (S.q.splits > 1) launch_sum<T>(part, S.all_q, S.q.splits, g->grad_q, S.all_q, st);
+    hipLaunchKernelGGL((attend_grad_kv_kernel<T, DP>), dim3(grid_of(S.kv.items * S.kv.splits)), dim3(256), 0, st, *a, *g,
+                       S.kv, stats, part);
+    if (S.kv.splits > 1) {
+        launch_sum<T>(part, 2 * S.all_k, S.kv.splits, g->grad_k, S.all_k, st);
+        launch_sum<T>(part + S.all_k, 2 * S.all_k, S.kv.splits, g->grad_v, S.all_k, st);
+    }
 }
 
 extern "C" int artread_attend_grad(int device, const artread_attend_t* a, const artread_attend_grads_t* gr,
@@ -407,21 +474,18 @@ extern "C" int artread_attend_grad(int device, const artread_attend_t* a, const 
                  "strides must be multiples of 8 in [0, 2^31)");
     READ_ARG(aligned(gr->grad_out, 16) && aligned(gr->grad_q, 16) && aligned(gr->grad_k, 16) && aligned(gr->grad_v, 16),
              "gradients must be 16-byte aligned");
-    const int64_t need = artread_attend_grad_workspace(a);
-    READ_ARG(workspace && aligned(workspace, 16) && workspace_bytes >= need,
-             "workspace of %lld bytes, %lld needed, 16-byte aligned", (long long)workspace_bytes, (long long)need);
+    const GradShape S = grad_shape(a);
+    READ_ARG(workspace && aligned(workspace, 16) && workspace_bytes >= S.total,
+             "workspace of %lld bytes, %lld needed, 16-byte aligned", (long long)workspace_bytes, (long long)S.total);
     ReadDeviceGuard g(device);
     READ_HIP(g.err);
     hipStream_t st = (hipStream_t)stream;
-    float* delta = (float*)workspace;
-    const dim3 gq(grid_of(a->batch * a->rows * a->heads));
-    const dim3 gk(grid_of(a->batch * a->passages * a->len * a->kv_heads));
     if (a->dtype == ARTREAD_F16) {
-        hipLaunchKernelGGL(attend_grad_q_simple_kernel<f16>, gq, dim3(64), 0, st, *a, *gr, delta);
-        hipLaunchKernelGGL(attend_grad_kv_simple_kernel<f16>, gk, dim3(64), 0, st, *a, *gr, delta);
+        if (a->dim <= 64) launch_attend_grad<f16, 64>(a, gr, S, workspace, st);
+        else launch_attend_grad<f16, 128>(a, gr, S, workspace, st);
     } else {
-        hipLaunchKernelGGL(attend_grad_q_simple_kernel<bf16>, gq, dim3(64), 0, st, *a, *gr, delta);
-        hipLaunchKernelGGL(attend_grad_kv_simple_kernel<bf16>, gk, dim3(64), 0, st, *a, *gr, delta);
+        if (a->dim <= 64) launch_attend_grad<bf16, 64>(a, gr, S, workspace, st);
+        else launch_attend_grad<bf16, 128>(a, gr, S, workspace, st);
     }
     READ_HIP(hipGetLastError());
     return 0;

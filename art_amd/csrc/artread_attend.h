@@ -49,6 +49,7 @@ struct AttendPlan {
     int share;
     int splits;           // parts the keys of an item are dealt to
     float c;              // |scale| * log2(e)
+    float unweight;       // takes back the factor that f16 weights carry
     uint32_t q_and, q_xor;   // scale's sign (and zero) applied to the bits of q: c stays positive
 };
 
@@ -98,21 +99,16 @@ __device__ __forceinline__ typename Mma<T>::V8 load8(const T* p, bool ok) {
 }
 
 // ---- LDS tiles of DP columns --------------------------------------------------------------------------
-// 16-byte chunks of a row are permuted by the row's number.  `key` order: 32 lanes that read the same chunk of 32
-// rows (A operands) meet every bank once; `value` order: the four rows x 64 bytes that half a wave's transposing
-// read touches do.
+// 16-byte chunks of a row are permuted by the row's number, so that both ways of reading meet every bank once: 16
+// rows of one chunk (A operands of rows), and the four rows x 64 bytes of half a wave's transposing read.
 template <int DP>
-__device__ __forceinline__ int key_chunk(int row, int chunk) {
-    return DP == 128 ? chunk ^ (row & 15) : chunk ^ ((row >> 1) & 7);
-}
-template <int DP>
-__device__ __forceinline__ int value_chunk(int row, int chunk) {
-    return DP == 128 ? chunk ^ ((row & 3) << 2) : chunk ^ (((row >> 1) & 1) << 2);
+__device__ __forceinline__ int tile_chunk(int row, int chunk) {
+    return DP == 128 ? chunk ^ (((row & 3) << 2) | ((row >> 2) & 3)) : chunk ^ ((((row >> 1) & 1) << 2) | ((row >> 2) & 3));
 }
 // A operand rows r0 + (l & 31), columns 16 * s + 8 * (l >> 5)..
 template <typename T, int DP>
 __device__ __forceinline__ typename Mma<T>::V8 lds_rows(const T* tile, int row, int s, int half) {
-    return *(const typename Mma<T>::V8*)(tile + row * DP + key_chunk<DP>(row, 2 * s + half) * 8);
+    return *(const typename Mma<T>::V8*)(tile + row * DP + tile_chunk<DP>(row, 2 * s + half) * 8);
 }
 // A operand of the transposed tile: columns 32 * db + (l & 31), k over rows r0 + {4 half + 0..3, 8 + 4 half + 0..3}
 template <typename T, int DP>
@@ -125,7 +121,7 @@ __device__ __forceinline__ typename Mma<T>::V8 lds_columns(const T* tile, int r0
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
         const int row = r0 + 8 * x + 4 * half + (i >> 2);
-        const T* p = tile + row * DP + value_chunk<DP>(row, col >> 3) * 8 + (col & 7);
+        const T* p = tile + row * DP + tile_chunk<DP>(row, col >> 3) * 8 + (col & 7);
         u.h[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
     }
     return u.v;
@@ -371,7 +367,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void attend_stream_kernel(ar
 #pragma unroll
             for (int x = 0; x < VN; ++x) {
                 const int row = vrow + x * VR;
-                *(V8*)(tile + row * DP + value_chunk<DP>(row, vchunk) * 8) = vr[x];
+                *(V8*)(tile + row * DP + tile_chunk<DP>(row, vchunk) * 8) = vr[x];
             }
             walk.advance();
             more = walk.settle();
@@ -454,8 +450,8 @@ __global__ __launch_bounds__(256, QB == 1 ? 2 : 1) void attend_tile_kernel(artre
 #pragma unroll
             for (int x = 0; x < TN; ++x) {
                 const int row = trow + x * TR;
-                *(V8*)(ktile[buf] + row * DP + key_chunk<DP>(row, tchunk) * 8) = kr[x];
-                *(V8*)(vtile[buf] + row * DP + value_chunk<DP>(row, tchunk) * 8) = vr[x];
+                *(V8*)(ktile[buf] + row * DP + tile_chunk<DP>(row, tchunk) * 8) = kr[x];
+                *(V8*)(vtile[buf] + row * DP + tile_chunk<DP>(row, tchunk) * 8) = vr[x];
             }
         };
         bool more = walk.settle();
