@@ -328,10 +328,14 @@ static void plan_scale(AttendPlan* P, float scale, int dtype) {
     P->q_and = scale == 0.0f ? 0u : 0xffffffffu;
     P->q_xor = scale < 0.0f ? 0x80008000u : 0u;
 }
+static void plan_share(AttendPlan* P, const artread_attend_t* a) {
+    P->share = (uint32_t)(a->heads / a->kv_heads);
+    P->inv_share = P->share == 1 ? 0xffffffffu : (uint32_t)(((uint64_t)1 << 32) / P->share);
+}
 static AttendShape attend_shape(const artread_attend_t* a) {
     AttendShape S;
     AttendPlan& P = S.plan;
-    P.share = (int)(a->heads / a->kv_heads);
+    plan_share(&P, a);
     P.row_count = a->rows * P.share;
     S.stream = P.row_count <= (a->dim <= 64 ? 64 : 32);
     S.qb = S.stream && P.row_count > 32 ? 2 : 1;
@@ -403,9 +407,10 @@ struct GradShape {
 static GradShape grad_shape(const artread_attend_t* a) {
     GradShape S;
     AttendPlan& Q = S.q;
-    Q.share = (int)(a->heads / a->kv_heads);
+    plan_share(&Q, a);
     Q.row_count = a->rows * Q.share;
     plan_scale(&Q, a->scale, a->dtype);
+    Q.pad_rows = round_up(Q.row_count, 32);
     S.kv = Q;
     S.narrow = Q.row_count <= 64;
     const int block = S.narrow ? 32 : 128, keys = S.narrow ? 32 : 64;
@@ -417,6 +422,7 @@ static GradShape grad_shape(const artread_attend_t* a) {
     Q.splits = (int)(want < 1 ? 1 : (want < 64 ? want : 64));
     AttendPlan& K = S.kv;
     K.row_blocks = 1;
+    K.by_head = K.row_count > 64;
     K.items = a->batch * a->passages * ((a->len + 127) / 128) * a->kv_heads;
     want = (512 + K.items - 1) / K.items;
     most = (K.row_count + 31) / 32 / 4;
@@ -425,7 +431,7 @@ static GradShape grad_shape(const artread_attend_t* a) {
     S.all_q = a->batch * a->rows * a->heads * a->dim;
     S.all_k = a->batch * a->passages * a->len * a->kv_heads * a->dim;
     S.stats = 0;
-    S.part = round_up(a->batch * a->kv_heads * Q.row_count * (int64_t)sizeof(RowStat), 256);
+    S.part = round_up(a->batch * a->kv_heads * Q.pad_rows * (int64_t)sizeof(RowStat), 256);
     const int64_t pq = Q.splits > 1 ? Q.splits * S.all_q * 4 : 0, pk = K.splits > 1 ? K.splits * 2 * S.all_k * 4 : 0;
     S.total = S.part + round_up(pq > pk ? pq : pk, 256);
     return S;
@@ -447,7 +453,7 @@ static void launch_attend_grad(const artread_attend_t* a, const artread_attend_g
                                hipStream_t st) {
     RowStat* stats = (RowStat*)((char*)ws + S.stats);
     float* part = (float*)((char*)ws + S.part);
-    const int64_t rows = a->batch * a->kv_heads * S.q.row_count;
+    const int64_t rows = a->batch * a->kv_heads * S.q.pad_rows;
     hipLaunchKernelGGL((attend_delta_kernel<T>), dim3(grid_of((rows + 15) / 16)), dim3(256), 0, st, *a, *g, S.q, rows, stats);
     const dim3 gq(grid_of(round_up(S.q.items * S.q.splits, 8)));
     if (S.narrow)
@@ -455,7 +461,7 @@ static void launch_attend_grad(const artread_attend_t* a, const artread_attend_g
     else
         hipLaunchKernelGGL((attend_grad_q_kernel<T, DP, 4, 2>), gq, dim3(256), 0, st, *a, *g, S.q, stats, part);
     if (S.q.splits > 1) launch_sum<T>(part, S.all_q, S.q.splits, g->grad_q, S.all_q, st);
-    hipLaunchKernelGGL((attend_grad_kv_kernel<T, DP>), dim3(grid_of(S.kv.items * S.kv.splits)), dim3(256), 0, st, *a, *g,
+    hipLaunchKernelGGL((attend_grad_kv_kernel<T, DP>), dim3(grid_of(round_up(S.kv.items * S.kv.splits, 8))), dim3(256), 0, st, *a, *g,
                        S.kv, stats, part);
     if (S.kv.splits > 1) {
         launch_sum<T>(part, 2 * S.all_k, S.kv.splits, g->grad_k, S.all_k, st);

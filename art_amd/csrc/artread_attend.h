@@ -44,14 +44,27 @@ __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirs
 // ---- the problem as the kernels see it --------------------------------------------------------------
 struct AttendPlan {
     int64_t row_count;    // rows x share
+    int64_t pad_rows;     // row_count in whole tiles of 32: the gradient's row statistics
     int64_t row_blocks;   // blocks of rows per (batch entry, key head)
     int64_t items;        // batch x kv_heads x row_blocks
-    int share;
+    uint32_t share, inv_share;   // heads per key head; floor(2^32 / share), 2^32 - 1 for 1
     int splits;           // parts the keys of an item are dealt to
+    int by_head;          // order of the key walk's items
     float c;              // |scale| * log2(e)
     float unweight;       // takes back the factor that f16 weights carry
     uint32_t q_and, q_xor;   // scale's sign (and zero) applied to the bits of q: c stays positive
 };
+
+// query position and head of row r < 2^31: the quotient from inv_share is at most one too small
+__device__ __forceinline__ void split_row(const AttendPlan& P, int64_t kh, uint32_t r, int64_t* t, int64_t* h) {
+    uint32_t q = __umulhi(r, P.inv_share), g = r - q * P.share;
+    if (g >= P.share) {
+        q += 1;
+        g -= P.share;
+    }
+    *t = q;
+    *h = kh * P.share + g;
+}
 
 // Deals the tiles of KT keys of a batch entry's passages to `splits` walkers, one after the other; a passage's
 // last tile may be short, the next passage starts a new tile.  Lengths are held 64 passages at a time, one per
@@ -105,27 +118,68 @@ template <int DP>
 __device__ __forceinline__ int tile_chunk(int row, int chunk) {
     return DP == 128 ? chunk ^ (((row & 3) << 2) | ((row >> 2) & 3)) : chunk ^ ((((row >> 1) & 1) << 2) | ((row >> 2) & 3));
 }
-// A operand rows r0 + (l & 31), columns 16 * s + 8 * (l >> 5)..
-template <typename T, int DP>
-__device__ __forceinline__ typename Mma<T>::V8 lds_rows(const T* tile, int row, int s, int half) {
-    return *(const typename Mma<T>::V8*)(tile + row * DP + tile_chunk<DP>(row, 2 * s + half) * 8);
+// The permutation only flips address bits below a row's size, so a lane's addresses differ from one base by XORs
+// with constants: one register for each way of reading a tile.  `opaque` keeps the compiler from holding all of them.
+__device__ __forceinline__ uint32_t lds_offset(const void* p) {
+    return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)p;
 }
-// A operand of the transposed tile: columns 32 * db + (l & 31), k over rows r0 + {4 half + 0..3, 8 + 4 half + 0..3}
+__device__ __forceinline__ uint32_t opaque(uint32_t x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+// a lane's place in the first row block of a tile, read as rows
+template <int DP>
+__device__ __forceinline__ uint32_t rows_base(int lane) {
+    const int row = lane & 31;
+    return (uint32_t)(row * DP * 2 + tile_chunk<DP>(row, lane >> 5) * 16);
+}
+// A operand: rows 32 * block + (l & 31), columns 16 * s + 8 * (l >> 5)..
 template <typename T, int DP>
-__device__ __forceinline__ typename Mma<T>::V8 lds_columns(const T* tile, int r0, int db, int lane) {
+__device__ __forceinline__ typename Mma<T>::V8 lds_rows(uint32_t base, int block, int s) {
+    typedef const __attribute__((address_space(3))) typename Mma<T>::V8* P;
+    return *(P)(uintptr_t)((base ^ (uint32_t)(32 * s)) + (uint32_t)(block * 32 * DP * 2));
+}
+// a lane's place in the first 16 rows of a tile, read as columns
+template <int DP>
+__device__ __forceinline__ uint32_t columns_base(int lane) {
+    const int i = lane & 15, row = 4 * (lane >> 5) + (i >> 2), col = (lane & 16) + 4 * (i & 3);
+    return (uint32_t)(row * DP * 2 + tile_chunk<DP>(row, col >> 3) * 16 + (col & 7) * 2);
+}
+// A operand of the transposed tile: columns 32 * db + (l & 31), k over rows r0 + {4 half + 0..3, 8 + 4 half + 0..3};
+// r0 is a multiple of 16
+template <typename T, int DP>
+__device__ __forceinline__ typename Mma<T>::V8 lds_columns(uint32_t base, int r0, int db) {
     union {
         s16x4 h[2];
         typename Mma<T>::V8 v;
     } u;
-    const int i = lane & 15, half = lane >> 5, col = 32 * db + (lane & 16) + 4 * (i & 3);
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-        const int row = r0 + 8 * x + 4 * half + (i >> 2);
-        const T* p = tile + row * DP + tile_chunk<DP>(row, col >> 3) * 8 + (col & 7);
-        u.h[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
-    }
+    for (int x = 0; x < 2; ++x)
+        u.h[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(uintptr_t)(
+            (base ^ (uint32_t)(64 * db + 32 * x)) + (uint32_t)((r0 + 8 * x) * DP * 2)));
     return u.v;
 }
+
+// ---- memory straight to LDS ---------------------------------------------------------------------------
+// One wave-instruction moves 64 x 16 (or 64 x 4) bytes: lane i's piece lands at dst + 16 * i (4 * i), so the chunk
+// order of the tile is made on the source side.  The compiler does not count these loads: dma_wait<N> waits until at
+// most N of the wave's vector memory operations are outstanding (its own only make that stricter).
+__device__ __forceinline__ void dma16(const void* src, uint32_t dst) {
+    uint32_t keep;
+    asm volatile("s_nop 4\n\ts_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep) : "s"(dst), "v"(src) : "memory");
+}
+__device__ __forceinline__ void dma4(const void* src, uint32_t dst) {
+    uint32_t keep;
+    asm volatile("s_nop 4\n\ts_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %2, off\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep) : "s"(dst), "v"(src) : "memory");
+}
+// also every LDS read of the wave is done: the barrier behind it lets others refill what it read
+template <int N>
+__device__ __forceinline__ void dma_wait() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void wave_meet() { asm volatile("s_barrier" ::: "memory"); }
 
 // ---- softmax over one tile ----------------------------------------------------------------------------
 __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
@@ -219,7 +273,8 @@ __device__ __forceinline__ void finish_rows(const artread_attend_t& A, const Att
             }
         return;
     }
-    const int64_t t = r / P.share, h = kh * P.share + r % P.share;
+    int64_t t, h;
+    split_row(P, kh, (uint32_t)r, &t, &h);
     const int64_t at = ((b * A.rows + t) * A.heads + h) * dim;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;   // no key: zeros
 #pragma unroll
@@ -279,7 +334,8 @@ __global__ __launch_bounds__(256) void attend_join_kernel(artread_attend_t A, At
         }
         if (!there || (G > 1 && group != 0)) continue;
         const int64_t r = R % P.row_count, bk = R / P.row_count, kh = bk % A.kv_heads, b = bk / A.kv_heads;
-        const int64_t t = r / P.share, h = kh * P.share + r % P.share;
+        int64_t t, h;
+        split_row(P, kh, (uint32_t)r, &t, &h);
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
         for (int x = 0; x < 4; ++x) o[x] *= inv;
@@ -293,7 +349,8 @@ template <typename T, int DP>
 __device__ __forceinline__ void load_q(const artread_attend_t& A, const AttendPlan& P, const T* base, int64_t s_batch,
                                        int64_t s_row, int64_t s_head, int64_t b, int64_t kh, int64_t r, int half,
                                        uint32_t q_and, uint32_t q_xor, typename Mma<T>::V8 (&q)[DP / 16]) {
-    const int64_t t = r / P.share, h = kh * P.share + r % P.share;
+    int64_t t, h;
+    split_row(P, kh, (uint32_t)r, &t, &h);
     const T* src = base + b * s_batch + t * s_row + h * s_head;
 #pragma unroll
     for (int s = 0; s < DP / 16; ++s) {
@@ -375,6 +432,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void attend_stream_kernel(ar
 #pragma unroll
             for (int x = 0; x < QB; ++x) softmax_tile<T, 1, DP / 32>(s[x], P.c, left, half, m[x], l[x], o[x]);
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // the tile is written: LDS keeps a wave's order
+            const uint32_t vcol = opaque(lds_offset(tile) + columns_base<DP>(lane));
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks) {
                 V8 pw[QB];
@@ -382,7 +440,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void attend_stream_kernel(ar
                 for (int x = 0; x < QB; ++x) pw[x] = weights8<T>(s[x][0], ks);
 #pragma unroll
                 for (int db = 0; db < DP / 32; ++db) {
-                    const V8 vt = lds_columns<T, DP>(tile, 16 * ks, db, lane);
+                    const V8 vt = lds_columns<T, DP>(vcol, 16 * ks, db);
 #pragma unroll
                     for (int x = 0; x < QB; ++x) o[x][db] = Mma<T>::mul(vt, pw[x], o[x][db]);
                 }
@@ -466,8 +524,8 @@ __global__ __launch_bounds__(256, QB == 1 ? 2 : 1) void attend_tile_kernel(artre
             walk.advance();
             more = walk.settle();
             if (more) load();
-            const T* kt = ktile[buf];
-            const T* vt = vtile[buf];
+            const uint32_t krow = opaque(lds_offset(ktile[buf]) + rows_base<DP>(lane));
+            const uint32_t vcol = opaque(lds_offset(vtile[buf]) + columns_base<DP>(lane));
             f32x16 s[QB][2];
 #pragma unroll
             for (int x = 0; x < QB; ++x) s[x][0] = s[x][1] = f32x16{};
@@ -475,7 +533,7 @@ __global__ __launch_bounds__(256, QB == 1 ? 2 : 1) void attend_tile_kernel(artre
             for (int k = 0; k < DP / 16; ++k)
 #pragma unroll
                 for (int kb = 0; kb < 2; ++kb) {
-                    const V8 a = lds_rows<T, DP>(kt, 32 * kb + (lane & 31), k, half);
+                    const V8 a = lds_rows<T, DP>(krow, kb, k);
 #pragma unroll
                     for (int x = 0; x < QB; ++x) s[x][kb] = Mma<T>::mul(a, q[x][k], s[x][kb]);
                 }
@@ -488,7 +546,7 @@ __global__ __launch_bounds__(256, QB == 1 ? 2 : 1) void attend_tile_kernel(artre
                 for (int x = 0; x < QB; ++x) pw[x] = weights8<T>(s[x][ks >> 1], ks & 1);
 #pragma unroll
                 for (int db = 0; db < DP / 32; ++db) {
-                    const V8 a = lds_columns<T, DP>(vt, 16 * ks, db, lane);
+                    const V8 a = lds_columns<T, DP>(vcol, 16 * ks, db);
 #pragma unroll
                     for (int x = 0; x < QB; ++x) o[x][db] = Mma<T>::mul(a, pw[x], o[x][db]);
                 }

@@ -7,6 +7,8 @@
 // and dV and goes over the rows, those of the heads that share a key head among them.  In both a lane owns one
 // column of S (a row, or a key), so P and dS are already the B operands of the second products.
 #pragma once
+#include <type_traits>
+
 #include "artread_attend.h"
 
 // log-sum and delta of every row in the order (batch entry, key head, r), the log-sum in powers of two and with the
@@ -15,14 +17,19 @@ struct RowStat {
     float x, delta;
 };
 
-// 16 lanes per row, eight columns each
+// 16 lanes per row, eight columns each.  The rows of a key head are padded to whole tiles of 32.
 template <typename T>
 __global__ __launch_bounds__(256) void attend_delta_kernel(artread_attend_t A, artread_attend_grads_t G, AttendPlan P,
                                                            int64_t all_rows, RowStat* __restrict__ stats) {
     const int lane = threadIdx.x & 15, d = lane * 8;
     for (int64_t R = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4); R < all_rows; R += (int64_t)gridDim.x * 16) {
-        const int64_t r = R % P.row_count, bk = R / P.row_count, kh = bk % A.kv_heads, b = bk / A.kv_heads;
-        const int64_t t = r / P.share, h = kh * P.share + r % P.share;
+        const int64_t r = R % P.pad_rows, bk = R / P.pad_rows, kh = bk % A.kv_heads, b = bk / A.kv_heads;
+        if (r >= P.row_count) {   // rows that are not there have no weight
+            if (lane == 0) stats[R] = RowStat{INFINITY, 0.0f};
+            continue;
+        }
+        int64_t t, h;
+        split_row(P, kh, (uint32_t)r, &t, &h);
         const int64_t at = ((b * A.rows + t) * A.heads + h) * A.dim + d;
         float sum = 0.0f;
         if (d < (int)A.dim) {
@@ -93,7 +100,7 @@ __device__ __forceinline__ void put4(T* p, const float* x) {
 // NW waves of 32 rows share tiles of 32 * KB keys, double-buffered in LDS.  With P.splits > 1 each split leaves
 // its f32 part of dQ at part + split * (all of dQ).
 template <typename T, int DP, int NW, int KB>
-__global__ __launch_bounds__(64 * NW, DP == 64 ? 2 : 1) void attend_grad_q_kernel(artread_attend_t A, artread_attend_grads_t G,
+__global__ __launch_bounds__(64 * NW, 2) void attend_grad_q_kernel(artread_attend_t A, artread_attend_grads_t G,
                                                                     AttendPlan P, const RowStat* __restrict__ stats,
                                                                     float* __restrict__ part) {
     __shared__ __attribute__((aligned(16))) T ktile[2][32 * KB * DP];
@@ -113,7 +120,7 @@ __global__ __launch_bounds__(64 * NW, DP == 64 ? 2 : 1) void attend_grad_q_kerne
         load_q<T, DP>(A, P, (const T*)A.q, A.q_batch, A.q_row, A.q_head, b, kh, r, half, P.q_and, P.q_xor, q);
         load_q<T, DP>(A, P, (const T*)G.grad_out, G.g_batch, G.g_row, G.g_head, b, kh, r, half, 0xffffffffu, 0u, g);
         RowStat st{INFINITY, 0.0f};
-        if (r < P.row_count) st = stats[bk * P.row_count + r];
+        if (r < P.row_count) st = stats[bk * P.pad_rows + r];
         f32x16 acc[DP / 32];
         Spread<T> spread;
 #pragma unroll
@@ -156,15 +163,16 @@ __global__ __launch_bounds__(64 * NW, DP == 64 ? 2 : 1) void attend_grad_q_kerne
             walk.advance();
             more = walk.settle();
             if (more) load();
-            const T* kt = ktile[buf];
-            const T* vt = vtile[buf];
+            const uint32_t krow = opaque(lds_offset(ktile[buf]) + rows_base<DP>(lane));
+            const uint32_t vrow = opaque(lds_offset(vtile[buf]) + rows_base<DP>(lane));
+            const uint32_t kcol = opaque(lds_offset(ktile[buf]) + columns_base<DP>(lane));
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) {
                 f32x16 s = f32x16{}, dp = f32x16{};
 #pragma unroll
                 for (int k = 0; k < DP / 16; ++k) {
-                    s = Mma<T>::mul(lds_rows<T, DP>(kt, 32 * kb + (lane & 31), k, half), q[k], s);
-                    dp = Mma<T>::mul(lds_rows<T, DP>(vt, 32 * kb + (lane & 31), k, half), g[k], dp);
+                    s = Mma<T>::mul(lds_rows<T, DP>(krow, kb, k), q[k], s);
+                    dp = Mma<T>::mul(lds_rows<T, DP>(vrow, kb, k), g[k], dp);
                 }
 #pragma unroll
                 for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], P.c, -st.x)) * (dp[i] - st.delta);
@@ -179,7 +187,7 @@ __global__ __launch_bounds__(64 * NW, DP == 64 ? 2 : 1) void attend_grad_q_kerne
                     const V8 ds = weights8<T>(s, ks);
 #pragma unroll
                     for (int db = 0; db < DP / 32; ++db)
-                        acc[db] = Mma<T>::mul(lds_columns<T, DP>(kt, 32 * kb + 16 * ks, db, lane), ds, acc[db]);
+                        acc[db] = Mma<T>::mul(lds_columns<T, DP>(kcol, 32 * kb + 16 * ks, db), ds, acc[db]);
                 }
             }
             if (more) put(buf ^ 1);
@@ -187,7 +195,8 @@ __global__ __launch_bounds__(64 * NW, DP == 64 ? 2 : 1) void attend_grad_q_kerne
             buf ^= 1;
         }
         if (r < P.row_count) {
-            const int64_t t = r / P.share, h = kh * P.share + r % P.share;
+            int64_t t, h;
+            split_row(P, kh, (uint32_t)r, &t, &h);
             const int64_t at = ((b * A.rows + t) * A.heads + h) * dim;
             const float f = A.scale * spread.inverse() * P.unweight;
 #pragma unroll
@@ -205,29 +214,46 @@ __global__ __launch_bounds__(64 * NW, DP == 64 ? 2 : 1) void attend_grad_q_kerne
 }
 
 // ---- dK and dV: the key walk ------------------------------------------------------------------------------
-// Four waves of 32 keys of one passage share tiles of 32 rows of Q and dO, double-buffered in LDS: each is read as
-// rows for S and dP and transposed for dK and dV.  With P.splits > 1 the rows are dealt to splits, which leave f32
-// parts of dK and dV.
+// Four waves of 32 keys of one passage share tiles of 32 rows of Q and dO, fetched two tiles ahead into a ring of
+// three in LDS: each is read as rows for S and dP and transposed for dK and dV.  With P.splits > 1 the rows are dealt
+// to splits, which leave f32 parts of dK and dV.
 template <typename T, int DP>
-__global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void attend_grad_kv_kernel(artread_attend_t A, artread_attend_grads_t G,
+__global__ __launch_bounds__(256, 2) void attend_grad_kv_kernel(artread_attend_t A, artread_attend_grads_t G,
                                                                   AttendPlan P, const RowStat* __restrict__ stats,
                                                                   float* __restrict__ part) {
-    __shared__ __attribute__((aligned(16))) T qtile[2][32 * DP];
-    __shared__ __attribute__((aligned(16))) T gtile[2][32 * DP];
-    __shared__ __attribute__((aligned(16))) RowStat stile[2][32];
+    constexpr int STAGES = 3;
+    __shared__ __attribute__((aligned(1024))) T qtile[2 * STAGES][32 * DP];   // Q's tiles and behind them dO's
+    __shared__ __attribute__((aligned(1024))) RowStat stile[STAGES][4][32];   // a copy for each wave
     typedef typename Mma<T>::V8 V8;
     const int lane = threadIdx.x & 63, half = lane >> 5, wave = uniform(threadIdx.x >> 6);
     const int dim = (int)A.dim;
     const int64_t key_blocks = (A.len + 127) / 128;
     const int64_t total = P.items * P.splits;   // batch x passages x key_blocks x kv_heads x splits
-    for (int64_t w = blockIdx.x; w < total; w += gridDim.x) {
-        const int split = (int)(w % P.splits);
-        int64_t item = w / P.splits;
-        const int64_t kh = item % A.kv_heads;
-        item /= A.kv_heads;
+    for (int64_t id = blockIdx.x; id < (total + 7) / 8 * 8; id += gridDim.x) {
+        // Many rows: the workgroups of one key head stand together on an XCD, whose L2 then serves its rows.  Few:
+        // the key heads of a state, neighbours in memory, are read side by side.
+        int64_t item = P.by_head ? xcd_item(id, total) : id;
+        if (item >= total) continue;
+        if (id != blockIdx.x) {   // the tiles of the item before are read
+            dma_wait<0>();
+            wave_meet();
+        }
+        const int split = (int)(item % P.splits);
+        item /= P.splits;
+        int64_t kh = 0;
+        if (!P.by_head) {
+            kh = item % A.kv_heads;
+            item /= A.kv_heads;
+        }
         const int64_t j0 = item % key_blocks * 128;
         item /= key_blocks;
-        const int64_t p = item % A.passages, b = item / A.passages;
+        const int64_t p = item % A.passages;
+        item /= A.passages;
+        if (P.by_head) {
+            kh = item % A.kv_heads;
+            item /= A.kv_heads;
+        }
+        const int64_t b = item;
         int n = (int)A.len;
         if (A.lengths) {
             const int x = uniform(A.lengths[b * A.passages + p]);
@@ -255,78 +281,74 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void attend_grad_kv_kernel(a
                 kf[s] = x.v;
                 vf[s] = load8<T>(vp + 16 * s, ok);
             }
-            constexpr int CH = DP / 8, TR = 256 / CH, TN = 32 / TR;   // threads per row, rows side by side, steps
-            const int trow = threadIdx.x / CH, tchunk = threadIdx.x % CH;
-            V8 qr[TN], gr[TN];
-            RowStat sr;
-            const int64_t tiles = (P.row_count + 31) / 32;
-            auto load = [&](int64_t tile) {
+            // pieces of 1 KiB: PR rows each, PW of a tile for each wave; rows that are not there repeat the last one
+            // (their weight is zero), columns behind dim the first (they meet zeros of K and V)
+            constexpr int CH = DP / 8, PR = 64 / CH, PW = 32 / PR / 4;
+            const int prow = lane / CH, tiles = (int)((P.row_count + 31) / 32);
+            const RowStat* sp = stats + (b * A.kv_heads + kh) * P.pad_rows;
+            auto fetch = [&](int tile, int stage) {
 #pragma unroll
-                for (int x = 0; x < TN; ++x) {
-                    const int64_t r = tile * 32 + trow + x * TR;
-                    const int64_t t = r / P.share, h = kh * P.share + r % P.share;
-                    const bool ok = r < P.row_count && 8 * tchunk < dim;
-                    qr[x] = load8<T>((const T*)A.q + b * A.q_batch + t * A.q_row + h * A.q_head + 8 * tchunk, ok);
-                    gr[x] = load8<T>((const T*)G.grad_out + b * G.g_batch + t * G.g_row + h * G.g_head + 8 * tchunk, ok);
+                for (int x = 0; x < PW; ++x) {
+                    const int piece = wave * PW + x, row = piece * PR + prow;
+                    int64_t r = (int64_t)tile * 32 + row, t, h;
+                    r = r < P.row_count ? r : P.row_count - 1;
+                    split_row(P, kh, (uint32_t)r, &t, &h);
+                    int col = tile_chunk<DP>(row, lane % CH) * 8;
+                    col = col < dim ? col : 0;
+                    dma16((const T*)A.q + b * A.q_batch + t * A.q_row + h * A.q_head + col, lds_offset(&qtile[stage][piece * 512]));
+                    dma16((const T*)G.grad_out + b * G.g_batch + t * G.g_row + h * G.g_head + col, lds_offset(&qtile[STAGES + stage][piece * 512]));
                 }
-                const int64_t r = tile * 32 + threadIdx.x;
-                sr = RowStat{INFINITY, 0.0f};   // rows that are not there have no weight
-                if (threadIdx.x < 32 && r < P.row_count) sr = stats[(b * A.kv_heads + kh) * P.row_count + r];
+                dma4((const float*)(sp + tile * 32) + lane, lds_offset(&stile[stage][wave][0]));
             };
-            auto put = [&](int buf) {
+            constexpr int LOADS = 2 * PW + 1;
+            if (split < tiles) fetch(split, 0);
+            if (split + P.splits < tiles) fetch(split + P.splits, 1);
+            // one loop for waves with keys and one for those without: both load and meet at the barriers
+            auto go = [&](auto with_keys) {
+                int stage = 0;
+                for (int tile = split; tile < tiles; tile += P.splits) {
+                    if (tile + P.splits < tiles) dma_wait<LOADS>();   // all but the next tile's
+                    else dma_wait<0>();
+                    wave_meet();   // everyone's pieces are there, and everyone is done with the tile before
+                    const int ahead = stage == 0 ? 2 : stage - 1;
+                    if (tile + 2 * P.splits < tiles) fetch(tile + 2 * P.splits, ahead);
+                    if constexpr (decltype(with_keys)::value) {
+                        const uint32_t qrow = opaque(lds_offset(qtile[stage]) + rows_base<DP>(lane));
+                        const uint32_t qcol = opaque(lds_offset(qtile[stage]) + columns_base<DP>(lane));
+                        f32x16 s = f32x16{}, dp = f32x16{};
 #pragma unroll
-                for (int x = 0; x < TN; ++x) {
-                    const int row = trow + x * TR;
-                    *(V8*)(qtile[buf] + row * DP + tile_chunk<DP>(row, tchunk) * 8) = qr[x];
-                    *(V8*)(gtile[buf] + row * DP + tile_chunk<DP>(row, tchunk) * 8) = gr[x];
-                }
-                if (threadIdx.x < 32) stile[buf][threadIdx.x] = sr;
-            };
-            if (split < tiles) {
-                load(split);
-                put(0);
-            }
-            __syncthreads();
-            int buf = 0;
-            for (int64_t tile = split; tile < tiles; tile += P.splits) {
-                const bool more = tile + P.splits < tiles;
-                if (more) load(tile + P.splits);
-                if (j0 + 32 * wave < n) {   // uniform over the wave
-                    const T* qt = qtile[buf];
-                    const T* gt = gtile[buf];
-                    f32x16 s = f32x16{}, dp = f32x16{};
+                        for (int k = 0; k < DP / 16; ++k) {
+                            s = Mma<T>::mul(lds_rows<T, DP>(qrow, 0, k), kf[k], s);
+                            dp = Mma<T>::mul(lds_rows<T, DP>(qrow, STAGES, k), vf[k], dp);
+                        }
 #pragma unroll
-                    for (int k = 0; k < DP / 16; ++k) {
-                        s = Mma<T>::mul(lds_rows<T, DP>(qt, lane & 31, k, half), kf[k], s);
-                        dp = Mma<T>::mul(lds_rows<T, DP>(gt, lane & 31, k, half), vf[k], dp);
-                    }
+                        for (int x = 0; x < 4; ++x) {
+                            const float4 a = *(const float4*)&stile[stage][wave][8 * x + 4 * half];
+                            const float4 c = *(const float4*)&stile[stage][wave][8 * x + 4 * half + 2];
+                            const float xs[4] = {a.x, a.z, c.x, c.z}, ds[4] = {a.y, a.w, c.y, c.w};
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        const float4 a = *(const float4*)&stile[buf][8 * x + 4 * half];
-                        const float4 c = *(const float4*)&stile[buf][8 * x + 4 * half + 2];
-                        const float xs[4] = {a.x, a.z, c.x, c.z}, ds[4] = {a.y, a.w, c.y, c.w};
+                            for (int e = 0; e < 4; ++e) {
+                                const int i = 4 * x + e;
+                                s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], P.c, -xs[e]));
+                                dp[i] = s[i] * (dp[i] - ds[e]);
+                            }
+                        }
+                        spread.fit(dp, dk);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int i = 4 * x + e;
-                            s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], P.c, -xs[e]));
-                            dp[i] = s[i] * (dp[i] - ds[e]);
+                        for (int ks = 0; ks < 2; ++ks) {
+                            const V8 pw = weights8<T>(s, ks), ds = weights8<T>(dp, ks);
+#pragma unroll
+                            for (int db = 0; db < DP / 32; ++db) {
+                                dv[db] = Mma<T>::mul(lds_columns<T, DP>(qcol, STAGES * 32 + 16 * ks, db), pw, dv[db]);
+                                dk[db] = Mma<T>::mul(lds_columns<T, DP>(qcol, 16 * ks, db), ds, dk[db]);
+                            }
                         }
                     }
-                    spread.fit(dp, dk);
-#pragma unroll
-                    for (int ks = 0; ks < 2; ++ks) {
-                        const V8 pw = weights8<T>(s, ks), ds = weights8<T>(dp, ks);
-#pragma unroll
-                        for (int db = 0; db < DP / 32; ++db) {
-                            dv[db] = Mma<T>::mul(lds_columns<T, DP>(gt, 16 * ks, db, lane), pw, dv[db]);
-                            dk[db] = Mma<T>::mul(lds_columns<T, DP>(qt, 16 * ks, db, lane), ds, dk[db]);
-                        }
-                    }
+                    stage = stage == 2 ? 0 : stage + 1;
                 }
-                if (more) put(buf ^ 1);
-                __syncthreads();
-                buf ^= 1;
-            }
+            };
+            if (j0 + 32 * wave < n) go(std::true_type{});   // uniform over the wave
+            else go(std::false_type{});
         }
         if (j < A.len) {
             const int64_t at = (((b * A.passages + p) * A.len + j) * A.kv_heads + kh) * dim;
