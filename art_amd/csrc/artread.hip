@@ -48,6 +48,9 @@ struct ReadDeviceGuard {
 extern "C" const char* artread_last_error(void) { return g_read_err; }
 
 static constexpr int64_t kLimit = (int64_t)1 << 31;
+static constexpr int64_t kStrideLimit = (int64_t)1 << 40;
+static constexpr int64_t kRowLimit = (int64_t)1 << 24;   // the rows of a tile stay within 32 bits of bytes
+static bool tile_fits(int64_t row, int64_t head, int64_t share) { return row < kRowLimit && head * share < 32 * kRowLimit; }
 static int elem_bytes(int dtype) { return dtype == ARTREAD_F32 ? 4 : 2; }
 static bool aligned(const void* p, uint64_t to) { return ((uintptr_t)p) % to == 0; }
 static int64_t round_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
@@ -289,8 +292,10 @@ static int check_attend(const artread_attend_t* a) {
     const int64_t strides[11] = {a->q_batch, a->q_row, a->q_head, a->k_batch, a->k_passage, a->k_row,
                                  a->k_head, a->v_batch, a->v_passage, a->v_row, a->v_head};
     for (int i = 0; i < 11; ++i)
-        READ_ARG(strides[i] >= 0 && strides[i] % 8 == 0 && strides[i] < kLimit,
-                 "strides must be multiples of 8 in [0, 2^31)");
+        READ_ARG(strides[i] >= 0 && strides[i] % 8 == 0 && strides[i] < kStrideLimit,
+                 "strides must be multiples of 8 in [0, 2^40)");
+    READ_ARG(a->k_row < kRowLimit && a->v_row < kRowLimit && tile_fits(a->q_row, a->q_head, a->heads / a->kv_heads),
+             "row strides must be below 2^24, the query heads that share a key head within 2^29 elements");
     return 0;
 }
 static int check_attend_call(const artread_attend_t* a) {
@@ -364,7 +369,7 @@ static void launch_attend(const artread_attend_t* a, const AttendShape& S, const
         else if constexpr (DP == 64) hipLaunchKernelGGL((attend_stream_kernel<T, DP, 2>), grid, dim3(256), 0, st, *a, S.plan, W);
     } else {
         const dim3 grid(grid_of(round_up(parts, 8)));
-        hipLaunchKernelGGL((attend_tile_kernel<T, DP, 1>), grid, dim3(256), 0, st, *a, S.plan, W);
+        hipLaunchKernelGGL((attend_tile_kernel<T, DP>), grid, dim3(256), 0, st, *a, S.plan, W);
     }
     if (S.plan.splits > 8)
         hipLaunchKernelGGL((attend_join_kernel<T, 8>), dim3(grid_of(W.rows)), dim3(256), 0, st, *a, S.plan, W);
@@ -476,8 +481,10 @@ extern "C" int artread_attend_grad(int device, const artread_attend_t* a, const 
     READ_ARG(gr && a->lse && gr->grad_out && gr->grad_q && gr->grad_k && gr->grad_v, "a pointer is NULL");
     const int64_t strides[3] = {gr->g_batch, gr->g_row, gr->g_head};
     for (int i = 0; i < 3; ++i)
-        READ_ARG(strides[i] >= 0 && strides[i] % 8 == 0 && strides[i] < kLimit,
-                 "strides must be multiples of 8 in [0, 2^31)");
+        READ_ARG(strides[i] >= 0 && strides[i] % 8 == 0 && strides[i] < kStrideLimit,
+                 "strides must be multiples of 8 in [0, 2^40)");
+    READ_ARG(tile_fits(gr->g_row, gr->g_head, a->heads / a->kv_heads),
+             "row strides must be below 2^24, the query heads that share a key head within 2^29 elements");
     READ_ARG(aligned(gr->grad_out, 16) && aligned(gr->grad_q, 16) && aligned(gr->grad_k, 16) && aligned(gr->grad_v, 16),
              "gradients must be 16-byte aligned");
     const GradShape S = grad_shape(a);

@@ -164,15 +164,22 @@ __device__ __forceinline__ typename Mma<T>::V8 lds_columns(uint32_t base, int r0
 // One wave-instruction moves 64 x 16 (or 64 x 4) bytes: lane i's piece lands at dst + 16 * i (4 * i), so the chunk
 // order of the tile is made on the source side.  The compiler does not count these loads: dma_wait<N> waits until at
 // most N of the wave's vector memory operations are outstanding (its own only make that stricter).
-__device__ __forceinline__ void dma16(const void* src, uint32_t dst) {
-    uint32_t keep;
-    asm volatile("s_nop 4\n\ts_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off\n\ts_mov_b32 m0, %0"
-                 : "=&s"(keep) : "s"(dst), "v"(src) : "memory");
+// Sources are a uniform base plus 32 bits of bytes per lane.
+__device__ __forceinline__ const void* uniform_ptr(const void* p) {
+    const uint64_t u = (uint64_t)(uintptr_t)p;
+    const uint64_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)u);
+    const uint64_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(u >> 32));
+    return (const void*)(uintptr_t)(lo | hi << 32);
 }
-__device__ __forceinline__ void dma4(const void* src, uint32_t dst) {
+__device__ __forceinline__ void dma16(const void* base, uint32_t lane_bytes, uint32_t dst) {
     uint32_t keep;
-    asm volatile("s_nop 4\n\ts_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %2, off\n\ts_mov_b32 m0, %0"
-                 : "=&s"(keep) : "s"(dst), "v"(src) : "memory");
+    asm volatile("s_nop 4\n\ts_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %3, %2\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep) : "s"(dst), "s"(uniform_ptr(base)), "v"(lane_bytes) : "memory");
+}
+__device__ __forceinline__ void dma4(const void* base, uint32_t lane_bytes, uint32_t dst) {
+    uint32_t keep;
+    asm volatile("s_nop 4\n\ts_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %3, %2\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep) : "s"(dst), "s"(uniform_ptr(base)), "v"(lane_bytes) : "memory");
 }
 // also every LDS read of the wave is done: the barrier behind it lets others refill what it read
 template <int N>
@@ -182,7 +189,15 @@ __device__ __forceinline__ void dma_wait() {
 __device__ __forceinline__ void wave_meet() { asm volatile("s_barrier" ::: "memory"); }
 
 // ---- softmax over one tile ----------------------------------------------------------------------------
-__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
+// the two halves of a wave hold one column between them: the greater, and the sum, of their values for both
+__device__ __forceinline__ float both_max(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float both_sum(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
 
 // scores of NB x 32 keys of one row per lane pair -> weights; m, l are the running maximum (of scores x c) and the
 // lane's own part of the sum, `o` the accumulators that a new maximum rescales
@@ -190,21 +205,23 @@ template <typename T, int NB, int NO>
 __device__ __forceinline__ void softmax_tile(f32x16 (&s)[NB], float c, int left, int half, float& m, float& l,
                                              f32x16 (&o)[NO]) {
     if (left < NB * 32) {
+        const int mine = left - 4 * half;   // keys of this lane's rows of C
+        asm volatile("");                   // a branch: most tiles are whole
 #pragma unroll
         for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
             for (int i = 0; i < 16; ++i)
-                if (32 * kb + 8 * (i >> 2) + 4 * half + (i & 3) >= left) s[kb][i] = -INFINITY;
+                if (32 * kb + 8 * (i >> 2) + (i & 3) >= mine) s[kb][i] = -INFINITY;
     }
     float top = s[0][0];
 #pragma unroll
     for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
         for (int i = 0; i < 16; ++i) top = fmaxf(top, s[kb][i]);
-    top = fmaxf(top, other_half(top)) * c;
+    top = both_max(top) * c;
     if (__any(top > m)) {
         const float m1 = fmaxf(m, top);
-        const float f = m1 == -INFINITY ? 1.0f : exp2f(m - m1);
+        const float f = m1 == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - m1);
         m = m1;
         l *= f;
 #pragma unroll
@@ -213,13 +230,15 @@ __device__ __forceinline__ void softmax_tile(f32x16 (&s)[NB], float c, int left,
             for (int i = 0; i < 16; ++i) o[x][i] *= f;
     }
     const float base = (m == -INFINITY ? 0.0f : m) - Mma<T>::kWeightLog2;
+    float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};   // four chains instead of one as long as the tile
 #pragma unroll
     for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             s[kb][i] = __builtin_amdgcn_exp2f(fmaf(s[kb][i], c, -base));
-            l += s[kb][i];
+            part[i & 3] += s[kb][i];
         }
+    l += (part[0] + part[1]) + (part[2] + part[3]);
 }
 
 template <typename T>
@@ -258,7 +277,7 @@ template <typename T, int DP>
 __device__ __forceinline__ void finish_rows(const artread_attend_t& A, const AttendPlan& P, const Partials& W, int64_t b,
                                             int64_t kh, int64_t r, int split, int half, float m, float l,
                                             f32x16 (&o)[DP / 32]) {
-    l += other_half(l);
+    l = both_sum(l);
     if (r >= P.row_count) return;
     const int dim = (int)A.dim;
     if (P.splits > 1) {
@@ -453,109 +472,131 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void attend_stream_kernel(ar
 }
 
 // ---- many rows: four waves share the tiles --------------------------------------------------------------
-// 128 * QB rows per workgroup, 64 keys per tile; K and V tiles are double-buffered in LDS, one barrier per tile.
 // Workgroups of one (batch entry, key head) sit on one XCD, whose L2 then serves its states.
 __device__ __forceinline__ int64_t xcd_item(int64_t id, int64_t items) {
     const int64_t per = (items + 7) / 8;
     return (id & 7) * per + (id >> 3);
 }
 
-template <typename T, int DP, int QB>
-__global__ __launch_bounds__(256, QB == 1 ? 2 : 1) void attend_tile_kernel(artread_attend_t A, AttendPlan P, Partials W) {
-    __shared__ __attribute__((aligned(16))) T ktile[2][64 * DP];
-    __shared__ __attribute__((aligned(16))) T vtile[2][64 * DP];
+// Brings tiles of KB x 32 states into a ring of LDS: 1 KiB pieces, PW of a tile for each of NW waves.  States behind
+// the passage's length and columns behind dim become zeros: a short tile's are written, the columns' are cleared once.
+template <typename T, int DP, int KB, int NW>
+struct TileFetch {
+    static constexpr int CH = DP / 8, PR = 64 / CH, PW = 32 * KB / PR / NW;   // chunks per row, rows per piece
+    int row, col, lane, wave;
+    __device__ __forceinline__ void start(int w) {
+        lane = threadIdx.x & 63;
+        wave = w;
+        row = lane / CH;
+        col = lane % CH;
+    }
+    // src: state 0 of the tile; left: states from there to the passage's end; stride below 2^24
+    __device__ __forceinline__ void fetch(const T* src, int64_t stride, int left, int dim, uint32_t tile) const {
+        const bool full = left >= 32 * KB;   // uniform
+        const uint32_t bytes = (uint32_t)row * (uint32_t)stride * 2;
+#pragma unroll
+        for (int x = 0; x < PW; ++x) {
+            const int piece = wave * PW + x, r = piece * PR + row, c = tile_chunk<DP>(r, col) * 8;
+            const uint32_t dst = tile + (uint32_t)piece * 1024;
+            const T* base = src + (int64_t)(piece * PR) * stride;
+            if (full) {
+                if (c < dim) dma16(base, bytes + c * 2, dst);
+            } else if (c < dim && r < left) {
+                dma16(base, bytes + c * 2, dst);
+            } else {
+                *(__attribute__((address_space(3))) u32x4*)(uintptr_t)(dst + lane * 16) = u32x4{0, 0, 0, 0};
+            }
+        }
+    }
+};
+
+// 128 rows per workgroup, 32 of them a wave's, 64 keys per tile; while a tile is worked on the next one arrives.
+template <typename T, int DP>
+__global__ __launch_bounds__(256, 2) void attend_tile_kernel(artread_attend_t A, AttendPlan P, Partials W) {
+    constexpr int KB = 2, TILE = 32 * KB * DP;
+    __shared__ __attribute__((aligned(1024))) T ring[4][TILE];   // two tiles of K, two of V
     typedef typename Mma<T>::V8 V8;
     const int lane = threadIdx.x & 63, half = lane >> 5, wave = uniform(threadIdx.x >> 6);
     const int dim = (int)A.dim;
+    TileFetch<T, DP, KB, 4> fetcher;
+    fetcher.start(wave);
+    if (dim < DP) {
+        for (int i = threadIdx.x; i < 4 * TILE / 8; i += 256) ((u32x4*)&ring[0][0])[i] = u32x4{0, 0, 0, 0};
+        __syncthreads();
+    }
     const int64_t total = P.items * P.splits;
     for (int64_t id = blockIdx.x; id < (total + 7) / 8 * 8; id += gridDim.x) {
         const int64_t w = xcd_item(id, total);
         if (w >= total) continue;
-        const int64_t rb = w % P.row_blocks, rest = w / P.row_blocks;
-        const int split = (int)(rest % P.splits);
-        const int64_t bk = rest / P.splits, kh = bk % A.kv_heads, b = bk / A.kv_heads;
-        const int64_t r0 = (rb * 4 + wave) * 32 * QB + (lane & 31);
-        V8 q[QB][DP / 16];
-        f32x16 o[QB][DP / 32];
-        float m[QB], l[QB];
-#pragma unroll
-        for (int x = 0; x < QB; ++x) {
-            load_q<T, DP>(A, P, (const T*)A.q, A.q_batch, A.q_row, A.q_head, b, kh, r0 + 32 * x, half, P.q_and, P.q_xor, q[x]);
-            m[x] = -INFINITY;
-            l[x] = 0.0f;
-#pragma unroll
-            for (int db = 0; db < DP / 32; ++db) o[x][db] = f32x16{};
+        if (id != blockIdx.x) {   // the tiles of the item before are read
+            dma_wait<0>();
+            wave_meet();
         }
-        constexpr int CH = DP / 8, TR = 256 / CH, TN = 64 / TR;   // threads per row, rows side by side, steps
-        const int trow = threadIdx.x / CH, tchunk = threadIdx.x % CH;
-        const T* kbase = (const T*)A.k + b * A.k_batch + kh * A.k_head + (int64_t)trow * A.k_row + 8 * tchunk;
-        const T* vbase = (const T*)A.v + b * A.v_batch + kh * A.v_head + (int64_t)trow * A.v_row + 8 * tchunk;
-        V8 kr[TN], vr[TN];
-        Walk<64> walk;
+        const int64_t rb = w % P.row_blocks, other = w / P.row_blocks;
+        const int split = (int)(other % P.splits);
+        const int64_t bk = other / P.splits, kh = bk % A.kv_heads, b = bk / A.kv_heads;
+        const int64_t r = (rb * 4 + wave) * 32 + (lane & 31);
+        const T* kbase = (const T*)A.k + b * A.k_batch + kh * A.k_head;
+        const T* vbase = (const T*)A.v + b * A.v_batch + kh * A.v_head;
+        Walk<32 * KB> walk;   // of the tiles fetched; `left` of the one worked on
         walk.start(A, b, split, P.splits);
-        auto load = [&]() {
+        auto fetch = [&](int stage) {   // keys of the tile, 0 behind the last
+            if (!walk.settle()) return 0;
             const int left = walk.n - walk.j0;
-            const T* kp = kbase + walk.p * A.k_passage + walk.j0 * A.k_row;
-            const T* vp = vbase + walk.p * A.v_passage + walk.j0 * A.v_row;
-#pragma unroll
-            for (int x = 0; x < TN; ++x) {
-                const bool ok = trow + x * TR < left && 8 * tchunk < dim;
-                kr[x] = load8<T>(kp + (int64_t)x * TR * A.k_row, ok);
-                vr[x] = load8<T>(vp + (int64_t)x * TR * A.v_row, ok);
-            }
-        };
-        auto put = [&](int buf) {
-#pragma unroll
-            for (int x = 0; x < TN; ++x) {
-                const int row = trow + x * TR;
-                *(V8*)(ktile[buf] + row * DP + tile_chunk<DP>(row, tchunk) * 8) = kr[x];
-                *(V8*)(vtile[buf] + row * DP + tile_chunk<DP>(row, tchunk) * 8) = vr[x];
-            }
-        };
-        bool more = walk.settle();
-        if (more) {
-            load();
-            put(0);
-        }
-        __syncthreads();
-        int buf = 0;
-        while (more) {
-            const int left = walk.n - walk.j0;
+            fetcher.fetch(kbase + walk.p * A.k_passage + walk.j0 * A.k_row, A.k_row, left, dim, lds_offset(ring[stage]));
+            fetcher.fetch(vbase + walk.p * A.v_passage + walk.j0 * A.v_row, A.v_row, left, dim, lds_offset(ring[2 + stage]));
             walk.advance();
-            more = walk.settle();
-            if (more) load();
-            const uint32_t krow = opaque(lds_offset(ktile[buf]) + rows_base<DP>(lane));
-            const uint32_t vcol = opaque(lds_offset(vtile[buf]) + columns_base<DP>(lane));
-            f32x16 s[QB][2];
+            return left;
+        };
+        int left = fetch(0);
+        V8 q[DP / 16];
+        f32x16 o[DP / 32];
+        float m = -INFINITY, l = 0.0f;
+        load_q<T, DP>(A, P, (const T*)A.q, A.q_batch, A.q_row, A.q_head, b, kh, r, half, P.q_and, P.q_xor, q);
 #pragma unroll
-            for (int x = 0; x < QB; ++x) s[x][0] = s[x][1] = f32x16{};
+        for (int db = 0; db < DP / 32; ++db) o[db] = f32x16{};
+        int stage = 0;
+        while (left) {
+            dma_wait<0>();
+            wave_meet();   // everyone's pieces are there, and everyone is done with the tile before
+            const int next = fetch(stage ^ 1);
+            const uint32_t krow = opaque(lds_offset(ring[stage]) + rows_base<DP>(lane));
+            const uint32_t vcol = opaque(lds_offset(ring[2 + stage]) + columns_base<DP>(lane));
+            f32x16 s[KB];
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) s[kb] = f32x16{};
+            constexpr int NK = KB * DP / 16, NV = 2 * KB * DP / 32, EARLY = NV < 8 ? NV : 8, AHEAD = NK < 6 ? NK : 6;
 #pragma unroll
             for (int k = 0; k < DP / 16; ++k)
 #pragma unroll
-                for (int kb = 0; kb < 2; ++kb) {
-                    const V8 a = lds_rows<T, DP>(krow, kb, k);
+                for (int kb = 0; kb < KB; ++kb) s[kb] = Mma<T>::mul(lds_rows<T, DP>(krow, kb, k), q[k], s[kb]);
+            // the first operands of the second product are on their way while the softmax runs
+            V8 vt[NV];
 #pragma unroll
-                    for (int x = 0; x < QB; ++x) s[x][kb] = Mma<T>::mul(a, q[x][k], s[x][kb]);
-                }
+            for (int i = 0; i < EARLY; ++i) vt[i] = lds_columns<T, DP>(vcol, 16 * (i / (DP / 32)), i % (DP / 32));
+            __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);   // LDS reads ahead, then one per product
 #pragma unroll
-            for (int x = 0; x < QB; ++x) softmax_tile<T, 2, DP / 32>(s[x], P.c, left, half, m[x], l[x], o[x]);
-#pragma unroll
-            for (int ks = 0; ks < 4; ++ks) {
-                V8 pw[QB];
-#pragma unroll
-                for (int x = 0; x < QB; ++x) pw[x] = weights8<T>(s[x][ks >> 1], ks & 1);
-#pragma unroll
-                for (int db = 0; db < DP / 32; ++db) {
-                    const V8 a = lds_columns<T, DP>(vcol, 16 * ks, db);
-#pragma unroll
-                    for (int x = 0; x < QB; ++x) o[x][db] = Mma<T>::mul(a, pw[x], o[x][db]);
-                }
+            for (int i = 0; i < NK - AHEAD; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
             }
-            if (more) put(buf ^ 1);
-            __syncthreads();
-            buf ^= 1;
-        }
 #pragma unroll
-        for (int x = 0; x < QB; ++x) finish_rows<T, DP>(A, P, W, b, kh, r0 + 32 * x, split, half, m[x], l[x], o[x]);
+            for (int i = 0; i < AHEAD; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+            }
+            softmax_tile<T, KB, DP / 32>(s, P.c, left, half, m, l, o);
+#pragma unroll
+            for (int i = EARLY; i < NV; ++i) vt[i] = lds_columns<T, DP>(vcol, 16 * (i / (DP / 32)), i % (DP / 32));
+#pragma unroll
+            for (int ks = 0; ks < 2 * KB; ++ks) {
+                const V8 pw = weights8<T>(s[ks >> 1], ks & 1);
+#pragma unroll
+                for (int db = 0; db < DP / 32; ++db) o[db] = Mma<T>::mul(vt[ks * (DP / 32) + db], pw, o[db]);
+            }
+            left = next;
+            stage ^= 1;
+        }
+        finish_rows<T, DP>(A, P, W, b, kh, r, split, half, m, l, o);
     }
 }

@@ -70,7 +70,7 @@ struct Spread<f16> {
 #pragma unroll
         for (int i = 1; i < 16; ++i) top = fmaxf(top, fabsf(ds[i]));
         if (__any(top > most)) {
-            top = fmaxf(top, other_half(top));
+            top = both_max(top);
             if (top > most) {
                 int e = 10 - ilogbf(top);                       // top * 2^e is in [2^10, 2^11)
                 e = e < -100 ? -100 : (e > 100 ? 100 : e);
@@ -97,25 +97,48 @@ __device__ __forceinline__ void put4(T* p, const float* x) {
 }
 
 // ---- dQ: the row walk -----------------------------------------------------------------------------------
-// NW waves of 32 rows share tiles of 32 * KB keys, double-buffered in LDS.  With P.splits > 1 each split leaves
+// NW waves of 32 rows share tiles of 32 * KB keys; while a tile is worked on the next one arrives in LDS.  With P.splits > 1 each split leaves
 // its f32 part of dQ at part + split * (all of dQ).
 template <typename T, int DP, int NW, int KB>
 __global__ __launch_bounds__(64 * NW, 2) void attend_grad_q_kernel(artread_attend_t A, artread_attend_grads_t G,
                                                                     AttendPlan P, const RowStat* __restrict__ stats,
                                                                     float* __restrict__ part) {
-    __shared__ __attribute__((aligned(16))) T ktile[2][32 * KB * DP];
-    __shared__ __attribute__((aligned(16))) T vtile[2][32 * KB * DP];
+    constexpr int TILE = 32 * KB * DP;
+    __shared__ __attribute__((aligned(1024))) T ring[4][TILE];   // two tiles of K, two of V
     typedef typename Mma<T>::V8 V8;
     const int lane = threadIdx.x & 63, half = lane >> 5, wave = uniform(threadIdx.x >> 6);
     const int dim = (int)A.dim;
+    TileFetch<T, DP, KB, NW> fetcher;
+    fetcher.start(wave);
+    if (dim < DP) {
+        for (int i = threadIdx.x; i < 4 * TILE / 8; i += 64 * NW) ((u32x4*)&ring[0][0])[i] = u32x4{0, 0, 0, 0};
+        __syncthreads();
+    }
     const int64_t total = P.items * P.splits;
     for (int64_t id = blockIdx.x; id < (total + 7) / 8 * 8; id += gridDim.x) {
         const int64_t w = xcd_item(id, total);
         if (w >= total) continue;
+        if (id != blockIdx.x) {   // the tiles of the item before are read
+            dma_wait<0>();
+            wave_meet();
+        }
         const int64_t rb = w % P.row_blocks, other = w / P.row_blocks;
         const int split = (int)(other % P.splits);
         const int64_t bk = other / P.splits, kh = bk % A.kv_heads, b = bk / A.kv_heads;
         const int64_t r = (rb * NW + wave) * 32 + (lane & 31);
+        const T* kbase = (const T*)A.k + b * A.k_batch + kh * A.k_head;
+        const T* vbase = (const T*)A.v + b * A.v_batch + kh * A.v_head;
+        Walk<32 * KB> walk;   // of the tiles fetched; `left` of the one worked on
+        walk.start(A, b, split, P.splits);
+        auto fetch = [&](int stage) {   // keys of the tile, 0 behind the last
+            if (!walk.settle()) return 0;
+            const int left = walk.n - walk.j0;
+            fetcher.fetch(kbase + walk.p * A.k_passage + walk.j0 * A.k_row, A.k_row, left, dim, lds_offset(ring[stage]));
+            fetcher.fetch(vbase + walk.p * A.v_passage + walk.j0 * A.v_row, A.v_row, left, dim, lds_offset(ring[2 + stage]));
+            walk.advance();
+            return left;
+        };
+        int left = fetch(0);
         V8 q[DP / 16], g[DP / 16];
         load_q<T, DP>(A, P, (const T*)A.q, A.q_batch, A.q_row, A.q_head, b, kh, r, half, P.q_and, P.q_xor, q);
         load_q<T, DP>(A, P, (const T*)G.grad_out, G.g_batch, G.g_row, G.g_head, b, kh, r, half, 0xffffffffu, 0u, g);
@@ -125,61 +148,29 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_grad_q_kernel(artread_atten
         Spread<T> spread;
 #pragma unroll
         for (int db = 0; db < DP / 32; ++db) acc[db] = f32x16{};
-        constexpr int CH = DP / 8, TR = 64 * NW / CH, TN = 32 * KB / TR;
-        const int trow = threadIdx.x / CH, tchunk = threadIdx.x % CH;
-        const T* kbase = (const T*)A.k + b * A.k_batch + kh * A.k_head + (int64_t)trow * A.k_row + 8 * tchunk;
-        const T* vbase = (const T*)A.v + b * A.v_batch + kh * A.v_head + (int64_t)trow * A.v_row + 8 * tchunk;
-        V8 kr[TN], vr[TN];
-        Walk<32 * KB> walk;
-        walk.start(A, b, split, P.splits);
-        auto load = [&]() {
-            const int left = walk.n - walk.j0;
-            const T* kp = kbase + walk.p * A.k_passage + walk.j0 * A.k_row;
-            const T* vp = vbase + walk.p * A.v_passage + walk.j0 * A.v_row;
-#pragma unroll
-            for (int x = 0; x < TN; ++x) {
-                const bool ok = trow + x * TR < left && 8 * tchunk < dim;
-                kr[x] = load8<T>(kp + (int64_t)x * TR * A.k_row, ok);
-                vr[x] = load8<T>(vp + (int64_t)x * TR * A.v_row, ok);
-            }
-        };
-        auto put = [&](int buf) {
-#pragma unroll
-            for (int x = 0; x < TN; ++x) {
-                const int row = trow + x * TR;
-                *(V8*)(ktile[buf] + row * DP + tile_chunk<DP>(row, tchunk) * 8) = kr[x];
-                *(V8*)(vtile[buf] + row * DP + tile_chunk<DP>(row, tchunk) * 8) = vr[x];
-            }
-        };
-        bool more = walk.settle();
-        if (more) {
-            load();
-            put(0);
-        }
-        __syncthreads();
-        int buf = 0;
-        while (more) {
-            const int left = walk.n - walk.j0;
-            walk.advance();
-            more = walk.settle();
-            if (more) load();
-            const uint32_t krow = opaque(lds_offset(ktile[buf]) + rows_base<DP>(lane));
-            const uint32_t vrow = opaque(lds_offset(vtile[buf]) + rows_base<DP>(lane));
-            const uint32_t kcol = opaque(lds_offset(ktile[buf]) + columns_base<DP>(lane));
+        int stage = 0;
+        while (left) {
+            dma_wait<0>();
+            wave_meet();   // everyone's pieces are there, and everyone is done with the tile before
+            const int next = fetch(stage ^ 1);
+            const uint32_t krow = opaque(lds_offset(ring[stage]) + rows_base<DP>(lane));
+            const uint32_t kcol = opaque(lds_offset(ring[stage]) + columns_base<DP>(lane));
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) {
                 f32x16 s = f32x16{}, dp = f32x16{};
 #pragma unroll
                 for (int k = 0; k < DP / 16; ++k) {
                     s = Mma<T>::mul(lds_rows<T, DP>(krow, kb, k), q[k], s);
-                    dp = Mma<T>::mul(lds_rows<T, DP>(vrow, kb, k), g[k], dp);
+                    dp = Mma<T>::mul(lds_rows<T, DP>(krow, 2 * KB + kb, k), g[k], dp);
                 }
 #pragma unroll
                 for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], P.c, -st.x)) * (dp[i] - st.delta);
                 if (left < 32 * KB) {
+                    const int mine = left - 4 * half;
+                    asm volatile("");   // a branch: most tiles are whole
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
-                        if (32 * kb + 8 * (i >> 2) + 4 * half + (i & 3) >= left) s[i] = 0.0f;
+                        if (32 * kb + 8 * (i >> 2) + (i & 3) >= mine) s[i] = 0.0f;
                 }
                 spread.fit(s, acc);
 #pragma unroll
@@ -190,9 +181,8 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_grad_q_kernel(artread_atten
                         acc[db] = Mma<T>::mul(lds_columns<T, DP>(kcol, 32 * kb + 16 * ks, db), ds, acc[db]);
                 }
             }
-            if (more) put(buf ^ 1);
-            __syncthreads();
-            buf ^= 1;
+            left = next;
+            stage ^= 1;
         }
         if (r < P.row_count) {
             int64_t t, h;
@@ -286,19 +276,25 @@ __global__ __launch_bounds__(256, 2) void attend_grad_kv_kernel(artread_attend_t
             constexpr int CH = DP / 8, PR = 64 / CH, PW = 32 / PR / 4;
             const int prow = lane / CH, tiles = (int)((P.row_count + 31) / 32);
             const RowStat* sp = stats + (b * A.kv_heads + kh) * P.pad_rows;
+            const T* qb = (const T*)A.q + b * A.q_batch + kh * P.share * A.q_head;
+            const T* gb = (const T*)G.grad_out + b * G.g_batch + kh * P.share * G.g_head;
             auto fetch = [&](int tile, int stage) {
+                int64_t t0, h0;
+                split_row(P, 0, (uint32_t)tile * 32, &t0, &h0);
 #pragma unroll
                 for (int x = 0; x < PW; ++x) {
                     const int piece = wave * PW + x, row = piece * PR + prow;
                     int64_t r = (int64_t)tile * 32 + row, t, h;
                     r = r < P.row_count ? r : P.row_count - 1;
-                    split_row(P, kh, (uint32_t)r, &t, &h);
+                    split_row(P, 0, (uint32_t)r, &t, &h);
                     int col = tile_chunk<DP>(row, lane % CH) * 8;
                     col = col < dim ? col : 0;
-                    dma16((const T*)A.q + b * A.q_batch + t * A.q_row + h * A.q_head + col, lds_offset(&qtile[stage][piece * 512]));
-                    dma16((const T*)G.grad_out + b * G.g_batch + t * G.g_row + h * G.g_head + col, lds_offset(&qtile[STAGES + stage][piece * 512]));
+                    // bytes from the tile's first query position: a tile spans at most 32 of them
+                    const uint32_t dt = (uint32_t)t - (uint32_t)t0;
+                    dma16(qb + t0 * A.q_row, (dt * (uint32_t)A.q_row + (uint32_t)(h * A.q_head) + col) * 2, lds_offset(&qtile[stage][piece * 512]));
+                    dma16(gb + t0 * G.g_row, (dt * (uint32_t)G.g_row + (uint32_t)(h * G.g_head) + col) * 2, lds_offset(&qtile[STAGES + stage][piece * 512]));
                 }
-                dma4((const float*)(sp + tile * 32) + lane, lds_offset(&stile[stage][wave][0]));
+                dma4(sp + tile * 32, (uint32_t)lane * 4, lds_offset(&stile[stage][wave][0]));
             };
             constexpr int LOADS = 2 * PW + 1;
             if (split < tiles) fetch(split, 0);

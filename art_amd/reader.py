@@ -215,15 +215,14 @@ def embed_tokens_grad(grad_out, tokens, vocab, lengths=None, scale=1.0, vocab_ba
 
 
 # ---- cross attention ------------------------------------------------------------------------------
-def _strided(t):
-    """`t` with the layout the kernels address: innermost stride 1, the others multiples of 8 elements
-    below 2**31, 16-byte aligned.  Anything else is copied."""
-    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0:
-        for s, n in zip(t.stride()[:-1], t.shape[:-1]):
-            if n > 1 and (s % 8 or s >= 1 << 31):
-                break
-        else:
-            return t
+def _strided(t, share=0):
+    """`t` [..., rows, heads, dim] with the layout the kernels address: innermost stride 1, the others multiples
+    of 8 elements, rows less than 2**24 apart, the `share` query heads of a key head within 2**29, 16-byte
+    aligned.  Anything else is copied."""
+    strides = _outer(t)
+    if (t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and not any(s % 8 for s in strides)
+            and strides[-2] < 1 << 24 and share * strides[-1] < 1 << 29):
+        return t
     return t.clone(memory_format=torch.contiguous_format)
 
 
@@ -272,7 +271,8 @@ def _attend(query, key, value, lengths, scale, want_lse, want_rest):
         return out, lse, rest
     if key.numel() == 0:
         return out.zero_(), lse.fill_(-math.inf) if want_lse else None, rest.zero_() if want_rest else None
-    query, key, value = _strided(query), _strided(key), _strided(value)
+    share = heads // key.shape[-2]
+    query, key, value = _strided(query, share), _strided(key), _strided(value)
     lengths = lengths.contiguous() if lengths is not None else None
     lib = _read()
     args = _attend_args(query, key, value, lengths, out, lse, rest, scale)
@@ -343,7 +343,8 @@ def cross_attention_grad(grad_out, query, key, value, out, saved, lengths=None, 
     grads = [torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (query, key, value)]
     if query.numel() == 0 or key.numel() == 0:
         return tuple(t.zero_() for t in grads)
-    query, key, value, grad_out = (_strided(t) for t in (query, key, value, grad_out))
+    share = heads // key.shape[-2]
+    query, grad_out, key, value = _strided(query, share), _strided(grad_out, share), _strided(key), _strided(value)
     lengths = lengths.contiguous() if lengths is not None else None
     lib = _read()
     args = _attend_args(query, key, value, lengths, out, lse, rest, scale)

@@ -66,7 +66,8 @@ int artread_embed_grad(int device, const void* grad_out, int grad_dtype, const v
  *            out + rest carries about twice out's bits, which the gradient's row sums need
  *   heads is a multiple of kv_heads: query head h reads key head h / (heads / kv_heads)
  * f16 or bf16, dim a multiple of 8 up to 128.  Strides count elements; the innermost one is 1, the
- * others are >= 0, multiples of 8 and below 2^31, and pointers are 16-byte aligned; out is contiguous. */
+ * others are >= 0 and multiples of 8, those of rows below 2^24, the query heads that share a key head
+ * within 2^29 elements, the rest below 2^40.  Pointers are 16-byte aligned; out is contiguous. */
 typedef struct {
     const void* q;
     const void* k;

@@ -195,7 +195,7 @@ BAD_ATTEND = [
     dict(dtype=2), dict(batch=0), dict(rows=0), dict(passages=0), dict(len=0), dict(heads=0), dict(kv_heads=0),
     dict(kv_heads=3), dict(dim=0), dict(dim=12), dict(dim=136), dict(rows=1 << 31), dict(batch=1 << 20, rows=1 << 20),
     dict(passages=1 << 20, len=1 << 20), dict(scale=float("nan")), dict(q_row=-8), dict(k_row=12),
-    dict(v_batch=1 << 31),
+    dict(v_batch=1 << 40), dict(k_row=1 << 24), dict(v_row=1 << 24), dict(q_row=1 << 24), dict(q_head=1 << 28),
 ]
 
 
@@ -217,7 +217,7 @@ def test_c_attend_grad_refuses():
     assert need > 0
     fine = dict(grad_out=SOME, g_batch=192, g_row=64, g_head=16, grad_q=SOME, grad_k=SOME, grad_v=SOME)
     for change in (dict(grad_out=None), dict(grad_q=None), dict(grad_k=None), dict(grad_v=None), dict(g_row=-8),
-                   dict(g_row=4), dict(grad_v=SOME + 8)):
+                   dict(g_row=4), dict(g_row=1 << 24), dict(g_head=1 << 28), dict(grad_v=SOME + 8)):
         g = rd.AttendGrads(*dict(fine, **change).values())
         assert lib.artread_attend_grad(0, ctypes.byref(a), ctypes.byref(g), SOME, need, None) == -1, change
     g = rd.AttendGrads(*fine.values())
