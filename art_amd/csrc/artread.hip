@@ -309,6 +309,11 @@ static int check_attend_call(const artread_attend_t* a) {
 }
 static unsigned grid_of(int64_t items) { return (unsigned)(items < (1 << 22) ? items : (1 << 22)); }
 
+static dim3 grid2(int64_t items) {   // at least `items` workgroups, a multiple of 8 wide: neighbours stay on their XCDs
+    const int64_t x = 1 << 16;
+    return items <= x ? dim3((unsigned)round_up(items, 8)) : dim3((unsigned)x, (unsigned)((items + x - 1) / x));
+}
+
 // How a forward call runs.  Up to 32 rows (64 at 64 columns) of a key head are one wave's, which streams the
 // keys; more share their tiles of keys in a workgroup.
 struct AttendShape {
@@ -364,11 +369,11 @@ template <typename T, int DP>
 static void launch_attend(const artread_attend_t* a, const AttendShape& S, const Partials& W, hipStream_t st) {
     const int64_t parts = S.plan.items * S.plan.splits;
     if (S.stream) {
-        const dim3 grid(grid_of((parts + 3) / 4));
+        const dim3 grid = grid2((parts + 3) / 4);
         if (S.qb == 1) hipLaunchKernelGGL((attend_stream_kernel<T, DP, 1>), grid, dim3(256), 0, st, *a, S.plan, W);
         else if constexpr (DP == 64) hipLaunchKernelGGL((attend_stream_kernel<T, DP, 2>), grid, dim3(256), 0, st, *a, S.plan, W);
     } else {
-        const dim3 grid(grid_of(round_up(parts, 8)));
+        const dim3 grid = grid2(parts);
         hipLaunchKernelGGL((attend_tile_kernel<T, DP>), grid, dim3(256), 0, st, *a, S.plan, W);
     }
     if (S.plan.splits > 8)
@@ -400,9 +405,10 @@ extern "C" int artread_attend(int device, const artread_attend_t* a, void* works
     return 0;
 }
 
-// How a gradient call runs: a walk over the keys for dQ and one over the rows for dK and dV, either of them split
-// where its workgroups would not fill the chip.
+// How a gradient call runs: up to 32 rows of a key head (64 at 64 columns) in one walk over the keys, more in a walk
+// over the keys for dQ and one over the rows for dK and dV; each split where its workgroups would not fill the chip.
 struct GradShape {
+    bool fused;
     bool narrow;           // dQ: one wave of 32 rows per workgroup, else four
     AttendPlan q, kv;
     int64_t all_q, all_k;  // elements
@@ -416,7 +422,11 @@ static GradShape grad_shape(const artread_attend_t* a) {
     Q.row_count = a->rows * Q.share;
     plan_scale(&Q, a->scale, a->dtype);
     Q.pad_rows = round_up(Q.row_count, 32);
+    Q.c = a->scale * kLog2e;   // no maximum is taken here: c may be negative or zero
+    Q.q_and = 0xffffffffu;
+    Q.q_xor = 0u;
     S.kv = Q;
+    S.fused = Q.row_count <= (a->dim <= 64 ? 64 : 32);
     S.narrow = Q.row_count <= 64;
     const int block = S.narrow ? 32 : 128, keys = S.narrow ? 32 : 64;
     Q.row_blocks = (Q.row_count + block - 1) / block;
@@ -425,6 +435,15 @@ static GradShape grad_shape(const artread_attend_t* a) {
     int64_t most = a->passages * ((a->len + keys - 1) / keys) / 4;
     want = want < most ? want : most;
     Q.splits = (int)(want < 1 ? 1 : (want < 64 ? want : 64));
+    if (S.fused) {
+        const int waves = a->dim <= 64 ? 4 : 2;
+        Q.row_blocks = 1;
+        Q.items = a->batch * a->kv_heads;
+        want = 512 / Q.items;   // two workgroups a compute unit: a third would wait for them
+        most = a->passages * ((a->len + 31) / 32) / (4 * waves);
+        want = want < most ? want : most;
+        Q.splits = (int)(want < 1 ? 1 : (want < 64 ? want : 64));
+    }
     AttendPlan& K = S.kv;
     K.row_blocks = 1;
     K.by_head = K.row_count > 64;
@@ -437,7 +456,7 @@ static GradShape grad_shape(const artread_attend_t* a) {
     S.all_k = a->batch * a->passages * a->len * a->kv_heads * a->dim;
     S.stats = 0;
     S.part = round_up(a->batch * a->kv_heads * Q.pad_rows * (int64_t)sizeof(RowStat), 256);
-    const int64_t pq = Q.splits > 1 ? Q.splits * S.all_q * 4 : 0, pk = K.splits > 1 ? K.splits * 2 * S.all_k * 4 : 0;
+    const int64_t pq = Q.splits > 1 ? Q.splits * S.all_q * 4 : 0, pk = !S.fused && K.splits > 1 ? K.splits * 2 * S.all_k * 4 : 0;
     S.total = S.part + round_up(pq > pk ? pq : pk, 256);
     return S;
 }
@@ -460,13 +479,26 @@ static void launch_attend_grad(const artread_attend_t* a, const artread_attend_g
     float* part = (float*)((char*)ws + S.part);
     const int64_t rows = a->batch * a->kv_heads * S.q.pad_rows;
     hipLaunchKernelGGL((attend_delta_kernel<T>), dim3(grid_of((rows + 15) / 16)), dim3(256), 0, st, *a, *g, S.q, rows, stats);
-    const dim3 gq(grid_of(round_up(S.q.items * S.q.splits, 8)));
+    if (S.fused) {
+        const dim3 grid = grid2(S.q.items * S.q.splits);
+        if constexpr (DP == 64) {
+            if (S.q.row_count <= 32)
+                hipLaunchKernelGGL((attend_grad_stream_kernel<T, 64, 1, 4>), grid, dim3(256), 0, st, *a, *g, S.q, stats, part);
+            else
+                hipLaunchKernelGGL((attend_grad_stream_kernel<T, 64, 2, 4>), grid, dim3(256), 0, st, *a, *g, S.q, stats, part);
+        } else {
+            hipLaunchKernelGGL((attend_grad_stream_kernel<T, 128, 1, 2>), grid, dim3(128), 0, st, *a, *g, S.q, stats, part);
+        }
+        if (S.q.splits > 1) launch_sum<T>(part, S.all_q, S.q.splits, g->grad_q, S.all_q, st);
+        return;
+    }
+    const dim3 gq = grid2(S.q.items * S.q.splits);
     if (S.narrow)
         hipLaunchKernelGGL((attend_grad_q_kernel<T, DP, 1, 1>), gq, dim3(64), 0, st, *a, *g, S.q, stats, part);
     else
         hipLaunchKernelGGL((attend_grad_q_kernel<T, DP, 4, 2>), gq, dim3(256), 0, st, *a, *g, S.q, stats, part);
     if (S.q.splits > 1) launch_sum<T>(part, S.all_q, S.q.splits, g->grad_q, S.all_q, st);
-    hipLaunchKernelGGL((attend_grad_kv_kernel<T, DP>), dim3(grid_of(round_up(S.kv.items * S.kv.splits, 8))), dim3(256), 0, st, *a, *g,
+    hipLaunchKernelGGL((attend_grad_kv_kernel<T, DP>), grid2(S.kv.items * S.kv.splits), dim3(256), 0, st, *a, *g,
                        S.kv, stats, part);
     if (S.kv.splits > 1) {
         launch_sum<T>(part, 2 * S.all_k, S.kv.splits, g->grad_k, S.all_k, st);

@@ -55,6 +55,9 @@ struct AttendPlan {
     uint32_t q_and, q_xor;   // scale's sign (and zero) applied to the bits of q: c stays positive
 };
 
+// Grids are two-dimensional, so that one workgroup an item never meets a grid's limits.
+__device__ __forceinline__ int64_t block_id() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }
+
 // query position and head of row r < 2^31: the quotient from inv_share is at most one too small
 __device__ __forceinline__ void split_row(const AttendPlan& P, int64_t kh, uint32_t r, int64_t* t, int64_t* h) {
     uint32_t q = __umulhi(r, P.inv_share), g = r - q * P.share;
@@ -397,85 +400,85 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void attend_stream_kernel(ar
     T* tile = tiles[wave];
     const int dim = (int)A.dim;
     const int64_t waves = P.items * P.splits;
-    for (int64_t w = (int64_t)blockIdx.x * 4 + wave; w < waves; w += (int64_t)gridDim.x * 4) {
-        const int split = (int)(w % P.splits);
-        const int64_t item = w / P.splits, rb = item % P.row_blocks, bk = item / P.row_blocks;
-        const int64_t kh = bk % A.kv_heads, b = bk / A.kv_heads, r0 = rb * 32 * QB + (lane & 31);
-        V8 q[QB][DP / 16];
-        f32x16 o[QB][DP / 32];
-        float m[QB], l[QB];
+    const int64_t w = block_id() * 4 + wave;
+    if (w >= waves) return;   // no barrier in this kernel
+    const int split = (int)(w % P.splits);
+    const int64_t item = w / P.splits, rb = item % P.row_blocks, bk = item / P.row_blocks;
+    const int64_t kh = bk % A.kv_heads, b = bk / A.kv_heads, r0 = rb * 32 * QB + (lane & 31);
+    V8 q[QB][DP / 16];
+    f32x16 o[QB][DP / 32];
+    float m[QB], l[QB];
 #pragma unroll
-        for (int x = 0; x < QB; ++x) {
-            load_q<T, DP>(A, P, (const T*)A.q, A.q_batch, A.q_row, A.q_head, b, kh, r0 + 32 * x, half, P.q_and, P.q_xor, q[x]);
-            m[x] = -INFINITY;
-            l[x] = 0.0f;
+    for (int x = 0; x < QB; ++x) {
+        load_q<T, DP>(A, P, (const T*)A.q, A.q_batch, A.q_row, A.q_head, b, kh, r0 + 32 * x, half, P.q_and, P.q_xor, q[x]);
+        m[x] = -INFINITY;
+        l[x] = 0.0f;
 #pragma unroll
-            for (int db = 0; db < DP / 32; ++db) o[x][db] = f32x16{};
-        }
-        const T* kbase = (const T*)A.k + b * A.k_batch + kh * A.k_head + (int64_t)(lane & 31) * A.k_row + 8 * half;
-        // V: 8 or 16 lanes per row
-        constexpr int CH = DP / 8, VR = 64 / CH, VN = 32 / VR;
-        const int vrow = lane / CH, vchunk = lane % CH;
-        const T* vbase = (const T*)A.v + b * A.v_batch + kh * A.v_head + (int64_t)vrow * A.v_row + 8 * vchunk;
-        V8 kr[DP / 16], vr[VN];
-        Walk<32> walk;
-        walk.start(A, b, split, P.splits);
-        auto load = [&]() {
-            const int left = walk.n - walk.j0;
-            const T* kp = kbase + walk.p * A.k_passage + walk.j0 * A.k_row;
-            const T* vp = vbase + walk.p * A.v_passage + walk.j0 * A.v_row;
-#pragma unroll
-            for (int s = 0; s < DP / 16; ++s) kr[s] = load8<T>(kp + 16 * s, (lane & 31) < left && 16 * s + 8 * half < dim);
-#pragma unroll
-            for (int x = 0; x < VN; ++x) vr[x] = load8<T>(vp + (int64_t)x * VR * A.v_row, vrow + x * VR < left && 8 * vchunk < dim);
-        };
-        bool more = walk.settle();
-        if (more) load();
-        while (more) {
-            const int left = walk.n - walk.j0;
-            f32x16 s[QB][1];
-#pragma unroll
-            for (int x = 0; x < QB; ++x) s[x][0] = f32x16{};
-#pragma unroll
-            for (int k = 0; k < DP / 16; ++k)
-#pragma unroll
-                for (int x = 0; x < QB; ++x) s[x][0] = Mma<T>::mul(kr[k], q[x][k], s[x][0]);
-#pragma unroll
-            for (int x = 0; x < VN; ++x) {
-                const int row = vrow + x * VR;
-                *(V8*)(tile + row * DP + tile_chunk<DP>(row, vchunk) * 8) = vr[x];
-            }
-            walk.advance();
-            more = walk.settle();
-            if (more) load();
-#pragma unroll
-            for (int x = 0; x < QB; ++x) softmax_tile<T, 1, DP / 32>(s[x], P.c, left, half, m[x], l[x], o[x]);
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // the tile is written: LDS keeps a wave's order
-            const uint32_t vcol = opaque(lds_offset(tile) + columns_base<DP>(lane));
-#pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-                V8 pw[QB];
-#pragma unroll
-                for (int x = 0; x < QB; ++x) pw[x] = weights8<T>(s[x][0], ks);
-#pragma unroll
-                for (int db = 0; db < DP / 32; ++db) {
-                    const V8 vt = lds_columns<T, DP>(vcol, 16 * ks, db);
-#pragma unroll
-                    for (int x = 0; x < QB; ++x) o[x][db] = Mma<T>::mul(vt, pw[x], o[x][db]);
-                }
-            }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        }
-#pragma unroll
-        for (int x = 0; x < QB; ++x) finish_rows<T, DP>(A, P, W, b, kh, r0 + 32 * x, split, half, m[x], l[x], o[x]);
+        for (int db = 0; db < DP / 32; ++db) o[x][db] = f32x16{};
     }
+    const T* kbase = (const T*)A.k + b * A.k_batch + kh * A.k_head + (int64_t)(lane & 31) * A.k_row + 8 * half;
+    // V: 8 or 16 lanes per row
+    constexpr int CH = DP / 8, VR = 64 / CH, VN = 32 / VR;
+    const int vrow = lane / CH, vchunk = lane % CH;
+    const T* vbase = (const T*)A.v + b * A.v_batch + kh * A.v_head + (int64_t)vrow * A.v_row + 8 * vchunk;
+    V8 kr[DP / 16], vr[VN];
+    Walk<32> walk;
+    walk.start(A, b, split, P.splits);
+    auto load = [&]() {
+        const int left = walk.n - walk.j0;
+        const T* kp = kbase + walk.p * A.k_passage + walk.j0 * A.k_row;
+        const T* vp = vbase + walk.p * A.v_passage + walk.j0 * A.v_row;
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) kr[s] = load8<T>(kp + 16 * s, (lane & 31) < left && 16 * s + 8 * half < dim);
+#pragma unroll
+        for (int x = 0; x < VN; ++x) vr[x] = load8<T>(vp + (int64_t)x * VR * A.v_row, vrow + x * VR < left && 8 * vchunk < dim);
+    };
+    bool more = walk.settle();
+    if (more) load();
+    while (more) {
+        const int left = walk.n - walk.j0;
+        f32x16 s[QB][1];
+#pragma unroll
+        for (int x = 0; x < QB; ++x) s[x][0] = f32x16{};
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k)
+#pragma unroll
+            for (int x = 0; x < QB; ++x) s[x][0] = Mma<T>::mul(kr[k], q[x][k], s[x][0]);
+#pragma unroll
+        for (int x = 0; x < VN; ++x) {
+            const int row = vrow + x * VR;
+            *(V8*)(tile + row * DP + tile_chunk<DP>(row, vchunk) * 8) = vr[x];
+        }
+        walk.advance();
+        more = walk.settle();
+        if (more) load();
+#pragma unroll
+        for (int x = 0; x < QB; ++x) softmax_tile<T, 1, DP / 32>(s[x], P.c, left, half, m[x], l[x], o[x]);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // the tile is written: LDS keeps a wave's order
+        const uint32_t vcol = opaque(lds_offset(tile) + columns_base<DP>(lane));
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            V8 pw[QB];
+#pragma unroll
+            for (int x = 0; x < QB; ++x) pw[x] = weights8<T>(s[x][0], ks);
+#pragma unroll
+            for (int db = 0; db < DP / 32; ++db) {
+                const V8 vt = lds_columns<T, DP>(vcol, 16 * ks, db);
+#pragma unroll
+                for (int x = 0; x < QB; ++x) o[x][db] = Mma<T>::mul(vt, pw[x], o[x][db]);
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+#pragma unroll
+    for (int x = 0; x < QB; ++x) finish_rows<T, DP>(A, P, W, b, kh, r0 + 32 * x, split, half, m[x], l[x], o[x]);
 }
 
 // ---- many rows: four waves share the tiles --------------------------------------------------------------
 // Workgroups of one (batch entry, key head) sit on one XCD, whose L2 then serves its states.
 __device__ __forceinline__ int64_t xcd_item(int64_t id, int64_t items) {
     const int64_t per = (items + 7) / 8;
-    return (id & 7) * per + (id >> 3);
+    return (id >> 3) < per ? (id & 7) * per + (id >> 3) : items;
 }
 
 // Brings tiles of KB x 32 states into a ring of LDS: 1 KiB pieces, PW of a tile for each of NW waves.  States behind
@@ -483,16 +486,13 @@ __device__ __forceinline__ int64_t xcd_item(int64_t id, int64_t items) {
 template <typename T, int DP, int KB, int NW>
 struct TileFetch {
     static constexpr int CH = DP / 8, PR = 64 / CH, PW = 32 * KB / PR / NW;   // chunks per row, rows per piece
-    int row, col, lane, wave;
-    __device__ __forceinline__ void start(int w) {
-        lane = threadIdx.x & 63;
-        wave = w;
-        row = lane / CH;
-        col = lane % CH;
-    }
+    int wave;
+    __device__ __forceinline__ void start(int w) { wave = w; }
     // src: state 0 of the tile; left: states from there to the passage's end; stride below 2^24
     __device__ __forceinline__ void fetch(const T* src, int64_t stride, int left, int dim, uint32_t tile) const {
         const bool full = left >= 32 * KB;   // uniform
+        // from the lane's number anew each time: the offsets of all pieces would not fit beside the accumulators
+        const int lane = (int)opaque(threadIdx.x & 63), row = lane / CH, col = lane % CH;
         const uint32_t bytes = (uint32_t)row * (uint32_t)stride * 2;
 #pragma unroll
         for (int x = 0; x < PW; ++x) {
@@ -525,78 +525,72 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(artread_attend_t A,
         __syncthreads();
     }
     const int64_t total = P.items * P.splits;
-    for (int64_t id = blockIdx.x; id < (total + 7) / 8 * 8; id += gridDim.x) {
-        const int64_t w = xcd_item(id, total);
-        if (w >= total) continue;
-        if (id != blockIdx.x) {   // the tiles of the item before are read
-            dma_wait<0>();
-            wave_meet();
+    const int64_t w = xcd_item(block_id(), total);
+    if (w >= total) return;
+    const int64_t rb = w % P.row_blocks, other = w / P.row_blocks;
+    const int split = (int)(other % P.splits);
+    const int64_t bk = other / P.splits, kh = bk % A.kv_heads, b = bk / A.kv_heads;
+    const int64_t r = (rb * 4 + wave) * 32 + (lane & 31);
+    const T* kbase = (const T*)A.k + b * A.k_batch + kh * A.k_head;
+    const T* vbase = (const T*)A.v + b * A.v_batch + kh * A.v_head;
+    Walk<32 * KB> walk;   // of the tiles fetched; `left` of the one worked on
+    walk.start(A, b, split, P.splits);
+    auto fetch = [&](int stage) {   // keys of the tile, 0 behind the last
+        if (!walk.settle()) return 0;
+        const int left = walk.n - walk.j0;
+        fetcher.fetch(kbase + walk.p * A.k_passage + walk.j0 * A.k_row, A.k_row, left, dim, lds_offset(ring[stage]));
+        fetcher.fetch(vbase + walk.p * A.v_passage + walk.j0 * A.v_row, A.v_row, left, dim, lds_offset(ring[2 + stage]));
+        walk.advance();
+        return left;
+    };
+    int left = fetch(0);
+    V8 q[DP / 16];
+    f32x16 o[DP / 32];
+    float m = -INFINITY, l = 0.0f;
+    load_q<T, DP>(A, P, (const T*)A.q, A.q_batch, A.q_row, A.q_head, b, kh, r, half, P.q_and, P.q_xor, q);
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db) o[db] = f32x16{};
+    int stage = 0;
+    while (left) {
+        dma_wait<0>();
+        wave_meet();   // everyone's pieces are there, and everyone is done with the tile before
+        const int next = fetch(stage ^ 1);
+        const uint32_t krow = opaque(lds_offset(ring[stage]) + rows_base<DP>(lane));
+        const uint32_t vcol = opaque(lds_offset(ring[2 + stage]) + columns_base<DP>(lane));
+        f32x16 s[KB];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) s[kb] = f32x16{};
+        constexpr int NK = KB * DP / 16, NV = 2 * KB * DP / 32, EARLY = NV < 8 ? NV : 8, AHEAD = NK < 6 ? NK : 6;
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k)
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) s[kb] = Mma<T>::mul(lds_rows<T, DP>(krow, kb, k), q[k], s[kb]);
+        // the first operands of the second product are on their way while the softmax runs
+        V8 vt[NV];
+#pragma unroll
+        for (int i = 0; i < EARLY; ++i) vt[i] = lds_columns<T, DP>(vcol, 16 * (i / (DP / 32)), i % (DP / 32));
+        __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);   // LDS reads ahead, then one per product
+#pragma unroll
+        for (int i = 0; i < NK - AHEAD; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         }
-        const int64_t rb = w % P.row_blocks, other = w / P.row_blocks;
-        const int split = (int)(other % P.splits);
-        const int64_t bk = other / P.splits, kh = bk % A.kv_heads, b = bk / A.kv_heads;
-        const int64_t r = (rb * 4 + wave) * 32 + (lane & 31);
-        const T* kbase = (const T*)A.k + b * A.k_batch + kh * A.k_head;
-        const T* vbase = (const T*)A.v + b * A.v_batch + kh * A.v_head;
-        Walk<32 * KB> walk;   // of the tiles fetched; `left` of the one worked on
-        walk.start(A, b, split, P.splits);
-        auto fetch = [&](int stage) {   // keys of the tile, 0 behind the last
-            if (!walk.settle()) return 0;
-            const int left = walk.n - walk.j0;
-            fetcher.fetch(kbase + walk.p * A.k_passage + walk.j0 * A.k_row, A.k_row, left, dim, lds_offset(ring[stage]));
-            fetcher.fetch(vbase + walk.p * A.v_passage + walk.j0 * A.v_row, A.v_row, left, dim, lds_offset(ring[2 + stage]));
-            walk.advance();
-            return left;
-        };
-        int left = fetch(0);
-        V8 q[DP / 16];
-        f32x16 o[DP / 32];
-        float m = -INFINITY, l = 0.0f;
-        load_q<T, DP>(A, P, (const T*)A.q, A.q_batch, A.q_row, A.q_head, b, kh, r, half, P.q_and, P.q_xor, q);
 #pragma unroll
-        for (int db = 0; db < DP / 32; ++db) o[db] = f32x16{};
-        int stage = 0;
-        while (left) {
-            dma_wait<0>();
-            wave_meet();   // everyone's pieces are there, and everyone is done with the tile before
-            const int next = fetch(stage ^ 1);
-            const uint32_t krow = opaque(lds_offset(ring[stage]) + rows_base<DP>(lane));
-            const uint32_t vcol = opaque(lds_offset(ring[2 + stage]) + columns_base<DP>(lane));
-            f32x16 s[KB];
-#pragma unroll
-            for (int kb = 0; kb < KB; ++kb) s[kb] = f32x16{};
-            constexpr int NK = KB * DP / 16, NV = 2 * KB * DP / 32, EARLY = NV < 8 ? NV : 8, AHEAD = NK < 6 ? NK : 6;
-#pragma unroll
-            for (int k = 0; k < DP / 16; ++k)
-#pragma unroll
-                for (int kb = 0; kb < KB; ++kb) s[kb] = Mma<T>::mul(lds_rows<T, DP>(krow, kb, k), q[k], s[kb]);
-            // the first operands of the second product are on their way while the softmax runs
-            V8 vt[NV];
-#pragma unroll
-            for (int i = 0; i < EARLY; ++i) vt[i] = lds_columns<T, DP>(vcol, 16 * (i / (DP / 32)), i % (DP / 32));
-            __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);   // LDS reads ahead, then one per product
-#pragma unroll
-            for (int i = 0; i < NK - AHEAD; ++i) {
-                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-            }
-#pragma unroll
-            for (int i = 0; i < AHEAD; ++i) {
-                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-            }
-            softmax_tile<T, KB, DP / 32>(s, P.c, left, half, m, l, o);
-#pragma unroll
-            for (int i = EARLY; i < NV; ++i) vt[i] = lds_columns<T, DP>(vcol, 16 * (i / (DP / 32)), i % (DP / 32));
-#pragma unroll
-            for (int ks = 0; ks < 2 * KB; ++ks) {
-                const V8 pw = weights8<T>(s[ks >> 1], ks & 1);
-#pragma unroll
-                for (int db = 0; db < DP / 32; ++db) o[db] = Mma<T>::mul(vt[ks * (DP / 32) + db], pw, o[db]);
-            }
-            left = next;
-            stage ^= 1;
+        for (int i = 0; i < AHEAD; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
         }
-        finish_rows<T, DP>(A, P, W, b, kh, r, split, half, m, l, o);
+        softmax_tile<T, KB, DP / 32>(s, P.c, left, half, m, l, o);
+#pragma unroll
+        for (int i = EARLY; i < NV; ++i) vt[i] = lds_columns<T, DP>(vcol, 16 * (i / (DP / 32)), i % (DP / 32));
+#pragma unroll
+        for (int ks = 0; ks < 2 * KB; ++ks) {
+            const V8 pw = weights8<T>(s[ks >> 1], ks & 1);
+#pragma unroll
+            for (int db = 0; db < DP / 32; ++db) o[db] = Mma<T>::mul(vt[ks * (DP / 32) + db], pw, o[db]);
+        }
+        left = next;
+        stage ^= 1;
     }
+    finish_rows<T, DP>(A, P, W, b, kh, r, split, half, m, l, o);
 }

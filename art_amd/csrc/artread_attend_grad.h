@@ -88,6 +88,40 @@ struct Spread<f16> {
     }
 };
 
+// The same with one power of two for a whole wave's dS, where its columns are not the accumulators' ones.
+template <typename T>
+struct SpreadAll {
+    __device__ __forceinline__ float inverse() const { return 1.0f; }
+    __device__ __forceinline__ float times(float x) const { return x; }
+    template <int N>
+    __device__ __forceinline__ void fit(const f32x16&, f32x16 (&)[N]) {}
+};
+template <>
+struct SpreadAll<f16> {
+    float f = 1.0f, most = 0.0f;
+    __device__ __forceinline__ float inverse() const { return 1.0f / f; }
+    __device__ __forceinline__ float times(float x) const { return x * f; }
+    template <int N>
+    __device__ __forceinline__ void fit(const f32x16& ds, f32x16 (&acc)[N]) {
+        float top = fabsf(ds[0]);
+#pragma unroll
+        for (int i = 1; i < 16; ++i) top = fmaxf(top, fabsf(ds[i]));
+        if (__any(top > most)) {
+#pragma unroll
+            for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+            int e = 10 - ilogbf(top);
+            e = e < -100 ? -100 : (e > 100 ? 100 : e);
+            const float g = ldexpf(1.0f, e), change = most == 0.0f ? 0.0f : g / f;
+            f = g;
+            most = ldexpf(1.0f, 14 - e);
+#pragma unroll
+            for (int x = 0; x < N; ++x)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[x][i] *= change;
+        }
+    }
+};
+
 template <typename T>
 __device__ __forceinline__ void put4(T* p, const float* x) {
     Vec<T, 4> w;
@@ -115,91 +149,85 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_grad_q_kernel(artread_atten
         __syncthreads();
     }
     const int64_t total = P.items * P.splits;
-    for (int64_t id = blockIdx.x; id < (total + 7) / 8 * 8; id += gridDim.x) {
-        const int64_t w = xcd_item(id, total);
-        if (w >= total) continue;
-        if (id != blockIdx.x) {   // the tiles of the item before are read
-            dma_wait<0>();
-            wave_meet();
-        }
-        const int64_t rb = w % P.row_blocks, other = w / P.row_blocks;
-        const int split = (int)(other % P.splits);
-        const int64_t bk = other / P.splits, kh = bk % A.kv_heads, b = bk / A.kv_heads;
-        const int64_t r = (rb * NW + wave) * 32 + (lane & 31);
-        const T* kbase = (const T*)A.k + b * A.k_batch + kh * A.k_head;
-        const T* vbase = (const T*)A.v + b * A.v_batch + kh * A.v_head;
-        Walk<32 * KB> walk;   // of the tiles fetched; `left` of the one worked on
-        walk.start(A, b, split, P.splits);
-        auto fetch = [&](int stage) {   // keys of the tile, 0 behind the last
-            if (!walk.settle()) return 0;
-            const int left = walk.n - walk.j0;
-            fetcher.fetch(kbase + walk.p * A.k_passage + walk.j0 * A.k_row, A.k_row, left, dim, lds_offset(ring[stage]));
-            fetcher.fetch(vbase + walk.p * A.v_passage + walk.j0 * A.v_row, A.v_row, left, dim, lds_offset(ring[2 + stage]));
-            walk.advance();
-            return left;
-        };
-        int left = fetch(0);
-        V8 q[DP / 16], g[DP / 16];
-        load_q<T, DP>(A, P, (const T*)A.q, A.q_batch, A.q_row, A.q_head, b, kh, r, half, P.q_and, P.q_xor, q);
-        load_q<T, DP>(A, P, (const T*)G.grad_out, G.g_batch, G.g_row, G.g_head, b, kh, r, half, 0xffffffffu, 0u, g);
-        RowStat st{INFINITY, 0.0f};
-        if (r < P.row_count) st = stats[bk * P.pad_rows + r];
-        f32x16 acc[DP / 32];
-        Spread<T> spread;
+    const int64_t w = xcd_item(block_id(), total);
+    if (w >= total) return;
+    const int64_t rb = w % P.row_blocks, other = w / P.row_blocks;
+    const int split = (int)(other % P.splits);
+    const int64_t bk = other / P.splits, kh = bk % A.kv_heads, b = bk / A.kv_heads;
+    const int64_t r = (rb * NW + wave) * 32 + (lane & 31);
+    const T* kbase = (const T*)A.k + b * A.k_batch + kh * A.k_head;
+    const T* vbase = (const T*)A.v + b * A.v_batch + kh * A.v_head;
+    Walk<32 * KB> walk;   // of the tiles fetched; `left` of the one worked on
+    walk.start(A, b, split, P.splits);
+    auto fetch = [&](int stage) {   // keys of the tile, 0 behind the last
+        if (!walk.settle()) return 0;
+        const int left = walk.n - walk.j0;
+        fetcher.fetch(kbase + walk.p * A.k_passage + walk.j0 * A.k_row, A.k_row, left, dim, lds_offset(ring[stage]));
+        fetcher.fetch(vbase + walk.p * A.v_passage + walk.j0 * A.v_row, A.v_row, left, dim, lds_offset(ring[2 + stage]));
+        walk.advance();
+        return left;
+    };
+    int left = fetch(0);
+    V8 q[DP / 16], g[DP / 16];
+    load_q<T, DP>(A, P, (const T*)A.q, A.q_batch, A.q_row, A.q_head, b, kh, r, half, P.q_and, P.q_xor, q);
+    load_q<T, DP>(A, P, (const T*)G.grad_out, G.g_batch, G.g_row, G.g_head, b, kh, r, half, 0xffffffffu, 0u, g);
+    RowStat st{INFINITY, 0.0f};
+    if (r < P.row_count) st = stats[bk * P.pad_rows + r];
+    f32x16 acc[DP / 32];
+    Spread<T> spread;
 #pragma unroll
-        for (int db = 0; db < DP / 32; ++db) acc[db] = f32x16{};
-        int stage = 0;
-        while (left) {
-            dma_wait<0>();
-            wave_meet();   // everyone's pieces are there, and everyone is done with the tile before
-            const int next = fetch(stage ^ 1);
-            const uint32_t krow = opaque(lds_offset(ring[stage]) + rows_base<DP>(lane));
-            const uint32_t kcol = opaque(lds_offset(ring[stage]) + columns_base<DP>(lane));
+    for (int db = 0; db < DP / 32; ++db) acc[db] = f32x16{};
+    int stage = 0;
+    while (left) {
+        dma_wait<0>();
+        wave_meet();   // everyone's pieces are there, and everyone is done with the tile before
+        const int next = fetch(stage ^ 1);
+        const uint32_t krow = opaque(lds_offset(ring[stage]) + rows_base<DP>(lane));
+        const uint32_t kcol = opaque(lds_offset(ring[stage]) + columns_base<DP>(lane));
 #pragma unroll
-            for (int kb = 0; kb < KB; ++kb) {
-                f32x16 s = f32x16{}, dp = f32x16{};
+        for (int kb = 0; kb < KB; ++kb) {
+            f32x16 s = f32x16{}, dp = f32x16{};
 #pragma unroll
-                for (int k = 0; k < DP / 16; ++k) {
-                    s = Mma<T>::mul(lds_rows<T, DP>(krow, kb, k), q[k], s);
-                    dp = Mma<T>::mul(lds_rows<T, DP>(krow, 2 * KB + kb, k), g[k], dp);
-                }
-#pragma unroll
-                for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], P.c, -st.x)) * (dp[i] - st.delta);
-                if (left < 32 * KB) {
-                    const int mine = left - 4 * half;
-                    asm volatile("");   // a branch: most tiles are whole
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        if (32 * kb + 8 * (i >> 2) + (i & 3) >= mine) s[i] = 0.0f;
-                }
-                spread.fit(s, acc);
-#pragma unroll
-                for (int ks = 0; ks < 2; ++ks) {
-                    const V8 ds = weights8<T>(s, ks);
-#pragma unroll
-                    for (int db = 0; db < DP / 32; ++db)
-                        acc[db] = Mma<T>::mul(lds_columns<T, DP>(kcol, 32 * kb + 16 * ks, db), ds, acc[db]);
-                }
+            for (int k = 0; k < DP / 16; ++k) {
+                s = Mma<T>::mul(lds_rows<T, DP>(krow, kb, k), q[k], s);
+                dp = Mma<T>::mul(lds_rows<T, DP>(krow, 2 * KB + kb, k), g[k], dp);
             }
-            left = next;
-            stage ^= 1;
-        }
-        if (r < P.row_count) {
-            int64_t t, h;
-            split_row(P, kh, (uint32_t)r, &t, &h);
-            const int64_t at = ((b * A.rows + t) * A.heads + h) * dim;
-            const float f = A.scale * spread.inverse() * P.unweight;
 #pragma unroll
-            for (int db = 0; db < DP / 32; ++db)
+            for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], P.c, -st.x)) * (dp[i] - st.delta);
+            if (left < 32 * KB) {
+                const int mine = left - 4 * half;
+                asm volatile("");   // a branch: most tiles are whole
 #pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    const int d = 32 * db + 8 * x + 4 * half;
-                    const float y[4] = {f * acc[db][4 * x], f * acc[db][4 * x + 1], f * acc[db][4 * x + 2], f * acc[db][4 * x + 3]};
-                    if (d >= dim) continue;
-                    if (P.splits > 1) *(float4*)(part + split * (A.batch * A.rows * A.heads * dim) + at + d) = make_float4(y[0], y[1], y[2], y[3]);
-                    else put4<T>((T*)G.grad_q + at + d, y);
-                }
+                for (int i = 0; i < 16; ++i)
+                    if (32 * kb + 8 * (i >> 2) + (i & 3) >= mine) s[i] = 0.0f;
+            }
+            spread.fit(s, acc);
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                const V8 ds = weights8<T>(s, ks);
+#pragma unroll
+                for (int db = 0; db < DP / 32; ++db)
+                    acc[db] = Mma<T>::mul(lds_columns<T, DP>(kcol, 32 * kb + 16 * ks, db), ds, acc[db]);
+            }
         }
+        left = next;
+        stage ^= 1;
+    }
+    if (r < P.row_count) {
+        int64_t t, h;
+        split_row(P, kh, (uint32_t)r, &t, &h);
+        const int64_t at = ((b * A.rows + t) * A.heads + h) * dim;
+        const float f = A.scale * spread.inverse() * P.unweight;
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const int d = 32 * db + 8 * x + 4 * half;
+                const float y[4] = {f * acc[db][4 * x], f * acc[db][4 * x + 1], f * acc[db][4 * x + 2], f * acc[db][4 * x + 3]};
+                if (d >= dim) continue;
+                if (P.splits > 1) *(float4*)(part + split * (A.batch * A.rows * A.heads * dim) + at + d) = make_float4(y[0], y[1], y[2], y[3]);
+                else put4<T>((T*)G.grad_q + at + d, y);
+            }
     }
 }
 
@@ -219,158 +247,404 @@ __global__ __launch_bounds__(256, 2) void attend_grad_kv_kernel(artread_attend_t
     const int dim = (int)A.dim;
     const int64_t key_blocks = (A.len + 127) / 128;
     const int64_t total = P.items * P.splits;   // batch x passages x key_blocks x kv_heads x splits
-    for (int64_t id = blockIdx.x; id < (total + 7) / 8 * 8; id += gridDim.x) {
-        // Many rows: the workgroups of one key head stand together on an XCD, whose L2 then serves its rows.  Few:
-        // the key heads of a state, neighbours in memory, are read side by side.
-        int64_t item = P.by_head ? xcd_item(id, total) : id;
-        if (item >= total) continue;
-        if (id != blockIdx.x) {   // the tiles of the item before are read
-            dma_wait<0>();
-            wave_meet();
-        }
-        const int split = (int)(item % P.splits);
-        item /= P.splits;
-        int64_t kh = 0;
-        if (!P.by_head) {
-            kh = item % A.kv_heads;
-            item /= A.kv_heads;
-        }
-        const int64_t j0 = item % key_blocks * 128;
-        item /= key_blocks;
-        const int64_t p = item % A.passages;
-        item /= A.passages;
-        if (P.by_head) {
-            kh = item % A.kv_heads;
-            item /= A.kv_heads;
-        }
-        const int64_t b = item;
-        int n = (int)A.len;
-        if (A.lengths) {
-            const int x = uniform(A.lengths[b * A.passages + p]);
-            n = x < n ? x : n;
-        }
-        const int64_t j = j0 + 32 * wave + (lane & 31);
-        f32x16 dk[DP / 32], dv[DP / 32];
-        Spread<T> spread;
+    const int64_t id = block_id();
+    // Many rows: the workgroups of one key head stand together on an XCD, whose L2 then serves its rows.  Few:
+    // the key heads of a state, neighbours in memory, are read side by side.
+    int64_t item = P.by_head ? xcd_item(id, total) : id;
+    if (item >= total) return;
+    const int split = (int)(item % P.splits);
+    item /= P.splits;
+    int64_t kh = 0;
+    if (!P.by_head) {
+        kh = item % A.kv_heads;
+        item /= A.kv_heads;
+    }
+    const int64_t j0 = item % key_blocks * 128;
+    item /= key_blocks;
+    const int64_t p = item % A.passages;
+    item /= A.passages;
+    if (P.by_head) {
+        kh = item % A.kv_heads;
+        item /= A.kv_heads;
+    }
+    const int64_t b = item;
+    int n = (int)A.len;
+    if (A.lengths) {
+        const int x = uniform(A.lengths[b * A.passages + p]);
+        n = x < n ? x : n;
+    }
+    const int64_t j = j0 + 32 * wave + (lane & 31);
+    f32x16 dk[DP / 32], dv[DP / 32];
+    Spread<T> spread;
 #pragma unroll
-        for (int db = 0; db < DP / 32; ++db) dk[db] = dv[db] = f32x16{};
-        if (j0 < n) {   // uniform over the workgroup
-            V8 kf[DP / 16], vf[DP / 16];
-            const T* kp = (const T*)A.k + b * A.k_batch + p * A.k_passage + j * A.k_row + kh * A.k_head + 8 * half;
-            const T* vp = (const T*)A.v + b * A.v_batch + p * A.v_passage + j * A.v_row + kh * A.v_head + 8 * half;
+    for (int db = 0; db < DP / 32; ++db) dk[db] = dv[db] = f32x16{};
+    if (j0 < n) {   // uniform over the workgroup
+        V8 kf[DP / 16], vf[DP / 16];
+        const T* kp = (const T*)A.k + b * A.k_batch + p * A.k_passage + j * A.k_row + kh * A.k_head + 8 * half;
+        const T* vp = (const T*)A.v + b * A.v_batch + p * A.v_passage + j * A.v_row + kh * A.v_head + 8 * half;
 #pragma unroll
-            for (int s = 0; s < DP / 16; ++s) {
-                const bool ok = j < n && 16 * s + 8 * half < dim;
-                union {
-                    V8 v;
-                    uint32_t u[4];
-                } x;
-                x.v = load8<T>(kp + 16 * s, ok);
+        for (int s = 0; s < DP / 16; ++s) {
+            const bool ok = j < n && 16 * s + 8 * half < dim;
+            kf[s] = load8<T>(kp + 16 * s, ok);
+            vf[s] = load8<T>(vp + 16 * s, ok);
+        }
+        // pieces of 1 KiB: PR rows each, PW of a tile for each wave; rows that are not there repeat the last one
+        // (their weight is zero), columns behind dim the first (they meet zeros of K and V)
+        constexpr int CH = DP / 8, PR = 64 / CH, PW = 32 / PR / 4;
+        const int prow = lane / CH, tiles = (int)((P.row_count + 31) / 32);
+        const RowStat* sp = stats + (b * A.kv_heads + kh) * P.pad_rows;
+        const T* qb = (const T*)A.q + b * A.q_batch + kh * P.share * A.q_head;
+        const T* gb = (const T*)G.grad_out + b * G.g_batch + kh * P.share * G.g_head;
+        auto fetch = [&](int tile, int stage) {
+            int64_t t0, h0;
+            split_row(P, 0, (uint32_t)tile * 32, &t0, &h0);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x.u[e] = (x.u[e] & P.q_and) ^ P.q_xor;   // scale's sign, on this side of S
-                kf[s] = x.v;
-                vf[s] = load8<T>(vp + 16 * s, ok);
+            for (int x = 0; x < PW; ++x) {
+                const int piece = wave * PW + x, row = piece * PR + prow;
+                int64_t r = (int64_t)tile * 32 + row, t, h;
+                r = r < P.row_count ? r : P.row_count - 1;
+                split_row(P, 0, (uint32_t)r, &t, &h);
+                int col = tile_chunk<DP>(row, lane % CH) * 8;
+                col = col < dim ? col : 0;
+                // bytes from the tile's first query position: a tile spans at most 32 of them
+                const uint32_t dt = (uint32_t)t - (uint32_t)t0;
+                dma16(qb + t0 * A.q_row, (dt * (uint32_t)A.q_row + (uint32_t)(h * A.q_head) + col) * 2, lds_offset(&qtile[stage][piece * 512]));
+                dma16(gb + t0 * G.g_row, (dt * (uint32_t)G.g_row + (uint32_t)(h * G.g_head) + col) * 2, lds_offset(&qtile[STAGES + stage][piece * 512]));
             }
-            // pieces of 1 KiB: PR rows each, PW of a tile for each wave; rows that are not there repeat the last one
-            // (their weight is zero), columns behind dim the first (they meet zeros of K and V)
-            constexpr int CH = DP / 8, PR = 64 / CH, PW = 32 / PR / 4;
-            const int prow = lane / CH, tiles = (int)((P.row_count + 31) / 32);
-            const RowStat* sp = stats + (b * A.kv_heads + kh) * P.pad_rows;
-            const T* qb = (const T*)A.q + b * A.q_batch + kh * P.share * A.q_head;
-            const T* gb = (const T*)G.grad_out + b * G.g_batch + kh * P.share * G.g_head;
-            auto fetch = [&](int tile, int stage) {
-                int64_t t0, h0;
-                split_row(P, 0, (uint32_t)tile * 32, &t0, &h0);
+            dma4(sp + tile * 32, (uint32_t)lane * 4, lds_offset(&stile[stage][wave][0]));
+        };
+        constexpr int LOADS = 2 * PW + 1;
+        if (split < tiles) fetch(split, 0);
+        if (split + P.splits < tiles) fetch(split + P.splits, 1);
+        // one loop for waves with keys and one for those without: both load and meet at the barriers
+        auto go = [&](auto with_keys) {
+            int stage = 0;
+            for (int tile = split; tile < tiles; tile += P.splits) {
+                if (tile + P.splits < tiles) dma_wait<LOADS>();   // all but the next tile's
+                else dma_wait<0>();
+                wave_meet();   // everyone's pieces are there, and everyone is done with the tile before
+                const int ahead = stage == 0 ? 2 : stage - 1;
+                if (tile + 2 * P.splits < tiles) fetch(tile + 2 * P.splits, ahead);
+                if constexpr (decltype(with_keys)::value) {
+                    const uint32_t qrow = opaque(lds_offset(qtile[stage]) + rows_base<DP>(lane));
+                    const uint32_t qcol = opaque(lds_offset(qtile[stage]) + columns_base<DP>(lane));
+                    f32x16 s = f32x16{}, dp = f32x16{};
 #pragma unroll
-                for (int x = 0; x < PW; ++x) {
-                    const int piece = wave * PW + x, row = piece * PR + prow;
-                    int64_t r = (int64_t)tile * 32 + row, t, h;
-                    r = r < P.row_count ? r : P.row_count - 1;
-                    split_row(P, 0, (uint32_t)r, &t, &h);
-                    int col = tile_chunk<DP>(row, lane % CH) * 8;
-                    col = col < dim ? col : 0;
-                    // bytes from the tile's first query position: a tile spans at most 32 of them
-                    const uint32_t dt = (uint32_t)t - (uint32_t)t0;
-                    dma16(qb + t0 * A.q_row, (dt * (uint32_t)A.q_row + (uint32_t)(h * A.q_head) + col) * 2, lds_offset(&qtile[stage][piece * 512]));
-                    dma16(gb + t0 * G.g_row, (dt * (uint32_t)G.g_row + (uint32_t)(h * G.g_head) + col) * 2, lds_offset(&qtile[STAGES + stage][piece * 512]));
-                }
-                dma4(sp + tile * 32, (uint32_t)lane * 4, lds_offset(&stile[stage][wave][0]));
-            };
-            constexpr int LOADS = 2 * PW + 1;
-            if (split < tiles) fetch(split, 0);
-            if (split + P.splits < tiles) fetch(split + P.splits, 1);
-            // one loop for waves with keys and one for those without: both load and meet at the barriers
-            auto go = [&](auto with_keys) {
-                int stage = 0;
-                for (int tile = split; tile < tiles; tile += P.splits) {
-                    if (tile + P.splits < tiles) dma_wait<LOADS>();   // all but the next tile's
-                    else dma_wait<0>();
-                    wave_meet();   // everyone's pieces are there, and everyone is done with the tile before
-                    const int ahead = stage == 0 ? 2 : stage - 1;
-                    if (tile + 2 * P.splits < tiles) fetch(tile + 2 * P.splits, ahead);
-                    if constexpr (decltype(with_keys)::value) {
-                        const uint32_t qrow = opaque(lds_offset(qtile[stage]) + rows_base<DP>(lane));
-                        const uint32_t qcol = opaque(lds_offset(qtile[stage]) + columns_base<DP>(lane));
-                        f32x16 s = f32x16{}, dp = f32x16{};
+                    for (int k = 0; k < DP / 16; ++k) {
+                        s = Mma<T>::mul(lds_rows<T, DP>(qrow, 0, k), kf[k], s);
+                        dp = Mma<T>::mul(lds_rows<T, DP>(qrow, STAGES, k), vf[k], dp);
+                    }
 #pragma unroll
-                        for (int k = 0; k < DP / 16; ++k) {
-                            s = Mma<T>::mul(lds_rows<T, DP>(qrow, 0, k), kf[k], s);
-                            dp = Mma<T>::mul(lds_rows<T, DP>(qrow, STAGES, k), vf[k], dp);
-                        }
+                    for (int x = 0; x < 4; ++x) {
+                        const float4 a = *(const float4*)&stile[stage][wave][8 * x + 4 * half];
+                        const float4 c = *(const float4*)&stile[stage][wave][8 * x + 4 * half + 2];
+                        const float xs[4] = {a.x, a.z, c.x, c.z}, ds[4] = {a.y, a.w, c.y, c.w};
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            const float4 a = *(const float4*)&stile[stage][wave][8 * x + 4 * half];
-                            const float4 c = *(const float4*)&stile[stage][wave][8 * x + 4 * half + 2];
-                            const float xs[4] = {a.x, a.z, c.x, c.z}, ds[4] = {a.y, a.w, c.y, c.w};
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const int i = 4 * x + e;
-                                s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], P.c, -xs[e]));
-                                dp[i] = s[i] * (dp[i] - ds[e]);
-                            }
-                        }
-                        spread.fit(dp, dk);
-#pragma unroll
-                        for (int ks = 0; ks < 2; ++ks) {
-                            const V8 pw = weights8<T>(s, ks), ds = weights8<T>(dp, ks);
-#pragma unroll
-                            for (int db = 0; db < DP / 32; ++db) {
-                                dv[db] = Mma<T>::mul(lds_columns<T, DP>(qcol, STAGES * 32 + 16 * ks, db), pw, dv[db]);
-                                dk[db] = Mma<T>::mul(lds_columns<T, DP>(qcol, 16 * ks, db), ds, dk[db]);
-                            }
+                        for (int e = 0; e < 4; ++e) {
+                            const int i = 4 * x + e;
+                            s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], P.c, -xs[e]));
+                            dp[i] = s[i] * (dp[i] - ds[e]);
                         }
                     }
-                    stage = stage == 2 ? 0 : stage + 1;
+                    spread.fit(dp, dk);
+#pragma unroll
+                    for (int ks = 0; ks < 2; ++ks) {
+                        const V8 pw = weights8<T>(s, ks), ds = weights8<T>(dp, ks);
+#pragma unroll
+                        for (int db = 0; db < DP / 32; ++db) {
+                            dv[db] = Mma<T>::mul(lds_columns<T, DP>(qcol, STAGES * 32 + 16 * ks, db), pw, dv[db]);
+                            dk[db] = Mma<T>::mul(lds_columns<T, DP>(qcol, 16 * ks, db), ds, dk[db]);
+                        }
+                    }
                 }
-            };
-            if (j0 + 32 * wave < n) go(std::true_type{});   // uniform over the wave
-            else go(std::false_type{});
+                stage = stage == 2 ? 0 : stage + 1;
+            }
+        };
+        if (j0 + 32 * wave < n) go(std::true_type{});   // uniform over the wave
+        else go(std::false_type{});
+    }
+    if (j < A.len) {
+        const int64_t at = (((b * A.passages + p) * A.len + j) * A.kv_heads + kh) * dim;
+        const int64_t all = A.batch * A.passages * A.len * A.kv_heads * dim;
+        const float fv = P.unweight, fk = A.scale * spread.inverse() * P.unweight;
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const int d = 32 * db + 8 * x + 4 * half;
+                if (d >= dim) continue;
+                float yk[4], yv[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {   // behind the length: zeros, whatever the accumulators hold
+                    yk[e] = j < n ? fk * dk[db][4 * x + e] : 0.0f;
+                    yv[e] = j < n ? fv * dv[db][4 * x + e] : 0.0f;
+                }
+                if (P.splits > 1) {
+                    *(float4*)(part + split * 2 * all + at + d) = make_float4(yk[0], yk[1], yk[2], yk[3]);
+                    *(float4*)(part + (split * 2 + 1) * all + at + d) = make_float4(yv[0], yv[1], yv[2], yv[3]);
+                } else {
+                    put4<T>((T*)G.grad_k + at + d, yk);
+                    put4<T>((T*)G.grad_v + at + d, yv);
+                }
+            }
+    }
+}
+
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+template <typename T>
+__device__ __forceinline__ u32x2 pack4(float a, float b, float c, float d) {
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    const T4 w = {(T)a, (T)b, (T)c, (T)d};
+    return __builtin_bit_cast(u32x2, w);
+}
+
+// ---- all three gradients at once: few rows -----------------------------------------------------------------
+// Up to 32 * RB rows per key head.  A wave walks tiles of 32 keys, those behind the lengths among them (they get their
+// zeros here), and finishes dK and dV of a tile before the next: every state is read once and every gradient written
+// once, which is what bounds this, where the two walks would read the states twice.  S^T and dP^T leave P^T and dS^T
+// as B operands over the keys, for dQ; dV and dK want them over the rows, so both go through a 32 x 32 tile of LDS and
+// come back by the transposing read.  A tile's results are stored once the next tile has arrived: waiting for that
+// tile then never waits for the stores.  The waves of a workgroup add their dQ in LDS, in order.
+template <typename T, int DP, int RB, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void attend_grad_stream_kernel(artread_attend_t A, artread_attend_grads_t G,
+                                                                        AttendPlan P, const RowStat* __restrict__ stats,
+                                                                        float* __restrict__ part) {
+    constexpr int TILE = 32 * DP, CH = DP / 8;
+    constexpr int SHARED = 2 * RB * TILE, OWN = 2 * TILE + 2 * 1024;   // elements: Q and dO; K, V, P and dS of a wave
+    constexpr int BYTES = (SHARED + NW * OWN) * 2, SUMS = NW * 32 * RB * DP * 4;
+    __shared__ __attribute__((aligned(1024))) char lds[BYTES > SUMS ? BYTES : SUMS];
+    typedef typename Mma<T>::V8 V8;
+    typedef __attribute__((address_space(3))) u32x2 lds_u32x2;
+    const int lane = threadIdx.x & 63, half = lane >> 5, wave = uniform(threadIdx.x >> 6);
+    const int dim = (int)A.dim, len = (int)A.len;
+    T* qtile = (T*)lds;
+    T* gtile = qtile + RB * TILE;
+    const uint32_t mine = lds_offset(lds) + (uint32_t)(SHARED + wave * OWN) * 2, pd = mine + 2 * TILE * 2;
+    TileFetch<T, DP, 1, 1> fetcher;
+    fetcher.start(0);
+    const int per_passage = (len + 31) / 32;
+    const int64_t total = P.items * P.splits;   // splits: workgroups per item
+    const int64_t id = block_id();
+    if (id >= total) return;
+    const int group = (int)(id % P.splits);
+    const int64_t bk = id / P.splits, kh = bk % A.kv_heads, b = bk / A.kv_heads;
+    for (int i = threadIdx.x; i < RB * 32 * CH; i += 64 * NW) {
+        const int row = i / CH, chunk = i % CH;
+        int64_t t, h;
+        split_row(P, kh, (uint32_t)row, &t, &h);
+        const bool ok = row < P.row_count && 8 * chunk < dim;
+        const int at = row * DP + tile_chunk<DP>(row, chunk) * 8;
+        *(V8*)(qtile + at) = load8<T>((const T*)A.q + b * A.q_batch + t * A.q_row + h * A.q_head + 8 * chunk, ok);
+        *(V8*)(gtile + at) = load8<T>((const T*)G.grad_out + b * G.g_batch + t * G.g_row + h * G.g_head + 8 * chunk, ok);
+    }
+    if (dim < DP)   // the columns behind dim of the wave's own tiles
+        for (int i = lane; i < 2 * TILE / 8; i += 64)
+            *(__attribute__((address_space(3))) u32x4*)(uintptr_t)(mine + i * 16) = u32x4{0, 0, 0, 0};
+    RowStat st[RB];
+    f32x16 dq[RB][DP / 32];
+    Spread<T> spread_q[RB];
+    SpreadAll<T> spread_k;
+#pragma unroll
+    for (int x = 0; x < RB; ++x) {
+        st[x] = RowStat{INFINITY, 0.0f};
+        if (32 * x < P.pad_rows) st[x] = stats[bk * P.pad_rows + 32 * x + (lane & 31)];
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db) dq[x][db] = f32x16{};
+    }
+    const T* kbase = (const T*)A.k + b * A.k_batch + kh * A.k_head;
+    const T* vbase = (const T*)A.v + b * A.v_batch + kh * A.v_head;
+    const int step = P.splits * NW, step_p = step / per_passage, step_j = step % per_passage;
+    int p = (group * NW + wave) / per_passage, jt = (group * NW + wave) % per_passage, left = 0;
+    int chunk = -1, lengths = len;   // of 64 passages, one per lane
+    auto fetch = [&]() {   // the tile at p, jt: keys in it
+        left = 0;
+        if (p >= (int)A.passages) return;
+        if (A.lengths && (p >> 6) != chunk) {   // rarely: a load here waits for the stores before it
+            chunk = p >> 6;
+            const int i = chunk * 64 + lane;
+            lengths = i < (int)A.passages ? A.lengths[b * A.passages + i] : 0;
         }
-        if (j < A.len) {
-            const int64_t at = (((b * A.passages + p) * A.len + j) * A.kv_heads + kh) * dim;
-            const int64_t all = A.batch * A.passages * A.len * A.kv_heads * dim;
-            const float fv = P.unweight, fk = A.scale * spread.inverse() * P.unweight;
+        left = min(len, __builtin_amdgcn_readlane(lengths, p & 63)) - 32 * jt;
+        if (left <= 0) return;
+        fetcher.fetch(kbase + p * A.k_passage + (int64_t)32 * jt * A.k_row, A.k_row, left, dim, mine);
+        fetcher.fetch(vbase + p * A.v_passage + (int64_t)32 * jt * A.v_row, A.v_row, left, dim, mine + TILE * 2);
+    };
+    f32x16 dk[DP / 32], dv[DP / 32];
+    u32x4 wk[DP / 16], wv[DP / 16];   // the tile before's, rounded, and where it was
+    int held_p = -1, held_j = 0;
+    auto store = [&]() {   // whole rows of 128 bytes: eight lanes each
+        if (held_p < 0) return;
+        const int ln = (int)opaque(lane);
 #pragma unroll
-            for (int db = 0; db < DP / 32; ++db)
+        for (int x = 0; x < 4; ++x) {
+            const int j = held_j + 8 * x + (ln >> 3), d = 8 * (ln & 7);
+            const int64_t at = (((b * A.passages + held_p) * A.len + j) * A.kv_heads + kh) * dim + d;
 #pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    const int d = 32 * db + 8 * x + 4 * half;
-                    if (d >= dim) continue;
-                    float yk[4], yv[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {   // behind the length: zeros, whatever the accumulators hold
-                        yk[e] = j < n ? fk * dk[db][4 * x + e] : 0.0f;
-                        yv[e] = j < n ? fv * dv[db][4 * x + e] : 0.0f;
-                    }
-                    if (P.splits > 1) {
-                        *(float4*)(part + split * 2 * all + at + d) = make_float4(yk[0], yk[1], yk[2], yk[3]);
-                        *(float4*)(part + (split * 2 + 1) * all + at + d) = make_float4(yv[0], yv[1], yv[2], yv[3]);
-                    } else {
-                        put4<T>((T*)G.grad_k + at + d, yk);
-                        put4<T>((T*)G.grad_v + at + d, yv);
-                    }
+            for (int c = 0; c < DP / 64; ++c)
+                if (j < len && 64 * c + d < dim) {
+                    *(u32x4*)((T*)G.grad_k + at + 64 * c) = wk[4 * c + x];
+                    *(u32x4*)((T*)G.grad_v + at + 64 * c) = wv[4 * c + x];
                 }
         }
+    };
+    // accumulators of a tile (lane: key, elements: columns) -> rows, through 4 KiB of LDS, 64 columns at a time
+    auto turn = [&](const f32x16 (&acc)[DP / 32], float f, bool key, u32x4 (&w)[DP / 16]) {
+        const int ln = (int)opaque(lane), row = ln & 31;
+#pragma unroll
+        for (int c = 0; c < DP / 64; ++c) {
+#pragma unroll
+            for (int y = 0; y < 8; ++y) {
+                const f32x16& v = acc[2 * c + (y >> 2)];
+                const int i = 4 * (y & 3);
+                u32x2 t = pack4<T>(f * v[i], f * v[i + 1], f * v[i + 2], f * v[i + 3]);
+                if (!key) t = u32x2{0, 0};   // behind the length: zeros, whatever the accumulators hold
+                *(lds_u32x2*)(uintptr_t)(pd + (uint32_t)(row * 128 + ((y ^ (row & 7)) * 16) + (ln >> 5) * 8)) = t;
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const int r = 8 * x + (ln >> 3);
+                w[4 * c + x] = *(__attribute__((address_space(3))) u32x4*)(uintptr_t)(pd + (uint32_t)(r * 128 + (((ln & 7) ^ (r & 7)) * 16)));
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        }
+    };
+    // dV and dK += the products of row block x, whose P and dS stand in LDS
+    auto add_block = [&](int x) {
+        const int i = lane & 15;
+        const uint32_t pr = opaque(pd + (uint32_t)((4 * half + (i >> 2)) * 64 + (((((lane & 16) >> 2) + (i & 3)) ^ half) * 8)));
+        const uint32_t qcol = opaque(lds_offset(qtile) + columns_base<DP>(lane));
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // they are written: LDS keeps a wave's order
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            V8 pk[2];
+#pragma unroll
+            for (int a = 0; a < 2; ++a) {
+                union {
+                    s16x4 h[2];
+                    V8 v;
+                } u;
+#pragma unroll
+                for (int y = 0; y < 2; ++y)
+                    u.h[y] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(uintptr_t)(
+                        (pr ^ (uint32_t)(32 * ks + 16 * y)) + (uint32_t)(a * 2048 + (16 * ks + 8 * y) * 64)));
+                pk[a] = u.v;
+            }
+#pragma unroll
+            for (int db = 0; db < DP / 32; ++db) {
+                dv[db] = Mma<T>::mul(lds_columns<T, DP>(qcol, 32 * (RB + x) + 16 * ks, db), pk[0], dv[db]);
+                dk[db] = Mma<T>::mul(lds_columns<T, DP>(qcol, 32 * x + 16 * ks, db), pk[1], dk[db]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // and read
+    };
+    fetch();
+    __syncthreads();   // Q and dO are there
+    while (true) {
+        if (left > 0) dma_wait<0>();
+        store();
+        if (p >= (int)A.passages) break;
+        held_p = p;
+        held_j = 32 * jt;
+        const int now = left;
+        if (now > 0) {
+            const uint32_t krow = opaque(mine + rows_base<DP>(lane));
+            const uint32_t qrow = opaque(lds_offset(qtile) + rows_base<DP>(lane));
+#pragma unroll
+            for (int db = 0; db < DP / 32; ++db) dk[db] = dv[db] = f32x16{};
+#pragma unroll
+            for (int x = 0; x < RB; ++x) {
+                if (x > 0) {   // dV and dK of the row block before
+                    add_block(x - 1);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                f32x16 s = f32x16{}, dp = f32x16{};
+#pragma unroll
+                for (int k = 0; k < DP / 16; ++k) {
+                    s = Mma<T>::mul(lds_rows<T, DP>(krow, 0, k), lds_rows<T, DP>(qrow, x, k), s);
+                    dp = Mma<T>::mul(lds_rows<T, DP>(krow, 1, k), lds_rows<T, DP>(qrow, RB + x, k), dp);
+                }
+                // operands two steps ahead and no further: more of them would not fit beside the accumulators
+                __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
+#pragma unroll
+                for (int k = 0; k < DP / 16 - 2; ++k) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+                }
+                __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], P.c, -st[x].x));
+                    dp[i] = s[i] * (dp[i] - st[x].delta);
+                }
+                if (now < 32) {
+                    const int keys = now - 4 * half;
+                    asm volatile("");   // a branch: most tiles are whole
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (8 * (i >> 2) + (i & 3) >= keys) dp[i] = 0.0f;
+                }
+                // P and dS to LDS as [row][key], 8-byte pieces permuted by the row
+                const uint32_t pw = opaque(pd + (uint32_t)((lane & 31) * 64 + ((half ^ ((lane >> 2) & 7)) * 8)));
+                spread_k.fit(dp, dk);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    *(lds_u32x2*)(uintptr_t)(pw ^ (16 * i)) = pack4<T>(s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]);
+                    *(lds_u32x2*)(uintptr_t)((pw ^ (16 * i)) + 2048) = pack4<T>(spread_k.times(dp[4 * i]), spread_k.times(dp[4 * i + 1]), spread_k.times(dp[4 * i + 2]), spread_k.times(dp[4 * i + 3]));
+                }
+                spread_q[x].fit(dp, dq[x]);
+                const uint32_t kcol = opaque(mine + columns_base<DP>(lane));
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks) {
+                    const V8 ds = weights8<T>(dp, ks);
+#pragma unroll
+                    for (int db = 0; db < DP / 32; ++db) dq[x][db] = Mma<T>::mul(lds_columns<T, DP>(kcol, 16 * ks, db), ds, dq[x][db]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // K and V are read: the next tile may come
+        }
+        p += step_p;
+        jt += step_j;
+        if (jt >= per_passage) {
+            jt -= per_passage;
+            ++p;
+        }
+        fetch();
+        if (now > 0) add_block(RB - 1);
+        const float fk = A.scale * spread_k.inverse() * P.unweight;
+        const bool key = (lane & 31) < now;
+        turn(dv, P.unweight, key, wv);
+        turn(dk, fk, key, wk);
+    }
+    // dQ of the workgroup: [wave][d][row]
+    float* sums = (float*)lds;
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < RB; ++x) {
+        const float f = A.scale * spread_q[x].inverse() * P.unweight;
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                sums[((wave * RB + x) * DP + 32 * db + 8 * (i >> 2) + 4 * half + (i & 3)) * 32 + (lane & 31)] = f * dq[x][db][i];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < RB * 32 * (DP / 4); i += 64 * NW) {
+        const int row = i & 31, d = (i >> 5) % (DP / 4) * 4, x = i / (32 * (DP / 4)), r = 32 * x + row;
+        if (r >= P.row_count || d >= dim) continue;
+        float y[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int w = 0; w < NW; ++w)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] += sums[((w * RB + x) * DP + d + e) * 32 + row];
+        int64_t t, h;
+        split_row(P, kh, (uint32_t)r, &t, &h);
+        const int64_t at = ((b * A.rows + t) * A.heads + h) * dim + d;
+        if (P.splits > 1) *(float4*)(part + group * (A.batch * A.rows * A.heads * dim) + at) = make_float4(y[0], y[1], y[2], y[3]);
+        else put4<T>((T*)G.grad_q + at, y);
     }
 }
 
