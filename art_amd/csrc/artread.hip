@@ -353,7 +353,7 @@ static AttendShape attend_shape(const artread_attend_t* a) {
     P.row_blocks = (P.row_count + block - 1) / block;
     P.items = a->batch * a->kv_heads * P.row_blocks;
     const int64_t tiles = a->passages * ((a->len + keys - 1) / keys);
-    int64_t want = ((S.stream ? 4096 : 512) + P.items - 1) / P.items, most = tiles / (S.stream ? 2 : 4);
+    int64_t want = ((S.stream ? 4096 : 512) + P.items - 1) / P.items, most = tiles / 4;   // a part of fewer tiles costs less than the join
     want = want < most ? want : most;
     P.splits = (int)(want < 1 ? 1 : (want < 256 ? want : 256));
     plan_scale(&P, a->scale, a->dtype);

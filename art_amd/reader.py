@@ -16,6 +16,7 @@ shared with an eager graph does not survive a capture.
 import ctypes
 import math
 import os
+import struct
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -64,7 +65,7 @@ def _read():
             raise ImportError("%s is missing: run art_amd/csrc/build.sh (or __graft_entry__.build())"
                               % READ_LIB_PATH)
         lib = ctypes.CDLL(READ_LIB_PATH)
-        f32, args, grads = ctypes.c_float, ctypes.POINTER(AttendArgs), ctypes.POINTER(AttendGrads)
+        f32, args, grads = ctypes.c_float, _vp, _vp   # the two structures, as their bytes or by reference
         lib.artread_embed.argtypes = [_i32, _vp, _i32, _i64, _i64, _i64, _vp, _i32, _vp, _i64, _i64, _i64, f32,
                                       _vp, _i32, _vp]
         lib.artread_embed.restype = _i32
@@ -108,7 +109,7 @@ def _stream(dev):
 
 def _scale_value(scale):
     scale = float(scale)
-    if not math.isfinite(scale) or math.isinf(ctypes.c_float(scale).value):
+    if not abs(scale) < 3.4e38:   # of a 32-bit float
         raise ValueError("scale must be finite, got %r" % scale)
     return scale
 
@@ -125,18 +126,19 @@ def _check_tokens(tokens, lengths):
 
 
 def _embed(tokens, table, lengths, scale, vocab_base, out_dtype):
-    out = torch.empty(tuple(tokens.shape) + (table.shape[1],), dtype=out_dtype, device=table.device)
-    if out.numel() == 0:
+    dev, shape = table.device, tokens.shape
+    vocab, dim = table.shape
+    out = torch.empty((*shape, dim), dtype=out_dtype, device=dev)
+    positions, length = tokens.numel(), shape[-1]
+    if positions * dim == 0:
         return out
     tokens = tokens.contiguous()
     lengths = lengths.contiguous() if lengths is not None else None
-    length = tokens.shape[-1]
-    with _on_device(table.device):
+    with _on_device(dev):
         _rcheck(_read().artread_embed(
-            table.device.index, table.data_ptr(), _ABI[table.dtype], table.shape[0], table.shape[1],
-            table.stride(0), tokens.data_ptr(), tokens.element_size(),
-            lengths.data_ptr() if lengths is not None else None, tokens.numel() // length, length, vocab_base,
-            scale, out.data_ptr(), _ABI[out_dtype], _stream(table.device)))
+            dev.index, table.data_ptr(), _ABI[table.dtype], vocab, dim, table.stride(0), tokens.data_ptr(),
+            tokens.element_size(), lengths.data_ptr() if lengths is not None else None, positions // length, length,
+            vocab_base, scale, out.data_ptr(), _ABI[out_dtype], _stream(dev)))
     return out
 
 
@@ -175,7 +177,7 @@ def embed_tokens(tokens, table, lengths=None, scale=1.0, vocab_base=0, out_dtype
         raise ValueError("out_dtype must be the table's type, or float16 / bfloat16 of a float32 table")
     scale = _scale_value(scale)
     _one_device(table, tokens, lengths)
-    if torch.is_grad_enabled() and table.requires_grad:
+    if table.requires_grad and torch.is_grad_enabled():
         return _EmbedTokens.apply(table, tokens, lengths, scale, int(vocab_base), out_dtype)
     return _embed(tokens, table, lengths, scale, int(vocab_base), out_dtype)
 
@@ -215,81 +217,86 @@ def embed_tokens_grad(grad_out, tokens, vocab, lengths=None, scale=1.0, vocab_ba
 
 
 # ---- cross attention ------------------------------------------------------------------------------
-def _strided(t, share=0):
-    """`t` [..., rows, heads, dim] with the layout the kernels address: innermost stride 1, the others multiples
-    of 8 elements, rows less than 2**24 apart, the `share` query heads of a key head within 2**29, 16-byte
-    aligned.  Anything else is copied."""
-    strides = _outer(t)
-    if (t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and not any(s % 8 for s in strides)
-            and strides[-2] < 1 << 24 and share * strides[-1] < 1 << 29):
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
+# artread_attend_t as bytes: filling a ctypes structure field by field costs more than the smallest launch
+_pack_args = struct.Struct("=7Q18qif").pack
+_pack_grads = struct.Struct("=Q3q3Q").pack
 
 
-def _outer(t):
-    """The strides of all dimensions but the last; those of dimensions of size 1 are never used."""
-    return [s if n > 1 else 0 for s, n in zip(t.stride()[:-1], t.shape[:-1])]
-
-
-def _check_attention(query, key, value, lengths, scale):
-    if query.dim() != 4 or key.dim() not in (4, 5) or value.shape != key.shape:
+def _plan(query, key, value, lengths, scale):
+    """Checks a call and returns (sizes, scale): sizes are batch, rows, passages, len, heads, kv_heads, dim."""
+    q_shape, k_shape = query.shape, key.shape
+    if len(q_shape) != 4 or len(k_shape) not in (4, 5) or value.shape != k_shape:
         raise ValueError("query must be [batch, rows, heads, dim], key and value [batch, len, kv_heads, dim] or "
                          "[batch, passages, len, kv_heads, dim]")
-    if query.dtype not in (torch.float16, torch.bfloat16) or key.dtype != query.dtype or value.dtype != query.dtype:
+    dtype = query.dtype
+    if dtype not in (torch.float16, torch.bfloat16) or key.dtype != dtype or value.dtype != dtype:
         raise ValueError("query, key and value must share a type, float16 or bfloat16")
-    batch, rows, heads, dim = query.shape
-    if key.shape[0] != batch or key.shape[-1] != dim:
-        raise ValueError("key %s does not fit query %s" % (tuple(key.shape), tuple(query.shape)))
+    batch, rows, heads, dim = q_shape
+    passages, (length, kv_heads) = (k_shape[1] if len(k_shape) == 5 else 1), k_shape[-3:-1]
+    if k_shape[0] != batch or k_shape[-1] != dim:
+        raise ValueError("key %s does not fit query %s" % (tuple(k_shape), tuple(q_shape)))
     if dim < 8 or dim > MAX_HEAD_DIM or dim % 8:
         raise ValueError("the head size must be a multiple of 8 up to %d, got %d" % (MAX_HEAD_DIM, dim))
-    if key.shape[-2] < 1 or heads % key.shape[-2]:
-        raise ValueError("%d query heads cannot share %d key heads" % (heads, key.shape[-2]))
-    if lengths is not None and (lengths.dtype != torch.int32 or lengths.shape != key.shape[:-3]):
-        raise ValueError("lengths must be an int32 tensor %s, one per passage" % (tuple(key.shape[:-3]),))
-    if max(query.numel() // max(1, dim), key.numel() // max(1, dim)) >= 1 << 31:
+    if kv_heads < 1 or heads % kv_heads:
+        raise ValueError("%d query heads cannot share %d key heads" % (heads, kv_heads))
+    if lengths is not None and (lengths.dtype != torch.int32 or lengths.shape != k_shape[:-3]):
+        raise ValueError("lengths must be an int32 tensor %s, one per passage" % (tuple(k_shape[:-3]),))
+    if max(batch * rows * heads, batch * passages * length * kv_heads) >= 1 << 31:
         raise ValueError("query and key hold at most 2**31 - 1 rows each")
-    return _scale_value(dim ** -0.5 if scale is None else scale)
+    return (batch, rows, passages, length, heads, kv_heads, dim), _scale_value(dim ** -0.5 if scale is None else scale)
 
 
-def _attend_args(query, key, value, lengths, out, lse, rest, scale):
-    batch, rows, heads, dim = query.shape
-    if key.dim() == 4:
-        key, value = key.unsqueeze(1), value.unsqueeze(1)
-    return AttendArgs(query.data_ptr(), key.data_ptr(), value.data_ptr(),
-                      lengths.data_ptr() if lengths is not None else None, out.data_ptr(),
-                      lse.data_ptr() if lse is not None else None, rest.data_ptr() if rest is not None else None, batch, rows, key.shape[1], key.shape[2], heads,
-                      key.shape[3], dim, *_outer(query), *_outer(key), *_outer(value), _ABI[query.dtype], scale)
+def _layout(t, share=1):
+    """`t` [batch, (passages,) rows, heads, dim] and the strides of all its dimensions but the last, in the layout
+    the kernels address: innermost stride 1, the others multiples of 8 elements, rows less than 2**24 apart, the
+    `share` query heads of a key head within 2**29, 16-byte aligned.  Anything else is copied."""
+    strides = t.stride()
+    *outer, row, head, one = strides
+    if one != 1 or t.data_ptr() & 15 or (row | head) & 7 or any(x & 7 for x in outer) or row >= 1 << 24 or share * head >= 1 << 29:
+        t = t.clone(memory_format=torch.contiguous_format)
+        strides = t.stride()
+    return t, (strides if len(strides) == 5 else (strides[0], 0) + strides[1:])
 
 
-def _attend(query, key, value, lengths, scale, want_lse, want_rest):
+def _args(query, key, value, lengths, out, lse, rest, sizes, scale):
+    """artread_attend_t of a call, and the tensors it points into."""
+    share = sizes[4] // sizes[5]
+    query, (q_batch, _, q_row, q_head, _) = _layout(query, share)
+    key, k_strides = _layout(key)
+    value, v_strides = _layout(value)
+    if lengths is not None:
+        lengths = lengths.contiguous()
+    return (_pack_args(query.data_ptr(), key.data_ptr(), value.data_ptr(),
+                       lengths.data_ptr() if lengths is not None else 0, out.data_ptr(),
+                       lse.data_ptr() if lse is not None else 0, rest.data_ptr() if rest is not None else 0, *sizes,
+                       q_batch, q_row, q_head, *k_strides[:4], *v_strides[:4], _ABI[query.dtype], scale),
+            (query, key, value, lengths))
+
+
+def _attend(query, key, value, lengths, sizes, scale, want_lse, want_rest):
     dev = query.device
-    batch, rows, heads, dim = query.shape
+    batch, rows, passages, length, heads, kv_heads, dim = sizes
     out = torch.empty(query.shape, dtype=query.dtype, device=dev)
     lse = torch.empty((batch, heads, rows), dtype=torch.float32, device=dev) if want_lse else None
     rest = torch.empty_like(out) if want_rest else None
-    if out.numel() == 0:
-        return out, lse, rest
-    if key.numel() == 0:
-        return out.zero_(), lse.fill_(-math.inf) if want_lse else None, rest.zero_() if want_rest else None
-    share = heads // key.shape[-2]
-    query, key, value = _strided(query, share), _strided(key), _strided(value)
-    lengths = lengths.contiguous() if lengths is not None else None
+    if not (batch and rows and heads and passages and length):
+        out.zero_()
+        return out, lse.fill_(-math.inf) if want_lse else None, rest.zero_() if want_rest else None
+    args, _held = _args(query, key, value, lengths, out, lse, rest, sizes, scale)
     lib = _read()
-    args = _attend_args(query, key, value, lengths, out, lse, rest, scale)
-    size = lib.artread_attend_workspace(ctypes.byref(args))
+    size = lib.artread_attend_workspace(args)
     with _on_device(dev):
-        ws = torch.empty((size,), dtype=torch.uint8, device=dev) if size else None
-        _rcheck(lib.artread_attend(dev.index, ctypes.byref(args), ws.data_ptr() if size else None, size,
-                                   _stream(dev)))
+        ws = torch.empty((size,), dtype=torch.uint8, device=dev) if size > 0 else None
+        _rcheck(lib.artread_attend(dev.index, args, ws.data_ptr() if ws is not None else None, size, _stream(dev)))
     return out, lse, rest
 
 
 class _CrossAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, query, key, value, lengths, scale):
-        out, lse, rest = _attend(query, key, value, lengths, scale, True, True)
+    def forward(ctx, query, key, value, lengths, sizes, scale):
+        out, lse, rest = _attend(query, key, value, lengths, sizes, scale, True, True)
         ctx.save_for_backward(query, key, value, lengths, out, lse, rest)
-        ctx.scale = scale
+        ctx.of = sizes, scale
         ctx.mark_non_differentiable(lse, rest)
         return out, lse, rest
 
@@ -297,7 +304,8 @@ class _CrossAttention(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad_out, _lse, _rest):
         query, key, value, lengths, out, lse, rest = ctx.saved_tensors
-        return cross_attention_grad(grad_out, query, key, value, out, (lse, rest), lengths, ctx.scale) + (None, None)
+        _one_device(query, grad_out)
+        return _attend_grad(grad_out, query, key, value, lengths, out, lse, rest, *ctx.of) + (None, None, None)
 
 
 def cross_attention(query, key, value, lengths=None, scale=None, return_lse=False, return_saved=False):
@@ -315,46 +323,50 @@ def cross_attention(query, key, value, lengths=None, scale=None, return_lse=Fals
     Returns [batch, rows, heads, dim], with ``return_lse`` also the float32 [batch, heads, rows] log of the
     softmax's sum (not differentiable), with ``return_saved`` instead what ``cross_attention_grad`` takes: that
     log and what rounding took from the result.  Differentiable in query, key and value."""
-    scale = _check_attention(query, key, value, lengths, scale)
+    sizes, scale = _plan(query, key, value, lengths, scale)
     _one_device(query, key, value, lengths)
-    if torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad):
-        out, lse, rest = _CrossAttention.apply(query, key, value, lengths, scale)
+    if (query.requires_grad or key.requires_grad or value.requires_grad) and torch.is_grad_enabled():
+        out, lse, rest = _CrossAttention.apply(query, key, value, lengths, sizes, scale)
     else:
-        out, lse, rest = _attend(query, key, value, lengths, scale, return_lse or return_saved, return_saved)
+        out, lse, rest = _attend(query, key, value, lengths, sizes, scale, return_lse or return_saved, return_saved)
     if return_saved:
         return out, (lse, rest)
     return (out, lse) if return_lse else out
 
 
+def _attend_grad(grad_out, query, key, value, lengths, out, lse, rest, sizes, scale):
+    dev = query.device
+    batch, rows, passages, length, heads, kv_heads, dim = sizes
+    grads = [torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (query, key, value)]
+    if not (batch and rows and heads and passages and length):
+        return tuple(t.zero_() for t in grads)
+    args, _held = _args(query, key, value, lengths, out, lse, rest, sizes, scale)
+    grad_out, (g_batch, _, g_row, g_head, _) = _layout(grad_out, heads // kv_heads)
+    more = _pack_grads(grad_out.data_ptr(), g_batch, g_row, g_head, *[t.data_ptr() for t in grads])
+    lib = _read()
+    size = lib.artread_attend_grad_workspace(args)
+    with _on_device(dev):
+        ws = torch.empty((size,), dtype=torch.uint8, device=dev) if size > 0 else None
+        _rcheck(lib.artread_attend_grad(dev.index, args, more, ws.data_ptr() if ws is not None else None, size,
+                                        _stream(dev)))
+    return tuple(grads)
+
+
 def cross_attention_grad(grad_out, query, key, value, out, saved, lengths=None, scale=None):
     """Gradients (query, key, value) of ``cross_attention`` from its result ``out`` and what it ``saved``.
     Written whole, zeros behind each passage's length; equal inputs give equal bits."""
-    scale = _check_attention(query, key, value, lengths, scale)
+    sizes, scale = _plan(query, key, value, lengths, scale)
     if grad_out.shape != query.shape or grad_out.dtype != query.dtype:
         raise ValueError("grad_out must have query's shape and type")
     lse, rest = saved
     for t in (out, rest):
         if t.shape != query.shape or t.dtype != query.dtype or not t.is_contiguous() or t.data_ptr() % 16:
             raise ValueError("out and saved must be what cross_attention returned")
-    batch, rows, heads, dim = query.shape
+    batch, rows, heads, _ = query.shape
     if lse.shape != (batch, heads, rows) or lse.dtype != torch.float32 or not lse.is_contiguous():
         raise ValueError("out and saved must be what cross_attention returned")
-    dev = _one_device(query, key, value, lengths, grad_out, out, lse, rest)
-    grads = [torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (query, key, value)]
-    if query.numel() == 0 or key.numel() == 0:
-        return tuple(t.zero_() for t in grads)
-    share = heads // key.shape[-2]
-    query, grad_out, key, value = _strided(query, share), _strided(grad_out, share), _strided(key), _strided(value)
-    lengths = lengths.contiguous() if lengths is not None else None
-    lib = _read()
-    args = _attend_args(query, key, value, lengths, out, lse, rest, scale)
-    more = AttendGrads(grad_out.data_ptr(), *_outer(grad_out), *[t.data_ptr() for t in grads])
-    size = lib.artread_attend_grad_workspace(ctypes.byref(args))
-    with _on_device(dev):
-        ws = torch.empty((size,), dtype=torch.uint8, device=dev) if size else None
-        _rcheck(lib.artread_attend_grad(dev.index, ctypes.byref(args), ctypes.byref(more),
-                                        ws.data_ptr() if size else None, size, _stream(dev)))
-    return tuple(grads)
+    _one_device(query, key, value, lengths, grad_out, out, lse, rest)
+    return _attend_grad(grad_out, query, key, value, lengths, out, lse, rest, sizes, scale)
 
 
 __all__ = ["embed_tokens", "embed_tokens_grad", "cross_attention", "cross_attention_grad", "ArtreadError"]

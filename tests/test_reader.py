@@ -26,6 +26,9 @@ def test_header_binding_and_library_agree():
     # seven pointers, eighteen int64, int32 + float; one pointer, three int64, three pointers
     assert ctypes.sizeof(rd.AttendArgs) == 25 * 8 + 8
     assert ctypes.sizeof(rd.AttendGrads) == 7 * 8
+    a, g = _attend(), rd.AttendGrads(*range(1, 8))
+    assert rd._pack_args(*(getattr(a, n) or 0 for n, _ in a._fields_)) == bytes(a)
+    assert rd._pack_grads(*range(1, 8)) == bytes(g)
 
 
 # ---- the Python layer -----------------------------------------------------------------------------
