@@ -79,7 +79,7 @@ static void launch_embed(const void* table, int64_t stride, const Tokens& T, flo
                          hipStream_t st) {
     const int cpr = dim / EPV, rpp = cpr < 256 ? 256 / cpr : 1;
     const int threads = cpr < 256 ? (int)round_up((int64_t)cpr * rpp, 64) : 256;
-    const int64_t want = (T.positions + (int64_t)rpp * 8 - 1) / ((int64_t)rpp * 8);
+    const int64_t want = (T.positions + (int64_t)rpp * kEmbedRows - 1) / ((int64_t)rpp * kEmbedRows);
     const unsigned grid = (unsigned)(want < (1 << 22) ? want : (1 << 22));
     hipLaunchKernelGGL((embed_kernel<TT, OT, IDX, EPV>), dim3(grid), dim3(threads), 0, st, (const TT*)table, stride, T,
                        scale, (OT*)out, dim, cpr, rpp);
@@ -88,15 +88,19 @@ static void launch_embed(const void* table, int64_t stride, const Tokens& T, flo
 template <typename TT, typename OT>
 static void embed_any(const void* table, int64_t stride, const Tokens& T, int token_bytes, float scale, void* out,
                       int dim, hipStream_t st) {
+    // chunks of 16 bytes of output where rows allow them, else pairs of elements, else one
     constexpr int W = 16 / sizeof(OT);
     const bool wide = dim % W == 0 && stride % (16 / (int)sizeof(TT)) == 0 && aligned(table, 16) && aligned(out, 16);
-    if (token_bytes == 4) {
-        if (wide) launch_embed<TT, OT, int32_t, W>(table, stride, T, scale, out, dim, st);
-        else launch_embed<TT, OT, int32_t, 1>(table, stride, T, scale, out, dim, st);
-    } else {
-        if (wide) launch_embed<TT, OT, int64_t, W>(table, stride, T, scale, out, dim, st);
-        else launch_embed<TT, OT, int64_t, 1>(table, stride, T, scale, out, dim, st);
-    }
+    const bool pairs = dim % 2 == 0 && stride % 2 == 0 && aligned(table, 2 * sizeof(TT)) && aligned(out, 2 * sizeof(OT));
+#define EMBED(IDX)                                                                              \
+    do {                                                                                        \
+        if (wide) launch_embed<TT, OT, IDX, W>(table, stride, T, scale, out, dim, st);          \
+        else if (pairs) launch_embed<TT, OT, IDX, 2>(table, stride, T, scale, out, dim, st);    \
+        else launch_embed<TT, OT, IDX, 1>(table, stride, T, scale, out, dim, st);               \
+    } while (0)
+    if (token_bytes == 4) EMBED(int32_t);
+    else EMBED(int64_t);
+#undef EMBED
 }
 
 extern "C" int artread_embed(int device, const void* table, int table_dtype, int64_t vocab, int64_t dim,
@@ -126,28 +130,29 @@ extern "C" int artread_embed(int device, const void* table, int table_dtype, int
     return 0;
 }
 
-// Sort digits of at most nine bits, at most 256 chunks of at least 4,096 positions.
+// Sort digits of at most nine bits; one chunk up to kSortAlone positions, else at most 256 of at least 4,096.
 static SortPlan sort_plan(int64_t vocab, int64_t positions) {
     SortPlan P;
     int bits = 1;
     while (bits < 31 && ((int64_t)1 << bits) < vocab) ++bits;
     P.passes = (bits + 8) / 9;
     P.bits = (bits + P.passes - 1) / P.passes;
-    P.chunk = round_up((positions + 255) / 256, 256);
-    if (P.chunk < 4096) P.chunk = 4096;
+    P.chunk = round_up(positions <= kSortAlone ? positions : (positions + 255) / 256, kSortThreads);
+    if (positions > kSortAlone && P.chunk < 4096) P.chunk = 4096;
     P.blocks = (int)((positions + P.chunk - 1) / P.chunk);
     return P;
 }
 
-// Workers of 64 positions where there are enough positions for them to fill the chip, fewer down to 8.
+// Ranges of 128 positions where that many fill the chip, down to 8 where not: the join of a token's partial sums is
+// as long as they are many (2,048 x 256 positions of 768 f16: join 12 us with 128, 19 with 64, 33 with 32; sums alike).
 static int sum_run(int64_t positions) {
-    int run = 64;
+    int run = 128;
     while (run > 8 && positions / run < 4096) run >>= 1;
     return run;
 }
 
 struct GradSpace {   // byte offsets into the workspace
-    int64_t meta, counts, used, pairs0, pairs1, chain_end, partial, total;
+    int64_t meta, counts, pairs0, pairs1, chain_end, partial, total;
     int64_t pad_dim;
     int run;
 };
@@ -164,7 +169,6 @@ static GradSpace grad_space(int64_t vocab, int64_t dim, int64_t positions) {
     s.pad_dim = round_up(dim, 4);
     s.meta = take(sizeof(SortMeta));
     s.counts = take((int64_t)P.blocks * (1 << P.bits) * 4);
-    s.used = take(round_up(vocab, 16));
     s.pairs0 = take(positions * 8);
     s.pairs1 = P.passes > 1 ? take(positions * 8) : s.pairs0;
     s.chain_end = take(vocab * 4);
@@ -181,8 +185,7 @@ extern "C" int64_t artread_embed_grad_workspace(int64_t vocab, int64_t dim, int6
 }
 
 template <typename GT, typename OT, int EPV>
-static void launch_grad_sums(const void* grad, const Pair* sorted, const SortMeta* meta, const uint8_t* used,
-                             const Tokens& T, float scale, void* table, int dim, const GradSpace& s, float* partial,
+static void launch_grad_sums(const void* grad, const Pair* sorted, const SortMeta* meta, const Tokens& T, float scale, void* table, int dim, const GradSpace& s, float* partial,
                              int32_t* chain_end, hipStream_t st) {
     SumPlan S;
     S.run = s.run;
@@ -192,24 +195,25 @@ static void launch_grad_sums(const void* grad, const Pair* sorted, const SortMet
     S.workers = (T.positions + s.run - 1) / s.run;
     S.sum_groups = (S.workers + S.rpp - 1) / S.rpp;
     const int threads = S.cpr < 256 ? (int)round_up((int64_t)S.cpr * S.rpp, 64) : 256;
-    int64_t clear = (T.vocab + S.rpp * 4 - 1) / (S.rpp * 4);
-    if (clear > 16384) clear = 16384;
+    const int64_t clear = (T.vocab + kClearRows - 1) / kClearRows;
     hipLaunchKernelGGL((grad_sum_kernel<GT, OT, EPV>), dim3((unsigned)(S.sum_groups + clear)), dim3(threads), 0, st,
-                       (const GT*)grad, sorted, meta, used, T.vocab, scale, (OT*)table, dim, S, partial, chain_end);
-    const unsigned jx = (unsigned)(S.workers < 4096 ? S.workers : 4096);
-    hipLaunchKernelGGL((grad_join_kernel<OT>), dim3(jx, (unsigned)((dim + 63) / 64)), dim3(256), 0, st, sorted, meta,
-                       scale, (OT*)table, dim, S, partial, chain_end);
+                       (const GT*)grad, sorted, meta, T.vocab, scale, (OT*)table, dim, S, partial, chain_end);
+    if (S.workers > 1)
+        hipLaunchKernelGGL((grad_join_kernel<OT>), dim3((unsigned)((S.workers + kJoinWaves - 1) / kJoinWaves), (unsigned)((dim + 255) / 256)),
+                           dim3(64 * kJoinWaves), 0, st, sorted, meta, scale, (OT*)table, dim, S, partial, chain_end);
 }
 
 template <typename GT, typename OT>
-static void grad_sums(const void* grad, const Pair* sorted, const SortMeta* meta, const uint8_t* used, const Tokens& T,
+static void grad_sums(const void* grad, const Pair* sorted, const SortMeta* meta, const Tokens& T,
                       float scale, void* table, int dim, const GradSpace& s, float* partial, int32_t* chain_end,
                       hipStream_t st) {
     constexpr int W = 16 / sizeof(GT);
     if (dim % W == 0 && aligned(grad, 16) && aligned(table, 16))
-        launch_grad_sums<GT, OT, W>(grad, sorted, meta, used, T, scale, table, dim, s, partial, chain_end, st);
+        launch_grad_sums<GT, OT, W>(grad, sorted, meta, T, scale, table, dim, s, partial, chain_end, st);
+    else if (dim % 2 == 0 && aligned(grad, 2 * sizeof(GT)) && aligned(table, 2 * sizeof(OT)))
+        launch_grad_sums<GT, OT, 2>(grad, sorted, meta, T, scale, table, dim, s, partial, chain_end, st);
     else
-        launch_grad_sums<GT, OT, 1>(grad, sorted, meta, used, T, scale, table, dim, s, partial, chain_end, st);
+        launch_grad_sums<GT, OT, 1>(grad, sorted, meta, T, scale, table, dim, s, partial, chain_end, st);
 }
 
 template <typename IDX>
@@ -217,20 +221,22 @@ static const Pair* sort_tokens(const Tokens& T, char* ws, const GradSpace& s, hi
     const SortPlan P = sort_plan(T.vocab, T.positions);
     SortMeta* meta = (SortMeta*)(ws + s.meta);
     uint32_t* counts = (uint32_t*)(ws + s.counts);
-    uint8_t* used = (uint8_t*)(ws + s.used);
     Pair* pairs[2] = {(Pair*)(ws + s.pairs0), (Pair*)(ws + s.pairs1)};
-    const dim3 grid((unsigned)P.blocks), block(256);
+    const dim3 grid((unsigned)P.blocks), block(kSortThreads);
+    if (P.blocks == 1) {
+        hipLaunchKernelGGL((sort_alone_kernel<IDX>), grid, block, 0, st, T, meta, P, pairs[0], pairs[1]);
+        return pairs[(P.passes - 1) & 1];
+    }
     for (int pass = 0; pass < P.passes; ++pass) {
         const int shift = pass * P.bits;
         const Pair* in = pairs[(pass + 1) & 1];
+        Pair* out = pairs[pass & 1];
         if (pass == 0) {
-            hipLaunchKernelGGL((sort_count_kernel<IDX, true>), grid, block, 0, st, T, in, meta, P, shift, counts, used);
-            hipLaunchKernelGGL((sort_place_kernel<IDX, true>), grid, block, 0, st, T, in, meta, P, shift, counts,
-                               pairs[0], used);
+            hipLaunchKernelGGL((sort_count_kernel<IDX, true>), grid, block, 0, st, T, in, meta, P, shift, counts);
+            hipLaunchKernelGGL((sort_place_kernel<IDX, true>), grid, block, 0, st, T, in, meta, P, shift, counts, out);
         } else {
-            hipLaunchKernelGGL((sort_count_kernel<IDX, false>), grid, block, 0, st, T, in, meta, P, shift, counts, used);
-            hipLaunchKernelGGL((sort_place_kernel<IDX, false>), grid, block, 0, st, T, in, meta, P, shift, counts,
-                               pairs[pass & 1], used);
+            hipLaunchKernelGGL((sort_count_kernel<IDX, false>), grid, block, 0, st, T, in, meta, P, shift, counts);
+            hipLaunchKernelGGL((sort_place_kernel<IDX, false>), grid, block, 0, st, T, in, meta, P, shift, counts, out);
         }
     }
     return pairs[(P.passes - 1) & 1];
@@ -259,10 +265,9 @@ extern "C" int artread_embed_grad(int device, const void* grad_out, int grad_dty
     const Pair* sorted = token_bytes == 4 ? sort_tokens<int32_t>(T, ws, s, st) : sort_tokens<int64_t>(T, ws, s, st);
     READ_HIP(hipGetLastError());
     const SortMeta* meta = (const SortMeta*)(ws + s.meta);
-    const uint8_t* used = (const uint8_t*)(ws + s.used);
     float* partial = (float*)(ws + s.partial);
     int32_t* ends = (int32_t*)(ws + s.chain_end);
-#define SUMS(GT, OT) grad_sums<GT, OT>(grad_out, sorted, meta, used, T, scale, grad_table, (int)dim, s, partial, ends, st)
+#define SUMS(GT, OT) grad_sums<GT, OT>(grad_out, sorted, meta, T, scale, grad_table, (int)dim, s, partial, ends, st)
     if (grad_dtype == ARTREAD_F32) SUMS(float, float);
     else if (grad_dtype == ARTREAD_F16 && table_dtype == ARTREAD_F16) SUMS(f16, f16);
     else if (grad_dtype == ARTREAD_F16) SUMS(f16, float);

@@ -42,23 +42,27 @@ __device__ __forceinline__ int32_t key_of(const Tokens& T, uint32_t pos) {
 
 // ---- lookup ---------------------------------------------------------------------------------------
 // A thread owns one chunk of EPV output elements (16 bytes where the layout allows, else one element)
-// of U rows at a time; `cpr` chunks make a row, a workgroup holds `rpp` rows side by side.  The keys of
-// its rows are requested before any table row, those before any store: three dependent round trips per
-// U * rpp rows.  The table is read through the caches (a few thousand rows serve a whole batch), the
-// output, which another kernel reads much later, is stored past them.
+// of U rows; `cpr` chunks make a row, a workgroup holds `rpp` rows side by side.  The keys of its rows are
+// requested before any table row, those before any store.  The U rows are a whole grid apart, so that the chip
+// writes one window of consecutive rows at a time: with rows of a workgroup next to each other, U decided how
+// many workgroups met on a memory channel (2,048 x 256 tokens of 768 bf16: U 1 246 us, 3 141, 8 215, 16 378);
+// with them apart 149 us for U 2 and 4.  The table is read through the caches (a few thousand rows serve a whole
+// batch), the output, which another kernel reads much later, is stored past them (251-340 us if it is not).
+// Bound by those stores.
+constexpr int kEmbedRows = 2;
 template <typename TT, typename OT, typename IDX, int EPV>
 __global__ __launch_bounds__(256) void embed_kernel(const TT* __restrict__ table, int64_t table_stride, Tokens T,
                                                     float scale, OT* __restrict__ out, int dim, int cpr, int rpp) {
-    constexpr int U = 8;
+    constexpr int U = kEmbedRows;
     const int r = cpr < 256 ? (int)threadIdx.x / cpr : 0;
     const int c0 = cpr < 256 ? (int)threadIdx.x - r * cpr : (int)threadIdx.x;
     if (r >= rpp) return;
-    const int64_t step = (int64_t)gridDim.x * rpp * U;
-    for (int64_t base = (int64_t)blockIdx.x * rpp * U + r; base < T.positions; base += step) {
+    const int64_t apart = (int64_t)gridDim.x * rpp;
+    for (int64_t base = (int64_t)blockIdx.x * rpp + r; base < T.positions; base += apart * U) {
         int32_t key[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int64_t pos = base + (int64_t)u * rpp;
+            const int64_t pos = base + u * apart;
             key[u] = pos < T.positions ? key_of<IDX>(T, (uint32_t)pos) : -1;
         }
         for (int c = c0; c < cpr; c += 256) {
@@ -71,7 +75,7 @@ __global__ __launch_bounds__(256) void embed_kernel(const TT* __restrict__ table
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int64_t pos = base + (int64_t)u * rpp;
+                const int64_t pos = base + u * apart;
                 if (pos >= T.positions) break;
                 Vec<OT, EPV> w;
 #pragma unroll
@@ -86,10 +90,14 @@ __global__ __launch_bounds__(256) void embed_kernel(const TT* __restrict__ table
 // A stable radix sort of the valid positions by key, least significant digit first, digits of at most
 // nine bits (two passes for every vocabulary up to 262,144).  Stability makes the order of a token's
 // positions, and with it every sum, a function of the tokens alone.  Per pass: digit counts of every
-// block's chunk, then each block derives its own bases from all counts and places its chunk.
+// workgroup's chunk, then each workgroup derives its own bases from all counts and places its chunk.  Up to
+// kSortAlone positions are one workgroup's, which makes all passes in one launch.  What a pass costs is the
+// length of its chains (steps of a wave, rows of counts), not its bytes: hence sixteen waves a workgroup.
+constexpr int kSortThreads = 1024, kSortWaves = 16, kSortDigits = 512;
+constexpr int64_t kSortAlone = 16384;
 struct SortPlan {
     int blocks;       // chunks of the position list
-    int64_t chunk;    // positions per chunk, a multiple of 256
+    int64_t chunk;    // positions per chunk, a multiple of kSortThreads
     int bits;         // of a digit
     int passes;
 };
@@ -112,89 +120,89 @@ __device__ __forceinline__ bool sort_item(const Tokens& T, const Pair* in, int64
     return true;
 }
 
-// digit counts [blocks][1 << bits]; the first pass also clears the marks of used table rows
+// digit counts [blocks][1 << bits]
 template <typename IDX, bool FIRST>
-__global__ __launch_bounds__(256) void sort_count_kernel(Tokens T, const Pair* __restrict__ in,
-                                                         const SortMeta* __restrict__ meta, SortPlan P, int shift,
-                                                         uint32_t* __restrict__ counts, uint8_t* __restrict__ used) {
-    __shared__ uint32_t hist[512];
+__global__ __launch_bounds__(kSortThreads) void sort_count_kernel(Tokens T, const Pair* __restrict__ in,
+                                                                  const SortMeta* __restrict__ meta, SortPlan P,
+                                                                  int shift, uint32_t* __restrict__ counts) {
+    __shared__ uint32_t hist[kSortDigits];
     const int digits = 1 << P.bits;
-    for (int d = threadIdx.x; d < digits; d += 256) hist[d] = 0;
+    if ((int)threadIdx.x < digits) hist[threadIdx.x] = 0;
     __syncthreads();
-    if (FIRST)
-        for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < (T.vocab + 15) / 16; i += (int64_t)gridDim.x * 256)
-            ((uint4*)used)[i] = make_uint4(0, 0, 0, 0);   // the array is padded to 16 bytes
     const int64_t count = FIRST ? T.positions : (int64_t)meta->valid;
     const int64_t lo = blockIdx.x * P.chunk, hi = lo + P.chunk < count ? lo + P.chunk : count;
-    for (int64_t i = lo + threadIdx.x; i < hi; i += 256) {
+    for (int64_t i = lo + threadIdx.x; i < hi; i += kSortThreads) {
         Pair p;
         if (sort_item<IDX, FIRST>(T, in, i, hi, &p)) atomicAdd(&hist[(p.key >> shift) & (digits - 1)], 1u);
     }
     __syncthreads();
-    for (int d = threadIdx.x; d < digits; d += 256) counts[(int64_t)blockIdx.x * digits + d] = hist[d];
+    if ((int)threadIdx.x < digits) counts[(int64_t)blockIdx.x * digits + threadIdx.x] = hist[threadIdx.x];
 }
 
-// Places one chunk.  Each of the four waves owns a quarter of it and walks the quarter in order, 64
-// positions at a time: the lanes that share a digit find each other by `bits` ballots, the lane's rank is
-// the number of them below it, and the highest one moves the wave's next free place of that digit on.
+struct SortSpace {
+    uint32_t next[kSortWaves][kSortDigits];   // a wave's next free place of each digit
+    uint32_t total[kSortDigits], before[kSortDigits], scan[kSortDigits];
+};
+
+// Places one chunk.  Each wave owns a part of it and walks the part in order, 64 positions at a time: the lanes
+// that share a digit find each other by `bits` ballots, the lane's rank is the number of them below it, and the
+// highest one moves the wave's next free place of that digit on.  counts: of all chunks, nullptr where this is the
+// only one.  Returns the number of positions placed by all chunks.
 template <typename IDX, bool FIRST>
-__global__ __launch_bounds__(256) void sort_place_kernel(Tokens T, const Pair* __restrict__ in, SortMeta* meta,
-                                                         SortPlan P, int shift, const uint32_t* __restrict__ counts,
-                                                         Pair* __restrict__ out, uint8_t* __restrict__ used) {
-    __shared__ uint32_t next[4][512];   // the wave's next free place of each digit
-    __shared__ uint32_t total[512], scan[256];
+__device__ __forceinline__ uint32_t sort_place(const Tokens& T, const Pair* in, int64_t count, const SortPlan& P,
+                                               int shift, const uint32_t* counts, Pair* out, SortSpace& S) {
     const int digits = 1 << P.bits, mask = digits - 1;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int64_t count = FIRST ? T.positions : (int64_t)meta->valid;
-    const int64_t lo = blockIdx.x * P.chunk, quarter = P.chunk / 4;
-    const int64_t w_lo = lo + wave * quarter;
-    int64_t w_hi = w_lo + quarter < count ? w_lo + quarter : count;
-    for (int d = threadIdx.x; d < digits; d += 256)
-#pragma unroll
-        for (int w = 0; w < 4; ++w) next[w][d] = 0;
+    const int64_t part = P.chunk / kSortWaves, w_lo = blockIdx.x * P.chunk + wave * part;
+    const int64_t w_hi = w_lo + part < count ? w_lo + part : count;
+    for (int i = threadIdx.x; i < kSortWaves * kSortDigits; i += kSortThreads) (&S.next[0][0])[i] = 0;
+    if (threadIdx.x < kSortDigits) S.total[threadIdx.x] = S.before[threadIdx.x] = 0;
     __syncthreads();
     for (int64_t i = w_lo + lane; i < w_hi; i += 64) {
         Pair p;
-        if (sort_item<IDX, FIRST>(T, in, i, w_hi, &p)) atomicAdd(&next[wave][(p.key >> shift) & mask], 1u);
+        if (sort_item<IDX, FIRST>(T, in, i, w_hi, &p)) atomicAdd(&S.next[wave][(p.key >> shift) & mask], 1u);
     }
-    // positions of this digit in the blocks before this one, and in all blocks
-    uint32_t before[2] = {0, 0};
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int d = threadIdx.x + h * 256;
-        if (d >= digits) continue;
-        uint32_t all = 0;
+    if (counts) {   // positions of each digit in all chunks, and in those before this one; several threads a digit
+        const int d = threadIdx.x & mask, each = kSortThreads >> P.bits, mine = threadIdx.x >> P.bits;
+        uint32_t all = 0, ahead = 0;
 #pragma unroll 8
-        for (int b = 0; b < P.blocks; ++b) {
+        for (int b = mine; b < P.blocks; b += each) {
             const uint32_t c = counts[(int64_t)b * digits + d];
-            if (b < (int)blockIdx.x) before[h] += c;
+            if (b < (int)blockIdx.x) ahead += c;
             all += c;
         }
-        total[d] = all;
+        atomicAdd(&S.total[d], all);
+        atomicAdd(&S.before[d], ahead);
     }
     __syncthreads();
-    // exclusive sums over the digits: two digits per thread (d and d + 1 next to each other)
-    uint32_t pair_sum = 0;
-    if (2 * (int)threadIdx.x < digits) pair_sum = total[2 * threadIdx.x] + (2 * (int)threadIdx.x + 1 < digits ? total[2 * threadIdx.x + 1] : 0);
-    scan[threadIdx.x] = pair_sum;
-    __syncthreads();
-    for (int o = 1; o < 256; o <<= 1) {
-        const uint32_t x = (int)threadIdx.x >= o ? scan[threadIdx.x - o] : 0;
-        __syncthreads();
-        scan[threadIdx.x] += x;
-        __syncthreads();
+    if (!counts && (int)threadIdx.x < digits) {
+        uint32_t all = 0;
+#pragma unroll
+        for (int w = 0; w < kSortWaves; ++w) all += S.next[w][threadIdx.x];
+        S.total[threadIdx.x] = all;
     }
-    if (FIRST && blockIdx.x == 0 && threadIdx.x == 255) meta->valid = scan[255];
+    __syncthreads();
+    if (threadIdx.x < kSortDigits) {   // inclusive sums over the digits, by wave
+        uint32_t x = S.total[threadIdx.x];
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t y = __shfl_up(x, o);
+            if (lane >= o) x += y;
+        }
+        S.scan[threadIdx.x] = x;
+    }
+    __syncthreads();
+    uint32_t lower = 0;
+    if (threadIdx.x < kSortDigits)
+        for (int w = 0; w < wave; ++w) lower += S.scan[64 * w + 63];
+    __syncthreads();
+    if (threadIdx.x < kSortDigits) S.scan[threadIdx.x] += lower;
+    __syncthreads();
+    if ((int)threadIdx.x < digits) {
+        uint32_t at = S.scan[threadIdx.x] - S.total[threadIdx.x] + S.before[threadIdx.x];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int d = threadIdx.x + h * 256;
-        if (d >= digits) continue;
-        const uint32_t upto = scan[d >> 1];   // through digit d | 1
-        uint32_t at = upto - total[d] - ((d & 1) == 0 && d + 1 < digits ? total[d + 1] : 0) + before[h];
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            const uint32_t c = next[w][d];
-            next[w][d] = at;
+        for (int w = 0; w < kSortWaves; ++w) {
+            const uint32_t c = S.next[w][threadIdx.x];
+            S.next[w][threadIdx.x] = at;
             at += c;
         }
     }
@@ -211,27 +219,53 @@ __global__ __launch_bounds__(256) void sort_place_kernel(Tokens T, const Pair* _
         }
         if (ok) {
             const uint64_t below = peers & ((1ull << lane) - 1);
-            const uint32_t first = next[wave][digit];
+            const uint32_t first = S.next[wave][digit];
             out[first + __popcll(below)] = p;
-            if (FIRST) used[p.key] = 1;   // every writer stores the same value
-            if ((peers >> lane) == 1) next[wave][digit] = first + __popcll(peers);
+            if ((peers >> lane) == 1) S.next[wave][digit] = first + __popcll(peers);
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // the next step reads what this one moved on
+    }
+    return S.scan[digits - 1];
+}
+
+template <typename IDX, bool FIRST>
+__global__ __launch_bounds__(kSortThreads) void sort_place_kernel(Tokens T, const Pair* __restrict__ in, SortMeta* meta,
+                                                                  SortPlan P, int shift,
+                                                                  const uint32_t* __restrict__ counts,
+                                                                  Pair* __restrict__ out) {
+    __shared__ SortSpace S;
+    const int64_t count = FIRST ? T.positions : (int64_t)meta->valid;
+    const uint32_t placed = sort_place<IDX, FIRST>(T, in, count, P, shift, counts, out, S);
+    if (FIRST && blockIdx.x == 0 && threadIdx.x == 0) meta->valid = placed;
+}
+
+// all passes of a list that one workgroup takes; the result lies in a or b as sort_tokens says
+template <typename IDX>
+__global__ __launch_bounds__(kSortThreads) void sort_alone_kernel(Tokens T, SortMeta* meta, SortPlan P, Pair* a, Pair* b) {
+    __shared__ SortSpace S;
+    const int64_t valid = sort_place<IDX, true>(T, nullptr, T.positions, P, 0, nullptr, a, S);
+    if (threadIdx.x == 0) meta->valid = (uint32_t)valid;
+    for (int pass = 1; pass < P.passes; ++pass) {
+        __syncthreads();   // the pairs are written: the workgroup shares its cache
+        sort_place<IDX, false>(T, pass & 1 ? a : b, valid, P, pass * P.bits, nullptr, pass & 1 ? b : a, S);
     }
 }
 
 // ---- gradient: the sums ---------------------------------------------------------------------------
-// A worker (one thread per chunk of EPV columns) walks `run` sorted positions and adds their rows while
-// the key stays the same.  A run of one key inside the worker's range is a finished table row; a run that
-// reaches over an end of the range leaves a partial sum: slot 0 what began before the range, slot 1 what
-// goes on behind it.  The workgroups behind the workers clear the table rows no valid position holds.
+// A worker (one thread per chunk of EPV columns) walks a range of `run` sorted positions and adds their rows while
+// the key stays the same.  A run of one key inside the range is a finished table row; a run that reaches over an
+// end of the range leaves a partial sum: slot 0 what began before the range, slot 1 what goes on behind it.  The
+// workgroups behind the workers clear the table rows that no valid position holds.  Bound by reading the gradient
+// and writing the table.  (Workers that read on behind their range to finish a run there leave only the longest
+// runs to the join, but are up to twice as long themselves: 154 us against 114 at 2,048 x 256 positions of 768 f16.)
 struct SumPlan {
-    int run;            // sorted positions per worker
+    int run;            // sorted positions of a range
     int cpr, rpp;       // chunks per row, workers side by side in a workgroup
     int64_t workers;    // over the largest possible number of valid positions
     int64_t sum_groups; // workgroups of workers; the rest clear rows
     int64_t pad_dim;    // floats of a partial row
 };
+constexpr int kClearRows = 64;   // table rows of a clearing workgroup: a lane of each looks for its row
 
 template <typename OT, int EPV>
 __device__ __forceinline__ void put_row(OT* table, int64_t key, int dim, int c, const float* acc, float scale) {
@@ -243,31 +277,44 @@ __device__ __forceinline__ void put_row(OT* table, int64_t key, int dim, int c, 
 
 template <typename GT, typename OT, int EPV>
 __global__ __launch_bounds__(256) void grad_sum_kernel(const GT* __restrict__ grad, const Pair* __restrict__ sorted,
-                                                       const SortMeta* __restrict__ meta,
-                                                       const uint8_t* __restrict__ used, int64_t vocab, float scale,
+                                                       const SortMeta* __restrict__ meta, int64_t vocab, float scale,
                                                        OT* __restrict__ table, int dim, SumPlan S,
                                                        float* __restrict__ partial, int32_t* __restrict__ chain_end) {
+    const int64_t valid = meta->valid;
+    if ((int64_t)blockIdx.x >= S.sum_groups) {
+        __shared__ uint64_t empty_rows;
+        const int64_t v0 = ((int64_t)blockIdx.x - S.sum_groups) * kClearRows;
+        if (threadIdx.x < 64) {
+            const int64_t v = v0 + threadIdx.x;
+            int64_t lo = 0, hi = valid;   // the first position whose key is not below v
+            while (lo < hi) {
+                const int64_t mid = (lo + hi) >> 1;
+                if ((int64_t)sorted[mid].key < v) lo = mid + 1;
+                else hi = mid;
+            }
+            const uint64_t found = __ballot(v < vocab && (lo >= valid || (int64_t)sorted[lo].key != v));
+            if (threadIdx.x == 0) empty_rows = found;
+        }
+        __syncthreads();
+        const float zero[EPV] = {};
+        for (uint64_t rows = empty_rows; rows; rows &= rows - 1)
+            for (int c = threadIdx.x; c < S.cpr; c += blockDim.x)
+                put_row<OT, EPV>(table, v0 + __ffsll((unsigned long long)rows) - 1, dim, c, zero, 1.0f);
+        return;
+    }
     const int r = S.cpr < 256 ? (int)threadIdx.x / S.cpr : 0;
     const int c0 = S.cpr < 256 ? (int)threadIdx.x - r * S.cpr : (int)threadIdx.x;
     if (r >= S.rpp) return;
-    if ((int64_t)blockIdx.x >= S.sum_groups) {
-        const float zero[EPV] = {};
-        for (int64_t v = ((int64_t)blockIdx.x - S.sum_groups) * S.rpp + r; v < vocab;
-             v += ((int64_t)gridDim.x - S.sum_groups) * S.rpp)
-            if (!used[v])
-                for (int c = c0; c < S.cpr; c += 256) put_row<OT, EPV>(table, v, dim, c, zero, 1.0f);
-        return;
-    }
     constexpr int U = 8;
-    const int64_t valid = meta->valid;
     const int64_t worker = (int64_t)blockIdx.x * S.rpp + r;
     const int64_t lo = worker * S.run, hi = lo + S.run < valid ? lo + S.run : valid;
     if (lo >= hi) return;
-    const bool head = lo > 0 && sorted[lo - 1].key == sorted[lo].key;
+    const uint32_t first_key = sorted[lo].key;
+    const bool head = lo > 0 && sorted[lo - 1].key == first_key;
     const bool tail = hi < valid && sorted[hi].key == sorted[hi - 1].key;
     for (int c = c0; c < S.cpr; c += 256) {
         float acc[EPV] = {};
-        uint32_t cur = sorted[lo].key;
+        uint32_t cur = first_key;
         bool first = true;   // the run that opens the range
         auto flush = [&](bool last) {
             if ((first && head) || (last && tail)) {
@@ -304,41 +351,71 @@ __global__ __launch_bounds__(256) void grad_sum_kernel(const GT* __restrict__ gr
     }
 }
 
-// The runs that cross workers: the worker a run starts in is followed by partial sums of slot 0 up to
-// chain_end.  A workgroup adds 64 columns of one run: 16 threads of 4 columns, 16 rows of partial sums side
-// by side, joined in a fixed order.
+// The runs that cross ranges: the range one begins in is followed by partial sums of slot 0 up to chain_end.  A
+// workgroup of sixteen waves takes sixteen ranges and 256 columns.  A run of up to kJoinShort partial sums is its
+// range's wave's; the longer ones are added by all waves, each every sixteenth partial sum, joined in order.
+constexpr int kJoinWaves = 16, kJoinShort = 16;
 template <typename OT>
-__global__ __launch_bounds__(256) void grad_join_kernel(const Pair* __restrict__ sorted,
-                                                        const SortMeta* __restrict__ meta, float scale,
-                                                        OT* __restrict__ table, int dim, SumPlan S,
-                                                        const float* __restrict__ partial,
-                                                        const int32_t* __restrict__ chain_end) {
-    __shared__ float part[16][64];
-    const int64_t valid = meta->valid;
-    const int col = blockIdx.y * 64 + (threadIdx.x & 15) * 4, lane = threadIdx.x >> 4;
-    for (int64_t w = blockIdx.x; (w + 1) * S.run < valid; w += gridDim.x) {
-        const int64_t lo = w * S.run, hi = lo + S.run;
-        const uint32_t key = sorted[hi - 1].key;
-        if (sorted[hi].key != key) continue;                                             // ends here
-        if (sorted[lo].key == key && lo > 0 && sorted[lo - 1].key == key) continue;      // did not start here
-        const int64_t n = chain_end[key] - w + 1;
-        float acc[4] = {0, 0, 0, 0};
-        if (col < (int)S.pad_dim)
-            for (int64_t i = lane; i < n; i += 16) {
+__global__ __launch_bounds__(64 * kJoinWaves) void grad_join_kernel(const Pair* __restrict__ sorted,
+                                                                    const SortMeta* __restrict__ meta, float scale,
+                                                                    OT* __restrict__ table, int dim, SumPlan S,
+                                                                    const float* __restrict__ partial,
+                                                                    const int32_t* __restrict__ chain_end) {
+    __shared__ float4 part[kJoinWaves][64];
+    __shared__ int longs[kJoinWaves];   // partial sums of a long run that begins in the wave's range
+    const int64_t valid = meta->valid, w0 = (int64_t)blockIdx.x * kJoinWaves;
+    if ((w0 + 1) * S.run >= valid) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int col = (blockIdx.y * 64 + lane) * 4;
+    auto add = [&](int64_t w, int64_t i0, int64_t n, int64_t step) {
+        float4 acc = make_float4(0, 0, 0, 0);
+        if (col < (int)S.pad_dim) {
+#pragma unroll 4
+            for (int64_t i = i0; i < n; i += step) {
                 const float4 x = *(const float4*)(partial + ((w + i) * 2 + (i == 0 ? 1 : 0)) * S.pad_dim + col);
-                acc[0] += x.x;
-                acc[1] += x.y;
-                acc[2] += x.z;
-                acc[3] += x.w;
+                acc.x += x.x;
+                acc.y += x.y;
+                acc.z += x.z;
+                acc.w += x.w;
             }
-        *(float4*)&part[lane][(threadIdx.x & 15) * 4] = make_float4(acc[0], acc[1], acc[2], acc[3]);
-        __syncthreads();
-        if (threadIdx.x < 64) {
-            const int c = blockIdx.y * 64 + threadIdx.x;
-            float sum = 0.0f;
+        }
+        return acc;
+    };
+    auto put = [&](uint32_t key, const float4& sum) {
+        const float y[4] = {sum.x, sum.y, sum.z, sum.w};
 #pragma unroll
-            for (int i = 0; i < 16; ++i) sum += part[i][threadIdx.x];
-            if (c < dim) table[(int64_t)key * dim + c] = from_f32<OT>(scale * sum);
+        for (int e = 0; e < 4; ++e)
+            if (col + e < dim) table[(int64_t)key * dim + col + e] = from_f32<OT>(scale * y[e]);
+    };
+    {
+        const int64_t w = w0 + wave, lo = w * S.run, hi = lo + S.run;
+        int64_t n = 0;
+        uint32_t key = 0;
+        if (hi < valid) {
+            key = sorted[hi - 1].key;
+            const bool began = lo > 0 && sorted[lo].key == key && sorted[lo - 1].key == key;
+            if (sorted[hi].key == key && !began) n = chain_end[key] - w + 1;
+        }
+        if (n > 0 && n <= kJoinShort) put(key, add(w, 0, n, 1));
+        if (lane == 0) longs[wave] = n > kJoinShort ? (int)n : 0;
+    }
+    __syncthreads();
+    for (int x = 0; x < kJoinWaves; ++x) {
+        const int n = longs[x];
+        if (!n) continue;
+        part[wave][lane] = add(w0 + x, wave, n, kJoinWaves);
+        __syncthreads();
+        if (wave == 0) {
+            float4 sum = part[0][lane];
+#pragma unroll
+            for (int i = 1; i < kJoinWaves; ++i) {
+                const float4 y = part[i][lane];
+                sum.x += y.x;
+                sum.y += y.y;
+                sum.z += y.z;
+                sum.w += y.w;
+            }
+            put(sorted[(w0 + x + 1) * S.run - 1].key, sum);
         }
         __syncthreads();
     }

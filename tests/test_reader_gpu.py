@@ -76,7 +76,7 @@ def grad_bound(want, total, count, dtype):
 
 
 SIZES = [(1, 1, 1, 8), (1, 24, 30522, 768), (3, 5, 7, 1), (5, 1, 50, 77), (2, 300, 11, 64), (67, 61, 28996, 1000),
-         (64, 129, 300, 2056), (33, 40, 512, 256), (9, 17, 513, 255), (1, 4097, 40, 16), (700, 13, 300000, 24)]
+         (64, 129, 300, 2056), (33, 40, 512, 256), (9, 17, 513, 255), (9, 17, 513, 770), (1, 4097, 40, 16), (3, 7001, 900, 18), (700, 13, 300000, 24)]
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16, F32])
