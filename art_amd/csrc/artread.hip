@@ -358,9 +358,25 @@ static AttendShape attend_shape(const artread_attend_t* a) {
     P.row_blocks = (P.row_count + block - 1) / block;
     P.items = a->batch * a->kv_heads * P.row_blocks;
     const int64_t tiles = a->passages * ((a->len + keys - 1) / keys);
-    int64_t want = ((S.stream ? 4096 : 512) + P.items - 1) / P.items, most = tiles / 4;   // a part of fewer tiles costs less than the join
-    want = want < most ? want : most;
-    P.splits = (int)(want < 1 ? 1 : (want < 256 ? want : 256));
+    P.walkers = 1;
+    if (S.stream) {
+        // Workgroups that fill the chip.  By registers two waves share a SIMD, three at 64 columns and 32 rows;
+        // a round more evens out the lengths, while each more leaves partial results to join (us, kernel + join,
+        // for 2048, 3072, 4096 waves: 64 questions x 32 passages x 64 columns 222, 203, 195; 2 x 100 x 128 columns
+        // 76, 87, 89; 48 rows 161, 151, 159).
+        const int64_t waves = a->dim > 64 ? 2048 : (S.qb == 2 ? 3072 : 4096);
+        int64_t want = (waves / 4 + P.items - 1) / P.items;
+        if (P.items < waves && tiles >= 4) P.walkers = 4;
+        else want = 1;
+        const int64_t most = tiles / 16;   // a part of fewer than four tiles a wave costs less than its join
+        want = want < most ? want : most;
+        P.splits = (int)(want < 1 ? 1 : (want < 256 ? want : 256));
+    } else {
+        int64_t want = (512 + P.items - 1) / P.items;
+        const int64_t most = tiles / 4;
+        want = want < most ? want : most;
+        P.splits = (int)(want < 1 ? 1 : (want < 256 ? want : 256));
+    }
     plan_scale(&P, a->scale, a->dtype);
     return S;
 }
@@ -374,7 +390,7 @@ template <typename T, int DP>
 static void launch_attend(const artread_attend_t* a, const AttendShape& S, const Partials& W, hipStream_t st) {
     const int64_t parts = S.plan.items * S.plan.splits;
     if (S.stream) {
-        const dim3 grid = grid2((parts + 3) / 4);
+        const dim3 grid = grid2(S.plan.walkers == 1 ? (parts + 3) / 4 : parts);
         if (S.qb == 1) hipLaunchKernelGGL((attend_stream_kernel<T, DP, 1>), grid, dim3(256), 0, st, *a, S.plan, W);
         else if constexpr (DP == 64) hipLaunchKernelGGL((attend_stream_kernel<T, DP, 2>), grid, dim3(256), 0, st, *a, S.plan, W);
     } else {

@@ -48,6 +48,7 @@ struct AttendPlan {
     int64_t row_blocks;   // blocks of rows per (batch entry, key head)
     int64_t items;        // batch x kv_heads x row_blocks
     uint32_t share, inv_share;   // heads per key head; floor(2^32 / share), 2^32 - 1 for 1
+    int walkers;          // waves of a workgroup that walk one item
     int splits;           // parts the keys of an item are dealt to
     int by_head;          // order of the key walk's items
     float c;              // |scale| * log2(e)
@@ -280,7 +281,6 @@ template <typename T, int DP>
 __device__ __forceinline__ void finish_rows(const artread_attend_t& A, const AttendPlan& P, const Partials& W, int64_t b,
                                             int64_t kh, int64_t r, int split, int half, float m, float l,
                                             f32x16 (&o)[DP / 32]) {
-    l = both_sum(l);
     if (r >= P.row_count) return;
     const int dim = (int)A.dim;
     if (P.splits > 1) {
@@ -391,19 +391,29 @@ __device__ __forceinline__ void load_q(const artread_attend_t& A, const AttendPl
 // ---- few rows: one wave walks its tiles alone ----------------------------------------------------------
 // QB x 32 rows per wave, 32 keys per tile.  Every key and value is read once, so this is bound by HBM: K goes
 // straight from memory into the A operand, V through a tile of LDS of the wave's own for the transposing read,
-// the next tile's loads are in flight while this one is worked on, and no wave waits for another.
+// the next tile's loads are in flight while this one is worked on, and no wave waits for another.  Where items are
+// few, the four waves of a workgroup walk one item between them (P.walkers of 4) and join what they have in LDS,
+// so that a quarter of the partial results is left to the join kernel, or none.
 template <typename T, int DP, int QB>
-__global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void attend_stream_kernel(artread_attend_t A, AttendPlan P, Partials W) {
-    __shared__ __attribute__((aligned(16))) T tiles[4][32 * DP];
+__global__ __launch_bounds__(256, 2) void attend_stream_kernel(artread_attend_t A, AttendPlan P, Partials W) {
+    constexpr int SLOT = QB * (DP / 2 + 2) * 64;   // floats of a wave's accumulators, maxima and sums
+    constexpr int TILES = 4 * 32 * DP * 2, SLOTS = 2 * SLOT * 4;
+    __shared__ __attribute__((aligned(1024))) char lds[TILES > SLOTS ? TILES : SLOTS];
     typedef typename Mma<T>::V8 V8;
     const int lane = threadIdx.x & 63, half = lane >> 5, wave = uniform(threadIdx.x >> 6);
-    T* tile = tiles[wave];
+    T* tile = (T*)lds + wave * 32 * DP;
     const int dim = (int)A.dim;
-    const int64_t waves = P.items * P.splits;
-    const int64_t w = block_id() * 4 + wave;
-    if (w >= waves) return;   // no barrier in this kernel
-    const int split = (int)(w % P.splits);
-    const int64_t item = w / P.splits, rb = item % P.row_blocks, bk = item / P.row_blocks;
+    int64_t item = block_id();
+    int split = 0, group = 0;
+    if (P.walkers == 1) {
+        item = item * 4 + wave;
+    } else {
+        group = (int)(item % P.splits);
+        item /= P.splits;
+        split = group * 4 + wave;
+    }
+    if (item >= P.items) return;   // whole workgroups where they have barriers
+    const int64_t rb = item % P.row_blocks, bk = item / P.row_blocks;
     const int64_t kh = bk % A.kv_heads, b = bk / A.kv_heads, r0 = rb * 32 * QB + (lane & 31);
     V8 q[QB][DP / 16];
     f32x16 o[QB][DP / 32];
@@ -423,7 +433,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void attend_stream_kernel(ar
     const T* vbase = (const T*)A.v + b * A.v_batch + kh * A.v_head + (int64_t)vrow * A.v_row + 8 * vchunk;
     V8 kr[DP / 16], vr[VN];
     Walk<32> walk;
-    walk.start(A, b, split, P.splits);
+    walk.start(A, b, split, P.splits * P.walkers);
     auto load = [&]() {
         const int left = walk.n - walk.j0;
         const T* kp = kbase + walk.p * A.k_passage + walk.j0 * A.k_row;
@@ -471,7 +481,42 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void attend_stream_kernel(ar
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
 #pragma unroll
-    for (int x = 0; x < QB; ++x) finish_rows<T, DP>(A, P, W, b, kh, r0 + 32 * x, split, half, m[x], l[x], o[x]);
+    for (int x = 0; x < QB; ++x) l[x] = both_sum(l[x]);
+    if (P.walkers > 1) {
+        float* slots = (float*)lds;
+#pragma unroll
+        for (int step = 2; step; step >>= 1) {
+            __syncthreads();   // tiles, and the slots of the step before, are read
+            if (wave >= step && wave < 2 * step) {
+                float* at = slots + (wave - step) * SLOT + lane;
+#pragma unroll
+                for (int x = 0; x < QB; ++x) {
+                    at[(x * 2) * 64] = m[x];
+                    at[(x * 2 + 1) * 64] = l[x];
+#pragma unroll
+                    for (int i = 0; i < DP / 2; ++i) at[(QB * 2 + x * (DP / 2) + i) * 64] = o[x][i >> 4][i & 15];
+                }
+            }
+            __syncthreads();
+            if (wave < step) {
+                const float* at = slots + wave * SLOT + lane;
+#pragma unroll
+                for (int x = 0; x < QB; ++x) {
+                    const float m2 = at[(x * 2) * 64], l2 = at[(x * 2 + 1) * 64], m1 = fmaxf(m[x], m2);
+                    const float base = m1 == -INFINITY ? 0.0f : m1;   // no key so far: zeros stay zeros
+                    const float f = __builtin_amdgcn_exp2f(m[x] - base), f2 = __builtin_amdgcn_exp2f(m2 - base);
+                    m[x] = m1;
+                    l[x] = l[x] * f + l2 * f2;
+#pragma unroll
+                    for (int i = 0; i < DP / 2; ++i)
+                        o[x][i >> 4][i & 15] = o[x][i >> 4][i & 15] * f + at[(QB * 2 + x * (DP / 2) + i) * 64] * f2;
+                }
+            }
+        }
+        if (wave > 0) return;
+    }
+#pragma unroll
+    for (int x = 0; x < QB; ++x) finish_rows<T, DP>(A, P, W, b, kh, r0 + 32 * x, group, half, m[x], l[x], o[x]);
 }
 
 // ---- many rows: four waves share the tiles --------------------------------------------------------------
@@ -592,5 +637,5 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(artread_attend_t A,
         left = next;
         stage ^= 1;
     }
-    finish_rows<T, DP>(A, P, W, b, kh, r, split, half, m, l, o);
+    finish_rows<T, DP>(A, P, W, b, kh, r, split, half, m, both_sum(l), o);
 }

@@ -142,6 +142,24 @@ def _embed(tokens, table, lengths, scale, vocab_base, out_dtype):
     return out
 
 
+def _embed_grad(grad_out, tokens, lengths, vocab, scale, vocab_base, dtype):
+    dev, dim, length, positions = grad_out.device, grad_out.shape[-1], tokens.shape[-1], tokens.numel()
+    if positions * dim == 0:
+        return torch.zeros((vocab, dim), dtype=dtype, device=dev)
+    out = torch.empty((vocab, dim), dtype=dtype, device=dev)
+    grad_out, tokens = grad_out.contiguous(), tokens.contiguous()
+    lengths = lengths.contiguous() if lengths is not None else None
+    n, lib = positions // length, _read()
+    size = lib.artread_embed_grad_workspace(vocab, dim, n, length)
+    with _on_device(dev):
+        ws = torch.empty((size,), dtype=torch.uint8, device=dev)
+        _rcheck(lib.artread_embed_grad(
+            dev.index, grad_out.data_ptr(), _ABI[grad_out.dtype], tokens.data_ptr(), tokens.element_size(),
+            lengths.data_ptr() if lengths is not None else None, n, length, vocab, dim, vocab_base, scale,
+            out.data_ptr(), _ABI[dtype], ws.data_ptr(), size, _stream(dev)))
+    return out
+
+
 class _EmbedTokens(torch.autograd.Function):
     @staticmethod
     def forward(ctx, table, tokens, lengths, scale, vocab_base, out_dtype):
@@ -154,8 +172,7 @@ class _EmbedTokens(torch.autograd.Function):
     def backward(ctx, grad_out):
         tokens, lengths = ctx.saved_tensors
         vocab, scale, vocab_base, dtype = ctx.of
-        return (embed_tokens_grad(grad_out, tokens, vocab, lengths, scale=scale, vocab_base=vocab_base,
-                                  dtype=dtype),) + (None,) * 5
+        return _embed_grad(grad_out, tokens, lengths, vocab, scale, vocab_base, dtype), None, None, None, None, None
 
 
 def embed_tokens(tokens, table, lengths=None, scale=1.0, vocab_base=0, out_dtype=None):
@@ -198,22 +215,8 @@ def embed_tokens_grad(grad_out, tokens, vocab, lengths=None, scale=1.0, vocab_ba
     if dtype != grad_out.dtype and dtype != torch.float32:
         raise ValueError("dtype must be grad_out's type or float32")
     scale = _scale_value(scale)
-    dev = _one_device(grad_out, tokens, lengths)
-    dim, length = grad_out.shape[-1], tokens.shape[-1]
-    if grad_out.numel() == 0:
-        return torch.zeros((vocab, dim), dtype=dtype, device=dev)
-    out = torch.empty((vocab, dim), dtype=dtype, device=dev)
-    grad_out, tokens = grad_out.contiguous(), tokens.contiguous()
-    lengths = lengths.contiguous() if lengths is not None else None
-    n = tokens.numel() // length
-    size = _read().artread_embed_grad_workspace(vocab, dim, n, length)
-    with _on_device(dev):
-        ws = torch.empty((size,), dtype=torch.uint8, device=dev)
-        _rcheck(_read().artread_embed_grad(
-            dev.index, grad_out.data_ptr(), _ABI[grad_out.dtype], tokens.data_ptr(), tokens.element_size(),
-            lengths.data_ptr() if lengths is not None else None, n, length, vocab, dim, int(vocab_base), scale,
-            out.data_ptr(), _ABI[dtype], ws.data_ptr(), size, _stream(dev)))
-    return out
+    _one_device(grad_out, tokens, lengths)
+    return _embed_grad(grad_out, tokens, lengths, vocab, scale, int(vocab_base), dtype)
 
 
 # ---- cross attention ------------------------------------------------------------------------------
