@@ -442,7 +442,7 @@ static GradShape grad_shape(const artread_attend_t* a) {
     plan_share(&Q, a);
     Q.row_count = a->rows * Q.share;
     plan_scale(&Q, a->scale, a->dtype);
-    Q.pad_rows = round_up(Q.row_count, 32);
+    Q.pad_rows = round_up(Q.row_count, 64);
     Q.c = a->scale * kLog2e;   // no maximum is taken here: c may be negative or zero
     Q.q_and = 0xffffffffu;
     Q.q_xor = 0u;
@@ -470,7 +470,7 @@ static GradShape grad_shape(const artread_attend_t* a) {
     K.by_head = K.row_count > 64;
     K.items = a->batch * a->passages * ((a->len + 127) / 128) * a->kv_heads;
     want = (512 + K.items - 1) / K.items;
-    most = (K.row_count + 31) / 32 / 4;
+    most = (K.row_count + 63) / 64 / 2;
     want = want < most ? want : most;
     K.splits = (int)(want < 1 ? 1 : (want < 64 ? want : 64));
     S.all_q = a->batch * a->rows * a->heads * a->dim;

@@ -44,7 +44,7 @@ __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirs
 // ---- the problem as the kernels see it --------------------------------------------------------------
 struct AttendPlan {
     int64_t row_count;    // rows x share
-    int64_t pad_rows;     // row_count in whole tiles of 32: the gradient's row statistics
+    int64_t pad_rows;     // row_count in whole tiles of 64: the gradient's row statistics
     int64_t row_blocks;   // blocks of rows per (batch entry, key head)
     int64_t items;        // batch x kv_heads x row_blocks
     uint32_t share, inv_share;   // heads per key head; floor(2^32 / share), 2^32 - 1 for 1

@@ -17,7 +17,7 @@ struct RowStat {
     float x, delta;
 };
 
-// 16 lanes per row, eight columns each.  The rows of a key head are padded to whole tiles of 32.
+// 16 lanes per row, eight columns each.  The rows of a key head are padded to whole tiles of 64.
 template <typename T>
 __global__ __launch_bounds__(256) void attend_delta_kernel(artread_attend_t A, artread_attend_grads_t G, AttendPlan P,
                                                            int64_t all_rows, RowStat* __restrict__ stats) {
@@ -130,6 +130,55 @@ __device__ __forceinline__ void put4(T* p, const float* x) {
     store_vec<T, 4>(p, w);
 }
 
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+template <typename T>
+__device__ __forceinline__ u32x2 pack4(float a, float b, float c, float d) {
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    const T4 w = {(T)a, (T)b, (T)c, (T)d};
+    return __builtin_bit_cast(u32x2, w);
+}
+
+// Accumulators of 32 keys (lane: key, elements: columns), times f, rounded, as rows: through 4 KiB of LDS of the
+// wave's own, 64 columns at a time, so that eight lanes hold 128 bytes of a row.  Stores of 8 bytes by 64 rows would
+// ask the L2 for eight times as many writes, which bound the gradient of few rows (456 us against 292).
+// w[4 * c + x]: row 8 * x + (lane >> 3), columns 64 * c + 8 * (lane & 7)..
+template <typename T, int DP>
+__device__ __forceinline__ void turn_keys(const f32x16 (&acc)[DP / 32], float f, bool key, uint32_t lds, int lane,
+                                          u32x4 (&w)[DP / 16]) {
+    typedef __attribute__((address_space(3))) u32x2 lds_u32x2;
+    const int ln = (int)opaque(lane), row = ln & 31;
+#pragma unroll
+    for (int c = 0; c < DP / 64; ++c) {
+#pragma unroll
+        for (int y = 0; y < 8; ++y) {
+            const f32x16& v = acc[2 * c + (y >> 2)];
+            const int i = 4 * (y & 3);
+            u32x2 t = pack4<T>(f * v[i], f * v[i + 1], f * v[i + 2], f * v[i + 3]);
+            if (!key) t = u32x2{0, 0};   // behind the length: zeros, whatever the accumulators hold
+            *(lds_u32x2*)(uintptr_t)(lds + (uint32_t)(row * 128 + ((y ^ (row & 7)) * 16) + (ln >> 5) * 8)) = t;
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const int r = 8 * x + (ln >> 3);
+            w[4 * c + x] = *(__attribute__((address_space(3))) u32x4*)(uintptr_t)(lds + (uint32_t)(r * 128 + (((ln & 7) ^ (r & 7)) * 16)));
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+}
+// and their way to memory: at(row) is the first element of row `row` of the 32, for those below `rows`
+template <typename T, int DP>
+__device__ __forceinline__ void store_turned(T* first, int64_t stride, int rows, int dim, int lane, const u32x4 (&w)[DP / 16]) {
+    const int ln = (int)opaque(lane), d = 8 * (ln & 7);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+        const int r = 8 * x + (ln >> 3);
+#pragma unroll
+        for (int c = 0; c < DP / 64; ++c)
+            if (r < rows && 64 * c + d < dim) *(u32x4*)(first + r * stride + 64 * c + d) = w[4 * c + x];
+    }
+}
+
 // ---- dQ: the row walk -----------------------------------------------------------------------------------
 // NW waves of 32 rows share tiles of 32 * KB keys; while a tile is worked on the next one arrives in LDS.  With P.splits > 1 each split leaves
 // its f32 part of dQ at part + split * (all of dQ).
@@ -232,16 +281,16 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_grad_q_kernel(artread_atten
 }
 
 // ---- dK and dV: the key walk ------------------------------------------------------------------------------
-// Four waves of 32 keys of one passage share tiles of 32 rows of Q and dO, fetched two tiles ahead into a ring of
-// three in LDS: each is read as rows for S and dP and transposed for dK and dV.  With P.splits > 1 the rows are dealt
+// Four waves of 32 keys of one passage share tiles of 64 rows of Q and dO; while a tile is worked on the next one
+// arrives in LDS.  Each is read as rows for S and dP and transposed for dK and dV.  With P.splits > 1 the rows are dealt
 // to splits, which leave f32 parts of dK and dV.
 template <typename T, int DP>
 __global__ __launch_bounds__(256, 2) void attend_grad_kv_kernel(artread_attend_t A, artread_attend_grads_t G,
                                                                   AttendPlan P, const RowStat* __restrict__ stats,
                                                                   float* __restrict__ part) {
-    constexpr int STAGES = 3;
-    __shared__ __attribute__((aligned(1024))) T qtile[2 * STAGES][32 * DP];   // Q's tiles and behind them dO's
-    __shared__ __attribute__((aligned(1024))) RowStat stile[STAGES][4][32];   // a copy for each wave
+    constexpr int RT = 2, TILE = 32 * RT * DP;
+    __shared__ __attribute__((aligned(1024))) T qtile[4][TILE];               // two tiles of Q, two of dO
+    __shared__ __attribute__((aligned(1024))) RowStat stile[2][4][32 * RT];   // a copy for each wave
     typedef typename Mma<T>::V8 V8;
     const int lane = threadIdx.x & 63, half = lane >> 5, wave = uniform(threadIdx.x >> 6);
     const int dim = (int)A.dim;
@@ -290,112 +339,113 @@ __global__ __launch_bounds__(256, 2) void attend_grad_kv_kernel(artread_attend_t
         }
         // pieces of 1 KiB: PR rows each, PW of a tile for each wave; rows that are not there repeat the last one
         // (their weight is zero), columns behind dim the first (they meet zeros of K and V)
-        constexpr int CH = DP / 8, PR = 64 / CH, PW = 32 / PR / 4;
-        const int prow = lane / CH, tiles = (int)((P.row_count + 31) / 32);
+        constexpr int CH = DP / 8, PR = 64 / CH, PW = 32 * RT / PR / 4;
+        const int tiles = (int)((P.row_count + 32 * RT - 1) / (32 * RT));
         const RowStat* sp = stats + (b * A.kv_heads + kh) * P.pad_rows;
         const T* qb = (const T*)A.q + b * A.q_batch + kh * P.share * A.q_head;
         const T* gb = (const T*)G.grad_out + b * G.g_batch + kh * P.share * G.g_head;
         auto fetch = [&](int tile, int stage) {
             int64_t t0, h0;
-            split_row(P, 0, (uint32_t)tile * 32, &t0, &h0);
+            split_row(P, 0, (uint32_t)tile * 32 * RT, &t0, &h0);
+            const int ln = (int)opaque(lane), prow = ln / CH;
 #pragma unroll
             for (int x = 0; x < PW; ++x) {
                 const int piece = wave * PW + x, row = piece * PR + prow;
-                int64_t r = (int64_t)tile * 32 + row, t, h;
+                int64_t r = (int64_t)tile * 32 * RT + row, t, h;
                 r = r < P.row_count ? r : P.row_count - 1;
                 split_row(P, 0, (uint32_t)r, &t, &h);
-                int col = tile_chunk<DP>(row, lane % CH) * 8;
+                int col = tile_chunk<DP>(row, ln % CH) * 8;
                 col = col < dim ? col : 0;
-                // bytes from the tile's first query position: a tile spans at most 32 of them
+                // bytes from the tile's first query position: a tile spans at most as many of them as rows
                 const uint32_t dt = (uint32_t)t - (uint32_t)t0;
                 dma16(qb + t0 * A.q_row, (dt * (uint32_t)A.q_row + (uint32_t)(h * A.q_head) + col) * 2, lds_offset(&qtile[stage][piece * 512]));
-                dma16(gb + t0 * G.g_row, (dt * (uint32_t)G.g_row + (uint32_t)(h * G.g_head) + col) * 2, lds_offset(&qtile[STAGES + stage][piece * 512]));
+                dma16(gb + t0 * G.g_row, (dt * (uint32_t)G.g_row + (uint32_t)(h * G.g_head) + col) * 2, lds_offset(&qtile[2 + stage][piece * 512]));
             }
-            dma4(sp + tile * 32, (uint32_t)lane * 4, lds_offset(&stile[stage][wave][0]));
+#pragma unroll
+            for (int x = 0; x < RT; ++x)   // the statistics are padded to whole tiles
+                dma4(sp + tile * 32 * RT + 32 * x, (uint32_t)lane * 4, lds_offset(&stile[stage][wave][32 * x]));
         };
-        constexpr int LOADS = 2 * PW + 1;
         if (split < tiles) fetch(split, 0);
-        if (split + P.splits < tiles) fetch(split + P.splits, 1);
         // one loop for waves with keys and one for those without: both load and meet at the barriers
         auto go = [&](auto with_keys) {
             int stage = 0;
             for (int tile = split; tile < tiles; tile += P.splits) {
-                if (tile + P.splits < tiles) dma_wait<LOADS>();   // all but the next tile's
-                else dma_wait<0>();
+                dma_wait<0>();
                 wave_meet();   // everyone's pieces are there, and everyone is done with the tile before
-                const int ahead = stage == 0 ? 2 : stage - 1;
-                if (tile + 2 * P.splits < tiles) fetch(tile + 2 * P.splits, ahead);
+                if (tile + P.splits < tiles) fetch(tile + P.splits, stage ^ 1);
                 if constexpr (decltype(with_keys)::value) {
                     const uint32_t qrow = opaque(lds_offset(qtile[stage]) + rows_base<DP>(lane));
                     const uint32_t qcol = opaque(lds_offset(qtile[stage]) + columns_base<DP>(lane));
-                    f32x16 s = f32x16{}, dp = f32x16{};
 #pragma unroll
-                    for (int k = 0; k < DP / 16; ++k) {
-                        s = Mma<T>::mul(lds_rows<T, DP>(qrow, 0, k), kf[k], s);
-                        dp = Mma<T>::mul(lds_rows<T, DP>(qrow, STAGES, k), vf[k], dp);
-                    }
+                    for (int x = 0; x < RT; ++x) {
+                        f32x16 s = f32x16{}, dp = f32x16{};
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        const float4 a = *(const float4*)&stile[stage][wave][8 * x + 4 * half];
-                        const float4 c = *(const float4*)&stile[stage][wave][8 * x + 4 * half + 2];
-                        const float xs[4] = {a.x, a.z, c.x, c.z}, ds[4] = {a.y, a.w, c.y, c.w};
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int i = 4 * x + e;
-                            s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], P.c, -xs[e]));
-                            dp[i] = s[i] * (dp[i] - ds[e]);
+                        for (int k = 0; k < DP / 16; ++k) {
+                            s = Mma<T>::mul(lds_rows<T, DP>(qrow, x, k), kf[k], s);
+                            dp = Mma<T>::mul(lds_rows<T, DP>(qrow, 2 * RT + x, k), vf[k], dp);
                         }
-                    }
-                    spread.fit(dp, dk);
 #pragma unroll
-                    for (int ks = 0; ks < 2; ++ks) {
-                        const V8 pw = weights8<T>(s, ks), ds = weights8<T>(dp, ks);
+                        for (int y = 0; y < 4; ++y) {
+                            const float4 a = *(const float4*)&stile[stage][wave][32 * x + 8 * y + 4 * half];
+                            const float4 c = *(const float4*)&stile[stage][wave][32 * x + 8 * y + 4 * half + 2];
+                            const float xs[4] = {a.x, a.z, c.x, c.z}, ds[4] = {a.y, a.w, c.y, c.w};
 #pragma unroll
-                        for (int db = 0; db < DP / 32; ++db) {
-                            dv[db] = Mma<T>::mul(lds_columns<T, DP>(qcol, STAGES * 32 + 16 * ks, db), pw, dv[db]);
-                            dk[db] = Mma<T>::mul(lds_columns<T, DP>(qcol, 16 * ks, db), ds, dk[db]);
+                            for (int e = 0; e < 4; ++e) {
+                                const int i = 4 * y + e;
+                                s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], P.c, -xs[e]));
+                                dp[i] = s[i] * (dp[i] - ds[e]);
+                            }
                         }
+                        spread.fit(dp, dk);
+#pragma unroll
+                        for (int ks = 0; ks < 2; ++ks) {
+                            const V8 pw = weights8<T>(s, ks), ds = weights8<T>(dp, ks);
+#pragma unroll
+                            for (int db = 0; db < DP / 32; ++db) {
+                                dv[db] = Mma<T>::mul(lds_columns<T, DP>(qcol, 32 * (2 * RT + x) + 16 * ks, db), pw, dv[db]);
+                                dk[db] = Mma<T>::mul(lds_columns<T, DP>(qcol, 32 * x + 16 * ks, db), ds, dk[db]);
+                            }
+                        }
+                        __builtin_amdgcn_sched_barrier(0);   // the next rows' operands would not fit beside these
                     }
                 }
-                stage = stage == 2 ? 0 : stage + 1;
+                stage ^= 1;
             }
         };
         if (j0 + 32 * wave < n) go(std::true_type{});   // uniform over the wave
         else go(std::false_type{});
     }
-    if (j < A.len) {
-        const int64_t at = (((b * A.passages + p) * A.len + j) * A.kv_heads + kh) * dim;
-        const int64_t all = A.batch * A.passages * A.len * A.kv_heads * dim;
-        const float fv = P.unweight, fk = A.scale * spread.inverse() * P.unweight;
-#pragma unroll
-        for (int db = 0; db < DP / 32; ++db)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                const int d = 32 * db + 8 * x + 4 * half;
-                if (d >= dim) continue;
-                float yk[4], yv[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {   // behind the length: zeros, whatever the accumulators hold
-                    yk[e] = j < n ? fk * dk[db][4 * x + e] : 0.0f;
-                    yv[e] = j < n ? fv * dv[db][4 * x + e] : 0.0f;
-                }
-                if (P.splits > 1) {
-                    *(float4*)(part + split * 2 * all + at + d) = make_float4(yk[0], yk[1], yk[2], yk[3]);
-                    *(float4*)(part + (split * 2 + 1) * all + at + d) = make_float4(yv[0], yv[1], yv[2], yv[3]);
-                } else {
-                    put4<T>((T*)G.grad_k + at + d, yk);
-                    put4<T>((T*)G.grad_v + at + d, yv);
-                }
-            }
+    const int64_t all = A.batch * A.passages * A.len * A.kv_heads * dim;
+    const float fv = P.unweight, fk = A.scale * spread.inverse() * P.unweight;
+    if (P.splits == 1) {
+        __syncthreads();   // the tiles are read
+        const uint32_t own = lds_offset(&qtile[0][0]) + (uint32_t)wave * 4096;
+        const int64_t j1 = j0 + 32 * wave, at = (((b * A.passages + p) * A.len + j1) * A.kv_heads + kh) * dim;
+        const int rows = A.len - j1 < 32 ? (int)(A.len - j1) : 32;
+        u32x4 w[DP / 16];
+        turn_keys<T, DP>(dv, fv, j < n, own, lane, w);
+        store_turned<T, DP>((T*)G.grad_v + at, A.kv_heads * dim, rows, dim, lane, w);
+        turn_keys<T, DP>(dk, fk, j < n, own, lane, w);
+        store_turned<T, DP>((T*)G.grad_k + at, A.kv_heads * dim, rows, dim, lane, w);
+        return;
     }
-}
-
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-template <typename T>
-__device__ __forceinline__ u32x2 pack4(float a, float b, float c, float d) {
-    typedef T T4 __attribute__((ext_vector_type(4)));
-    const T4 w = {(T)a, (T)b, (T)c, (T)d};
-    return __builtin_bit_cast(u32x2, w);
+    if (j >= A.len) return;
+    const int64_t at = (((b * A.passages + p) * A.len + j) * A.kv_heads + kh) * dim;
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const int d = 32 * db + 8 * x + 4 * half;
+            if (d >= dim) continue;
+            float yk[4], yv[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {   // behind the length: zeros, whatever the accumulators hold
+                yk[e] = j < n ? fk * dk[db][4 * x + e] : 0.0f;
+                yv[e] = j < n ? fv * dv[db][4 * x + e] : 0.0f;
+            }
+            *(float4*)(part + split * 2 * all + at + d) = make_float4(yk[0], yk[1], yk[2], yk[3]);
+            *(float4*)(part + (split * 2 + 1) * all + at + d) = make_float4(yv[0], yv[1], yv[2], yv[3]);
+        }
 }
 
 // ---- all three gradients at once: few rows -----------------------------------------------------------------
@@ -472,42 +522,11 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_grad_stream_kernel(artread_
     f32x16 dk[DP / 32], dv[DP / 32];
     u32x4 wk[DP / 16], wv[DP / 16];   // the tile before's, rounded, and where it was
     int held_p = -1, held_j = 0;
-    auto store = [&]() {   // whole rows of 128 bytes: eight lanes each
+    auto store = [&]() {
         if (held_p < 0) return;
-        const int ln = (int)opaque(lane);
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-            const int j = held_j + 8 * x + (ln >> 3), d = 8 * (ln & 7);
-            const int64_t at = (((b * A.passages + held_p) * A.len + j) * A.kv_heads + kh) * dim + d;
-#pragma unroll
-            for (int c = 0; c < DP / 64; ++c)
-                if (j < len && 64 * c + d < dim) {
-                    *(u32x4*)((T*)G.grad_k + at + 64 * c) = wk[4 * c + x];
-                    *(u32x4*)((T*)G.grad_v + at + 64 * c) = wv[4 * c + x];
-                }
-        }
-    };
-    // accumulators of a tile (lane: key, elements: columns) -> rows, through 4 KiB of LDS, 64 columns at a time
-    auto turn = [&](const f32x16 (&acc)[DP / 32], float f, bool key, u32x4 (&w)[DP / 16]) {
-        const int ln = (int)opaque(lane), row = ln & 31;
-#pragma unroll
-        for (int c = 0; c < DP / 64; ++c) {
-#pragma unroll
-            for (int y = 0; y < 8; ++y) {
-                const f32x16& v = acc[2 * c + (y >> 2)];
-                const int i = 4 * (y & 3);
-                u32x2 t = pack4<T>(f * v[i], f * v[i + 1], f * v[i + 2], f * v[i + 3]);
-                if (!key) t = u32x2{0, 0};   // behind the length: zeros, whatever the accumulators hold
-                *(lds_u32x2*)(uintptr_t)(pd + (uint32_t)(row * 128 + ((y ^ (row & 7)) * 16) + (ln >> 5) * 8)) = t;
-            }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                const int r = 8 * x + (ln >> 3);
-                w[4 * c + x] = *(__attribute__((address_space(3))) u32x4*)(uintptr_t)(pd + (uint32_t)(r * 128 + (((ln & 7) ^ (r & 7)) * 16)));
-            }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        }
+        const int64_t at = (((b * A.passages + held_p) * A.len + held_j) * A.kv_heads + kh) * dim;
+        store_turned<T, DP>((T*)G.grad_k + at, A.kv_heads * dim, len - held_j, dim, lane, wk);
+        store_turned<T, DP>((T*)G.grad_v + at, A.kv_heads * dim, len - held_j, dim, lane, wv);
     };
     // dV and dK += the products of row block x, whose P and dS stand in LDS
     auto add_block = [&](int x) {
@@ -616,8 +635,8 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_grad_stream_kernel(artread_
         if (now > 0) add_block(RB - 1);
         const float fk = A.scale * spread_k.inverse() * P.unweight;
         const bool key = (lane & 31) < now;
-        turn(dv, P.unweight, key, wv);
-        turn(dk, fk, key, wk);
+        turn_keys<T, DP>(dv, P.unweight, key, pd, lane, wv);
+        turn_keys<T, DP>(dk, fk, key, pd, lane, wk);
     }
     // dQ of the workgroup: [wave][d][row]
     float* sums = (float*)lds;
