@@ -293,6 +293,7 @@ static int check_attend(const artread_attend_t* a) {
     READ_ARG((double)a->batch * a->rows * a->heads < (double)kLimit &&
                  (double)a->batch * a->passages * a->len * a->kv_heads < (double)kLimit,
              "q and k hold at most 2^31 - 1 rows each");
+    READ_ARG(a->passages * a->len <= kLimit - (1 << 20), "a batch entry holds at most 2^31 - 2^20 states");
     READ_ARG(isfinite(a->scale), "scale must be finite");
     const int64_t strides[11] = {a->q_batch, a->q_row, a->q_head, a->k_batch, a->k_passage, a->k_row,
                                  a->k_head, a->v_batch, a->v_passage, a->v_row, a->v_head};
@@ -322,6 +323,7 @@ static dim3 grid2(int64_t items) {   // at least `items` workgroups, a multiple 
 // How a forward call runs.  Up to 32 rows (64 at 64 columns) of a key head are one wave's, which streams the
 // keys; more share their tiles of keys in a workgroup.
 struct AttendShape {
+    artread_attend_t args;   // as the kernels take them
     bool stream;
     int qb;
     AttendPlan plan;
@@ -347,9 +349,28 @@ static void plan_share(AttendPlan* P, const artread_attend_t* a) {
     P->share = (uint32_t)(a->heads / a->kv_heads);
     P->inv_share = P->share == 1 ? 0xffffffffu : (uint32_t)(((uint64_t)1 << 32) / P->share);
 }
-static AttendShape attend_shape(const artread_attend_t* a) {
+// Passages that lie one behind the other are one long passage where every entry is valid, and one with holes where they
+// are short: of a tile of keys a passage of 7 would fill 7.  Longer ones keep tiles of their own, which end with them.
+constexpr int64_t kPackLength = 32;
+static artread_attend_t pack_passages(const artread_attend_t* given, AttendPlan* P) {
+    artread_attend_t a = *given;
+    P->pack = P->inv_pack = 0;
+    P->pack_passages = a.passages;
+    if (a.passages > 1 && (!a.lengths || a.len <= kPackLength) && a.k_passage == a.len * a.k_row && a.v_passage == a.len * a.v_row) {
+        if (a.lengths) {
+            P->pack = (uint32_t)a.len;
+            P->inv_pack = a.len == 1 ? 0xffffffffu : (uint32_t)(((uint64_t)1 << 32) / (uint64_t)a.len);
+        }
+        a.len *= a.passages;
+        a.passages = 1;
+    }
+    return a;
+}
+static AttendShape attend_shape(const artread_attend_t* given) {
     AttendShape S;
     AttendPlan& P = S.plan;
+    S.args = pack_passages(given, &P);
+    const artread_attend_t* a = &S.args;
     plan_share(&P, a);
     P.row_count = a->rows * P.share;
     S.stream = P.row_count <= (a->dim <= 64 ? 64 : 32);
@@ -415,6 +436,7 @@ extern "C" int artread_attend(int device, const artread_attend_t* a, void* works
     ReadDeviceGuard g(device);
     READ_HIP(g.err);
     hipStream_t st = (hipStream_t)stream;
+    a = &S.args;
     if (a->dtype == ARTREAD_F16) {
         if (a->dim <= 64) launch_attend<f16, 64>(a, S, W, st);
         else launch_attend<f16, 128>(a, S, W, st);
@@ -429,6 +451,7 @@ extern "C" int artread_attend(int device, const artread_attend_t* a, void* works
 // How a gradient call runs: up to 32 rows of a key head (64 at 64 columns) in one walk over the keys, more in a walk
 // over the keys for dQ and one over the rows for dK and dV; each split where its workgroups would not fill the chip.
 struct GradShape {
+    artread_attend_t args;   // as the kernels take them
     bool fused;
     bool narrow;           // dQ: one wave of 32 rows per workgroup, else four
     AttendPlan q, kv;
@@ -436,9 +459,11 @@ struct GradShape {
     int64_t stats, part;   // byte offsets; the two walks run one after the other and share their parts
     int64_t total;
 };
-static GradShape grad_shape(const artread_attend_t* a) {
+static GradShape grad_shape(const artread_attend_t* given) {
     GradShape S;
     AttendPlan& Q = S.q;
+    S.args = pack_passages(given, &Q);
+    const artread_attend_t* a = &S.args;
     plan_share(&Q, a);
     Q.row_count = a->rows * Q.share;
     plan_scale(&Q, a->scale, a->dtype);
@@ -502,14 +527,20 @@ static void launch_attend_grad(const artread_attend_t* a, const artread_attend_g
     hipLaunchKernelGGL((attend_delta_kernel<T>), dim3(grid_of((rows + 15) / 16)), dim3(256), 0, st, *a, *g, S.q, rows, stats);
     if (S.fused) {
         const dim3 grid = grid2(S.q.items * S.q.splits);
+        constexpr int NW = DP == 64 ? 4 : 2;
+#define GRADS(RB, PACK) \
+    hipLaunchKernelGGL((attend_grad_stream_kernel<T, DP, RB, NW, PACK>), grid, dim3(64 * NW), 0, st, *a, *g, S.q, stats, part)
         if constexpr (DP == 64) {
-            if (S.q.row_count <= 32)
-                hipLaunchKernelGGL((attend_grad_stream_kernel<T, 64, 1, 4>), grid, dim3(256), 0, st, *a, *g, S.q, stats, part);
-            else
-                hipLaunchKernelGGL((attend_grad_stream_kernel<T, 64, 2, 4>), grid, dim3(256), 0, st, *a, *g, S.q, stats, part);
-        } else {
-            hipLaunchKernelGGL((attend_grad_stream_kernel<T, 128, 1, 2>), grid, dim3(128), 0, st, *a, *g, S.q, stats, part);
+            if (S.q.row_count > 32) {
+                if (S.q.pack) GRADS(2, true);
+                else GRADS(2, false);
+            }
         }
+        if (S.q.row_count <= 32) {
+            if (S.q.pack) GRADS(1, true);
+            else GRADS(1, false);
+        }
+#undef GRADS
         if (S.q.splits > 1) launch_sum<T>(part, S.all_q, S.q.splits, g->grad_q, S.all_q, st);
         return;
     }
@@ -546,6 +577,7 @@ extern "C" int artread_attend_grad(int device, const artread_attend_t* a, const 
     ReadDeviceGuard g(device);
     READ_HIP(g.err);
     hipStream_t st = (hipStream_t)stream;
+    a = &S.args;
     if (a->dtype == ARTREAD_F16) {
         if (a->dim <= 64) launch_attend_grad<f16, 64>(a, gr, S, workspace, st);
         else launch_attend_grad<f16, 128>(a, gr, S, workspace, st);

@@ -10,6 +10,8 @@
 // over the keys in C's order; V^T as the A operand follows that order through the transposing LDS read
 // (ds_read_b64_tr_b16: four rows of the tile as four consecutive k).  So no weight ever crosses lanes.
 #pragma once
+#include <type_traits>
+
 #include "artread_common.h"
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -47,6 +49,8 @@ struct AttendPlan {
     int64_t pad_rows;     // row_count in whole tiles of 64: the gradient's row statistics
     int64_t row_blocks;   // blocks of rows per (batch entry, key head)
     int64_t items;        // batch x kv_heads x row_blocks
+    uint32_t pack, inv_pack;     // entries of a passage where short passages are packed, 0 where not; floor(2^32 / pack)
+    int64_t pack_passages;       // passages of a batch entry there; the problem then has one, pack_passages x pack long
     uint32_t share, inv_share;   // heads per key head; floor(2^32 / share), 2^32 - 1 for 1
     int walkers;          // waves of a workgroup that walk one item
     int splits;           // parts the keys of an item are dealt to
@@ -70,31 +74,71 @@ __device__ __forceinline__ void split_row(const AttendPlan& P, int64_t kh, uint3
     *h = kh * P.share + g;
 }
 
+// Valid entries of a packed batch entry from entry f0 on, one per lane: the lane's passage's length is asked for here
+// and compared when it is needed.
+struct Packed {
+    const int32_t* lengths;   // of the batch entry
+    uint32_t pack, inv_pack;
+    int total;                // entries
+    int entry, length;        // the lane's, in its passage; the passage's length
+    __device__ __forceinline__ void start(const artread_attend_t& A, const AttendPlan& P, int64_t b) {
+        lengths = A.lengths + b * P.pack_passages;
+        pack = P.pack;
+        inv_pack = P.inv_pack;
+        total = (int)A.len;
+    }
+    __device__ __forceinline__ void ask(int f) {
+        entry = length = 0;
+        if (f < total) {
+            uint32_t p = __umulhi((uint32_t)f, inv_pack), j = (uint32_t)f - p * pack;
+            if (j >= pack) {   // the quotient is at most one too small
+                p += 1;
+                j -= pack;
+            }
+            entry = (int)j;
+            length = lengths[p];
+        }
+    }
+    __device__ __forceinline__ bool valid() const { return entry < length; }
+};
+
 // Deals the tiles of KT keys of a batch entry's passages to `splits` walkers, one after the other; a passage's
 // last tile may be short, the next passage starts a new tile.  Lengths are held 64 passages at a time, one per
-// lane.  All of it is uniform over the wave.
+// lane.  Passages too short to fill tiles of their own are packed: the batch entry is one long passage with holes.
+// Either way `mask` says which of a tile's keys are valid.  All of it is uniform over the wave.
 template <int KT>
 struct Walk {
     const int32_t* lengths;
+    Packed packed;
+    uint64_t mask;
     int passages, len, p, n, j0, step;
     int held;
+    bool is_packed;
     __device__ __forceinline__ void hold() {
         const int i = p + (int)(threadIdx.x & 63);
         int x = len;
         if (lengths) x = i < passages ? lengths[i] : 0;
         held = x < 0 ? 0 : (x < len ? x : len);
     }
-    __device__ __forceinline__ void start(const artread_attend_t& A, int64_t b, int split, int splits) {
-        lengths = A.lengths ? A.lengths + b * A.passages : nullptr;
+    __device__ __forceinline__ void start(const artread_attend_t& A, const AttendPlan& P, int64_t b, int split, int splits) {
+        is_packed = P.pack != 0;
         passages = (int)A.passages;
         len = (int)A.len;
         p = 0;
-        hold();
-        n = uniform(held);
         j0 = split * KT;
         step = splits * KT;
+        if (is_packed) {
+            lengths = nullptr;
+            n = len;
+            packed.start(A, P, b);
+            packed.ask(j0 + (int)(threadIdx.x & 63));
+        } else {
+            lengths = A.lengths ? A.lengths + b * A.passages : nullptr;
+            hold();
+            n = uniform(held);
+        }
     }
-    // false: no tile left; else passage p, first key j0, n keys in the passage
+    // false: no tile left; else passage p, first key j0, and mask
     __device__ __forceinline__ bool settle() {
         while (j0 >= n) {
             j0 -= (n + KT - 1) / KT * KT;
@@ -102,10 +146,18 @@ struct Walk {
             if ((p & 63) == 0) hold();
             n = __builtin_amdgcn_readlane(held, p & 63);
         }
+        const int left = n - j0;
+        mask = left >= 64 ? ~0ull : (1ull << left) - 1;
+        if (is_packed) mask = __ballot(packed.valid());
         return true;
     }
-    __device__ __forceinline__ void advance() { j0 += step; }
+    __device__ __forceinline__ void advance() {
+        j0 += step;
+        if (is_packed) packed.ask(j0 + (int)(threadIdx.x & 63));   // in time for the tile after this one
+    }
 };
+template <int KB>
+__device__ __forceinline__ bool whole_tile(uint64_t mask) { return KB == 1 ? (uint32_t)mask == ~0u : mask == ~0ull; }
 
 // 16-byte pieces of rows: zero behind `dim` and for rows that are not there
 template <typename T>
@@ -206,16 +258,16 @@ __device__ __forceinline__ float both_sum(float x) {
 // scores of NB x 32 keys of one row per lane pair -> weights; m, l are the running maximum (of scores x c) and the
 // lane's own part of the sum, `o` the accumulators that a new maximum rescales
 template <typename T, int NB, int NO>
-__device__ __forceinline__ void softmax_tile(f32x16 (&s)[NB], float c, int left, int half, float& m, float& l,
+__device__ __forceinline__ void softmax_tile(f32x16 (&s)[NB], float c, uint64_t mask, int half, float& m, float& l,
                                              f32x16 (&o)[NO]) {
-    if (left < NB * 32) {
-        const int mine = left - 4 * half;   // keys of this lane's rows of C
-        asm volatile("");                   // a branch: most tiles are whole
+    if (!whole_tile<NB>(mask)) {
+        const uint64_t mine = mask >> (4 * half);   // keys of this lane's rows of C
+        asm volatile("");                           // a branch: most tiles are whole
 #pragma unroll
         for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
             for (int i = 0; i < 16; ++i)
-                if (32 * kb + 8 * (i >> 2) + (i & 3) >= mine) s[kb][i] = -INFINITY;
+                if (!((uint32_t)(mine >> (32 * kb)) & (1u << (8 * (i >> 2) + (i & 3))))) s[kb][i] = -INFINITY;
     }
     float top = s[0][0];
 #pragma unroll
@@ -433,20 +485,20 @@ __global__ __launch_bounds__(256, 2) void attend_stream_kernel(artread_attend_t 
     const T* vbase = (const T*)A.v + b * A.v_batch + kh * A.v_head + (int64_t)vrow * A.v_row + 8 * vchunk;
     V8 kr[DP / 16], vr[VN];
     Walk<32> walk;
-    walk.start(A, b, split, P.splits * P.walkers);
+    walk.start(A, P, b, split, P.splits * P.walkers);
     auto load = [&]() {
-        const int left = walk.n - walk.j0;
+        const uint32_t valid = (uint32_t)walk.mask;
         const T* kp = kbase + walk.p * A.k_passage + walk.j0 * A.k_row;
         const T* vp = vbase + walk.p * A.v_passage + walk.j0 * A.v_row;
 #pragma unroll
-        for (int s = 0; s < DP / 16; ++s) kr[s] = load8<T>(kp + 16 * s, (lane & 31) < left && 16 * s + 8 * half < dim);
+        for (int s = 0; s < DP / 16; ++s) kr[s] = load8<T>(kp + 16 * s, (valid >> (lane & 31) & 1) && 16 * s + 8 * half < dim);
 #pragma unroll
-        for (int x = 0; x < VN; ++x) vr[x] = load8<T>(vp + (int64_t)x * VR * A.v_row, vrow + x * VR < left && 8 * vchunk < dim);
+        for (int x = 0; x < VN; ++x) vr[x] = load8<T>(vp + (int64_t)x * VR * A.v_row, (valid >> (vrow + x * VR) & 1) && 8 * vchunk < dim);
     };
     bool more = walk.settle();
     if (more) load();
     while (more) {
-        const int left = walk.n - walk.j0;
+        const uint64_t mask = walk.mask;
         f32x16 s[QB][1];
 #pragma unroll
         for (int x = 0; x < QB; ++x) s[x][0] = f32x16{};
@@ -463,7 +515,7 @@ __global__ __launch_bounds__(256, 2) void attend_stream_kernel(artread_attend_t 
         more = walk.settle();
         if (more) load();
 #pragma unroll
-        for (int x = 0; x < QB; ++x) softmax_tile<T, 1, DP / 32>(s[x], P.c, left, half, m[x], l[x], o[x]);
+        for (int x = 0; x < QB; ++x) softmax_tile<T, 1, DP / 32>(s[x], P.c, mask, half, m[x], l[x], o[x]);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // the tile is written: LDS keeps a wave's order
         const uint32_t vcol = opaque(lds_offset(tile) + columns_base<DP>(lane));
 #pragma unroll
@@ -526,16 +578,17 @@ __device__ __forceinline__ int64_t xcd_item(int64_t id, int64_t items) {
     return (id >> 3) < per ? (id & 7) * per + (id >> 3) : items;
 }
 
-// Brings tiles of KB x 32 states into a ring of LDS: 1 KiB pieces, PW of a tile for each of NW waves.  States behind
-// the passage's length and columns behind dim become zeros: a short tile's are written, the columns' are cleared once.
+// Brings tiles of KB x 32 states into a ring of LDS: 1 KiB pieces, PW of a tile for each of NW waves.  States that are
+// not valid and columns behind dim become zeros: the states are written, the columns cleared once.
 template <typename T, int DP, int KB, int NW>
 struct TileFetch {
     static constexpr int CH = DP / 8, PR = 64 / CH, PW = 32 * KB / PR / NW;   // chunks per row, rows per piece
     int wave;
     __device__ __forceinline__ void start(int w) { wave = w; }
-    // src: state 0 of the tile; left: states from there to the passage's end; stride below 2^24
-    __device__ __forceinline__ void fetch(const T* src, int64_t stride, int left, int dim, uint32_t tile) const {
-        const bool full = left >= 32 * KB;   // uniform
+    // src: state 0 of the tile; mask: which of its states are valid; stride below 2^24
+    typedef typename std::conditional<KB == 1, uint32_t, uint64_t>::type Mask;
+    __device__ __forceinline__ void fetch(const T* src, int64_t stride, Mask mask, int dim, uint32_t tile) const {
+        const bool full = whole_tile<KB>(mask);   // uniform
         // from the lane's number anew each time: the offsets of all pieces would not fit beside the accumulators
         const int lane = (int)opaque(threadIdx.x & 63), row = lane / CH, col = lane % CH;
         const uint32_t bytes = (uint32_t)row * (uint32_t)stride * 2;
@@ -546,7 +599,7 @@ struct TileFetch {
             const T* base = src + (int64_t)(piece * PR) * stride;
             if (full) {
                 if (c < dim) dma16(base, bytes + c * 2, dst);
-            } else if (c < dim && r < left) {
+            } else if (c < dim && (mask >> r & 1)) {
                 dma16(base, bytes + c * 2, dst);
             } else {
                 *(__attribute__((address_space(3))) u32x4*)(uintptr_t)(dst + lane * 16) = u32x4{0, 0, 0, 0};
@@ -578,17 +631,18 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(artread_attend_t A,
     const int64_t r = (rb * 4 + wave) * 32 + (lane & 31);
     const T* kbase = (const T*)A.k + b * A.k_batch + kh * A.k_head;
     const T* vbase = (const T*)A.v + b * A.v_batch + kh * A.v_head;
-    Walk<32 * KB> walk;   // of the tiles fetched; `left` of the one worked on
-    walk.start(A, b, split, P.splits);
-    auto fetch = [&](int stage) {   // keys of the tile, 0 behind the last
-        if (!walk.settle()) return 0;
-        const int left = walk.n - walk.j0;
-        fetcher.fetch(kbase + walk.p * A.k_passage + walk.j0 * A.k_row, A.k_row, left, dim, lds_offset(ring[stage]));
-        fetcher.fetch(vbase + walk.p * A.v_passage + walk.j0 * A.v_row, A.v_row, left, dim, lds_offset(ring[2 + stage]));
+    Walk<32 * KB> walk;   // of the tiles fetched
+    walk.start(A, P, b, split, P.splits);
+    uint64_t mask = 0, next_mask = 0;   // of the tile worked on, and of the one being fetched
+    auto fetch = [&](int stage) {
+        if (!walk.settle()) return false;
+        next_mask = walk.mask;
+        fetcher.fetch(kbase + walk.p * A.k_passage + walk.j0 * A.k_row, A.k_row, next_mask, dim, lds_offset(ring[stage]));
+        fetcher.fetch(vbase + walk.p * A.v_passage + walk.j0 * A.v_row, A.v_row, next_mask, dim, lds_offset(ring[2 + stage]));
         walk.advance();
-        return left;
+        return true;
     };
-    int left = fetch(0);
+    bool more = fetch(0);
     V8 q[DP / 16];
     f32x16 o[DP / 32];
     float m = -INFINITY, l = 0.0f;
@@ -596,10 +650,11 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(artread_attend_t A,
 #pragma unroll
     for (int db = 0; db < DP / 32; ++db) o[db] = f32x16{};
     int stage = 0;
-    while (left) {
+    while (more) {
+        mask = next_mask;
         dma_wait<0>();
         wave_meet();   // everyone's pieces are there, and everyone is done with the tile before
-        const int next = fetch(stage ^ 1);
+        more = fetch(stage ^ 1);
         const uint32_t krow = opaque(lds_offset(ring[stage]) + rows_base<DP>(lane));
         const uint32_t vcol = opaque(lds_offset(ring[2 + stage]) + columns_base<DP>(lane));
         f32x16 s[KB];
@@ -625,7 +680,7 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(artread_attend_t A,
             __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
             __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
         }
-        softmax_tile<T, KB, DP / 32>(s, P.c, left, half, m, l, o);
+        softmax_tile<T, KB, DP / 32>(s, P.c, mask, half, m, l, o);
 #pragma unroll
         for (int i = EARLY; i < NV; ++i) vt[i] = lds_columns<T, DP>(vcol, 16 * (i / (DP / 32)), i % (DP / 32));
 #pragma unroll
@@ -634,7 +689,6 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(artread_attend_t A,
 #pragma unroll
             for (int db = 0; db < DP / 32; ++db) o[db] = Mma<T>::mul(vt[ks * (DP / 32) + db], pw, o[db]);
         }
-        left = next;
         stage ^= 1;
     }
     finish_rows<T, DP>(A, P, W, b, kh, r, split, half, m, both_sum(l), o);

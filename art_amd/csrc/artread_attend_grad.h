@@ -7,8 +7,6 @@
 // and dV and goes over the rows, those of the heads that share a key head among them.  In both a lane owns one
 // column of S (a row, or a key), so P and dS are already the B operands of the second products.
 #pragma once
-#include <type_traits>
-
 #include "artread_attend.h"
 
 // log-sum and delta of every row in the order (batch entry, key head, r), the log-sum in powers of two and with the
@@ -206,17 +204,18 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_grad_q_kernel(artread_atten
     const int64_t r = (rb * NW + wave) * 32 + (lane & 31);
     const T* kbase = (const T*)A.k + b * A.k_batch + kh * A.k_head;
     const T* vbase = (const T*)A.v + b * A.v_batch + kh * A.v_head;
-    Walk<32 * KB> walk;   // of the tiles fetched; `left` of the one worked on
-    walk.start(A, b, split, P.splits);
-    auto fetch = [&](int stage) {   // keys of the tile, 0 behind the last
-        if (!walk.settle()) return 0;
-        const int left = walk.n - walk.j0;
-        fetcher.fetch(kbase + walk.p * A.k_passage + walk.j0 * A.k_row, A.k_row, left, dim, lds_offset(ring[stage]));
-        fetcher.fetch(vbase + walk.p * A.v_passage + walk.j0 * A.v_row, A.v_row, left, dim, lds_offset(ring[2 + stage]));
+    Walk<32 * KB> walk;   // of the tiles fetched
+    walk.start(A, P, b, split, P.splits);
+    uint64_t mask = 0, next_mask = 0;   // of the tile worked on, and of the one being fetched
+    auto fetch = [&](int stage) {
+        if (!walk.settle()) return false;
+        next_mask = walk.mask;
+        fetcher.fetch(kbase + walk.p * A.k_passage + walk.j0 * A.k_row, A.k_row, next_mask, dim, lds_offset(ring[stage]));
+        fetcher.fetch(vbase + walk.p * A.v_passage + walk.j0 * A.v_row, A.v_row, next_mask, dim, lds_offset(ring[2 + stage]));
         walk.advance();
-        return left;
+        return true;
     };
-    int left = fetch(0);
+    bool more = fetch(0);
     V8 q[DP / 16], g[DP / 16];
     load_q<T, DP>(A, P, (const T*)A.q, A.q_batch, A.q_row, A.q_head, b, kh, r, half, P.q_and, P.q_xor, q);
     load_q<T, DP>(A, P, (const T*)G.grad_out, G.g_batch, G.g_row, G.g_head, b, kh, r, half, 0xffffffffu, 0u, g);
@@ -227,10 +226,11 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_grad_q_kernel(artread_atten
 #pragma unroll
     for (int db = 0; db < DP / 32; ++db) acc[db] = f32x16{};
     int stage = 0;
-    while (left) {
+    while (more) {
+        mask = next_mask;
         dma_wait<0>();
         wave_meet();   // everyone's pieces are there, and everyone is done with the tile before
-        const int next = fetch(stage ^ 1);
+        more = fetch(stage ^ 1);
         const uint32_t krow = opaque(lds_offset(ring[stage]) + rows_base<DP>(lane));
         const uint32_t kcol = opaque(lds_offset(ring[stage]) + columns_base<DP>(lane));
 #pragma unroll
@@ -243,12 +243,12 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_grad_q_kernel(artread_atten
             }
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], P.c, -st.x)) * (dp[i] - st.delta);
-            if (left < 32 * KB) {
-                const int mine = left - 4 * half;
+            if (!whole_tile<KB>(mask)) {
+                const uint32_t mine = (uint32_t)(mask >> (32 * kb + 4 * half));
                 asm volatile("");   // a branch: most tiles are whole
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    if (32 * kb + 8 * (i >> 2) + (i & 3) >= mine) s[i] = 0.0f;
+                    if (!(mine & (1u << (8 * (i >> 2) + (i & 3))))) s[i] = 0.0f;
             }
             spread.fit(s, acc);
 #pragma unroll
@@ -259,7 +259,6 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_grad_q_kernel(artread_atten
                     acc[db] = Mma<T>::mul(lds_columns<T, DP>(kcol, 32 * kb + 16 * ks, db), ds, acc[db]);
             }
         }
-        left = next;
         stage ^= 1;
     }
     if (r < P.row_count) {
@@ -317,12 +316,19 @@ __global__ __launch_bounds__(256, 2) void attend_grad_kv_kernel(artread_attend_t
         item /= A.kv_heads;
     }
     const int64_t b = item;
+    const int64_t j = j0 + 32 * wave + (lane & 31);
     int n = (int)A.len;
-    if (A.lengths) {
+    bool key = j < n;   // this lane's
+    if (P.pack) {
+        Packed packed;
+        packed.start(A, P, b);
+        packed.ask((int)j);
+        key = packed.valid();
+    } else if (A.lengths) {
         const int x = uniform(A.lengths[b * A.passages + p]);
         n = x < n ? x : n;
+        key = j < n;
     }
-    const int64_t j = j0 + 32 * wave + (lane & 31);
     f32x16 dk[DP / 32], dv[DP / 32];
     Spread<T> spread;
 #pragma unroll
@@ -333,7 +339,7 @@ __global__ __launch_bounds__(256, 2) void attend_grad_kv_kernel(artread_attend_t
         const T* vp = (const T*)A.v + b * A.v_batch + p * A.v_passage + j * A.v_row + kh * A.v_head + 8 * half;
 #pragma unroll
         for (int s = 0; s < DP / 16; ++s) {
-            const bool ok = j < n && 16 * s + 8 * half < dim;
+            const bool ok = key && 16 * s + 8 * half < dim;
             kf[s] = load8<T>(kp + 16 * s, ok);
             vf[s] = load8<T>(vp + 16 * s, ok);
         }
@@ -412,7 +418,7 @@ __global__ __launch_bounds__(256, 2) void attend_grad_kv_kernel(artread_attend_t
                 stage ^= 1;
             }
         };
-        if (j0 + 32 * wave < n) go(std::true_type{});   // uniform over the wave
+        if (__any(key)) go(std::true_type{});   // uniform over the wave
         else go(std::false_type{});
     }
     const int64_t all = A.batch * A.passages * A.len * A.kv_heads * dim;
@@ -423,9 +429,9 @@ __global__ __launch_bounds__(256, 2) void attend_grad_kv_kernel(artread_attend_t
         const int64_t j1 = j0 + 32 * wave, at = (((b * A.passages + p) * A.len + j1) * A.kv_heads + kh) * dim;
         const int rows = A.len - j1 < 32 ? (int)(A.len - j1) : 32;
         u32x4 w[DP / 16];
-        turn_keys<T, DP>(dv, fv, j < n, own, lane, w);
+        turn_keys<T, DP>(dv, fv, key, own, lane, w);
         store_turned<T, DP>((T*)G.grad_v + at, A.kv_heads * dim, rows, dim, lane, w);
-        turn_keys<T, DP>(dk, fk, j < n, own, lane, w);
+        turn_keys<T, DP>(dk, fk, key, own, lane, w);
         store_turned<T, DP>((T*)G.grad_k + at, A.kv_heads * dim, rows, dim, lane, w);
         return;
     }
@@ -440,8 +446,8 @@ __global__ __launch_bounds__(256, 2) void attend_grad_kv_kernel(artread_attend_t
             float yk[4], yv[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {   // behind the length: zeros, whatever the accumulators hold
-                yk[e] = j < n ? fk * dk[db][4 * x + e] : 0.0f;
-                yv[e] = j < n ? fv * dv[db][4 * x + e] : 0.0f;
+                yk[e] = key ? fk * dk[db][4 * x + e] : 0.0f;
+                yv[e] = key ? fv * dv[db][4 * x + e] : 0.0f;
             }
             *(float4*)(part + split * 2 * all + at + d) = make_float4(yk[0], yk[1], yk[2], yk[3]);
             *(float4*)(part + (split * 2 + 1) * all + at + d) = make_float4(yv[0], yv[1], yv[2], yv[3]);
@@ -454,8 +460,9 @@ __global__ __launch_bounds__(256, 2) void attend_grad_kv_kernel(artread_attend_t
 // once, which is what bounds this, where the two walks would read the states twice.  S^T and dP^T leave P^T and dS^T
 // as B operands over the keys, for dQ; dV and dK want them over the rows, so both go through a 32 x 32 tile of LDS and
 // come back by the transposing read.  A tile's results are stored once the next tile has arrived: waiting for that
-// tile then never waits for the stores.  The waves of a workgroup add their dQ in LDS, in order.
-template <typename T, int DP, int RB, int NW>
+// tile then never waits for the stores.  The waves of a workgroup add their dQ in LDS, in order.  PACK: passages too
+// short to fill tiles of their own are packed; a kernel of its own, for the registers.
+template <typename T, int DP, int RB, int NW, bool PACK>
 __global__ __launch_bounds__(64 * NW, 2) void attend_grad_stream_kernel(artread_attend_t A, artread_attend_grads_t G,
                                                                         AttendPlan P, const RowStat* __restrict__ stats,
                                                                         float* __restrict__ part) {
@@ -504,20 +511,31 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_grad_stream_kernel(artread_
     const T* kbase = (const T*)A.k + b * A.k_batch + kh * A.k_head;
     const T* vbase = (const T*)A.v + b * A.v_batch + kh * A.v_head;
     const int step = P.splits * NW, step_p = step / per_passage, step_j = step % per_passage;
-    int p = (group * NW + wave) / per_passage, jt = (group * NW + wave) % per_passage, left = 0;
+    int p = (group * NW + wave) / per_passage, jt = (group * NW + wave) % per_passage;
+    uint32_t mask = 0;   // valid keys of the tile at p, jt; 0: nothing was fetched
     int chunk = -1, lengths = len;   // of 64 passages, one per lane
-    auto fetch = [&]() {   // the tile at p, jt: keys in it
-        left = 0;
+    Packed packed;
+    if constexpr (PACK) {
+        packed.start(A, P, b);
+        packed.ask(32 * jt + (lane & 31));
+    }
+    auto fetch = [&]() {
+        mask = 0;
         if (p >= (int)A.passages) return;
-        if (A.lengths && (p >> 6) != chunk) {   // rarely: a load here waits for the stores before it
-            chunk = p >> 6;
-            const int i = chunk * 64 + lane;
-            lengths = i < (int)A.passages ? A.lengths[b * A.passages + i] : 0;
+        if constexpr (PACK) {
+            mask = (uint32_t)__ballot(packed.valid());
+        } else {
+            if (A.lengths && (p >> 6) != chunk) {   // rarely: a load here waits for the stores before it
+                chunk = p >> 6;
+                const int i = chunk * 64 + lane;
+                lengths = i < (int)A.passages ? A.lengths[b * A.passages + i] : 0;
+            }
+            const int left = min(len, __builtin_amdgcn_readlane(lengths, p & 63)) - 32 * jt;
+            mask = left <= 0 ? 0u : (left >= 32 ? ~0u : (1u << left) - 1);
         }
-        left = min(len, __builtin_amdgcn_readlane(lengths, p & 63)) - 32 * jt;
-        if (left <= 0) return;
-        fetcher.fetch(kbase + p * A.k_passage + (int64_t)32 * jt * A.k_row, A.k_row, left, dim, mine);
-        fetcher.fetch(vbase + p * A.v_passage + (int64_t)32 * jt * A.v_row, A.v_row, left, dim, mine + TILE * 2);
+        if (!mask) return;
+        fetcher.fetch(kbase + p * A.k_passage + (int64_t)32 * jt * A.k_row, A.k_row, mask, dim, mine);
+        fetcher.fetch(vbase + p * A.v_passage + (int64_t)32 * jt * A.v_row, A.v_row, mask, dim, mine + TILE * 2);
     };
     f32x16 dk[DP / 32], dv[DP / 32];
     u32x4 wk[DP / 16], wv[DP / 16];   // the tile before's, rounded, and where it was
@@ -559,15 +577,16 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_grad_stream_kernel(artread_
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // and read
     };
     fetch();
+    if constexpr (PACK) packed.ask(32 * (jt + step_j) + (lane & 31));
     __syncthreads();   // Q and dO are there
     while (true) {
-        if (left > 0) dma_wait<0>();
+        if (mask) dma_wait<0>();
         store();
         if (p >= (int)A.passages) break;
         held_p = p;
         held_j = 32 * jt;
-        const int now = left;
-        if (now > 0) {
+        const uint32_t now = mask;
+        if (now) {
             const uint32_t krow = opaque(mine + rows_base<DP>(lane));
             const uint32_t qrow = opaque(lds_offset(qtile) + rows_base<DP>(lane));
 #pragma unroll
@@ -598,12 +617,11 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_grad_stream_kernel(artread_
                     s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], P.c, -st[x].x));
                     dp[i] = s[i] * (dp[i] - st[x].delta);
                 }
-                if (now < 32) {
-                    const int keys = now - 4 * half;
-                    asm volatile("");   // a branch: most tiles are whole
+                if (now != ~0u) {
+                    const uint32_t keys = opaque(now >> (4 * half));
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
-                        if (8 * (i >> 2) + (i & 3) >= keys) dp[i] = 0.0f;
+                        if (!(keys & (1u << (8 * (i >> 2) + (i & 3))))) dp[i] = 0.0f;
                 }
                 // P and dS to LDS as [row][key], 8-byte pieces permuted by the row
                 const uint32_t pw = opaque(pd + (uint32_t)((lane & 31) * 64 + ((half ^ ((lane >> 2) & 7)) * 8)));
@@ -632,9 +650,10 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_grad_stream_kernel(artread_
             ++p;
         }
         fetch();
-        if (now > 0) add_block(RB - 1);
+        if constexpr (PACK) packed.ask(32 * (jt + step_j) + (lane & 31));   // one passage: the tile after, or none
+        if (now) add_block(RB - 1);
         const float fk = A.scale * spread_k.inverse() * P.unweight;
-        const bool key = (lane & 31) < now;
+        const bool key = now >> (lane & 31) & 1;
         turn_keys<T, DP>(dv, P.unweight, key, pd, lane, wv);
         turn_keys<T, DP>(dk, fk, key, pd, lane, wk);
     }

@@ -244,8 +244,8 @@ def _plan(query, key, value, lengths, scale):
         raise ValueError("%d query heads cannot share %d key heads" % (heads, kv_heads))
     if lengths is not None and (lengths.dtype != torch.int32 or lengths.shape != k_shape[:-3]):
         raise ValueError("lengths must be an int32 tensor %s, one per passage" % (tuple(k_shape[:-3]),))
-    if max(batch * rows * heads, batch * passages * length * kv_heads) >= 1 << 31:
-        raise ValueError("query and key hold at most 2**31 - 1 rows each")
+    if max(batch * rows * heads, batch * passages * length * kv_heads) >= 1 << 31 or passages * length > (1 << 31) - (1 << 20):
+        raise ValueError("query and key hold at most 2**31 - 1 rows each, a batch entry at most 2**31 - 2**20 states")
     return (batch, rows, passages, length, heads, kv_heads, dim), _scale_value(dim ** -0.5 if scale is None else scale)
 
 

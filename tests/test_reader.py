@@ -197,7 +197,7 @@ def _attend(**change):
 BAD_ATTEND = [
     dict(dtype=2), dict(batch=0), dict(rows=0), dict(passages=0), dict(len=0), dict(heads=0), dict(kv_heads=0),
     dict(kv_heads=3), dict(dim=0), dict(dim=12), dict(dim=136), dict(rows=1 << 31), dict(batch=1 << 20, rows=1 << 20),
-    dict(passages=1 << 20, len=1 << 20), dict(scale=float("nan")), dict(q_row=-8), dict(k_row=12),
+    dict(passages=1 << 20, len=1 << 20), dict(batch=1, passages=1, len=(1 << 31) - 1, kv_heads=1, heads=1), dict(scale=float("nan")), dict(q_row=-8), dict(k_row=12),
     dict(v_batch=1 << 40), dict(k_row=1 << 24), dict(v_row=1 << 24), dict(q_row=1 << 24), dict(q_head=1 << 28),
 ]
 

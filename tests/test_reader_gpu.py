@@ -304,7 +304,8 @@ SHAPES = [
     (2, 31, 1, 64, 3, 3, 64), (2, 32, 4, 33, 4, 1, 128), (1, 33, 5, 63, 6, 2, 80), (2, 64, 2, 129, 2, 2, 40),
     (1, 65, 3, 100, 2, 1, 128), (1, 127, 1, 1, 3, 3, 64), (1, 130, 2, 300, 2, 2, 96), (1, 257, 3, 77, 4, 2, 128),
     (5, 16, 1, 16, 16, 2, 64), (2, 3, 40, 3, 5, 5, 72), (1, 17, 1, 700, 1, 1, 120), (4, 1, 32, 200, 4, 4, 64),
-    (9, 4, 2, 20, 24, 3, 16), (1, 300, 1, 513, 2, 2, 64),
+    (9, 4, 2, 20, 24, 3, 16), (1, 300, 1, 513, 2, 2, 64), (3, 40, 100, 7, 4, 2, 64), (2, 200, 70, 1, 3, 3, 128),
+    (1, 70, 33, 32, 2, 1, 40), (2, 5, 300, 31, 2, 2, 128), (4, 100, 9, 13, 2, 2, 64),
 ]
 
 
