@@ -120,6 +120,20 @@ struct SpreadAll<f16> {
     }
 };
 
+// dS as two terms, the rounded value and what the rounding took, for products that share the other operand's LDS read.
+// With one term the error of dQ is up to 1.5 times that of its own rounding, where a row's sum hangs on few keys; with
+// two it is that rounding (train_top100: 2.08e-4 instead of 3.1e-4 of f16 dQ, row walk of train_long 480 us instead of
+// 407).  The key walk takes one: its sums run over more than 32 rows, 1.4 times, and the registers of a second term
+// would spill V.  P takes one everywhere.
+template <typename T>
+__device__ __forceinline__ void terms8(const f32x16& s, int ks, typename Mma<T>::V8& hi, typename Mma<T>::V8& lo) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        hi[e] = (T)s[8 * ks + e];
+        lo[e] = (T)(s[8 * ks + e] - (float)hi[e]);
+    }
+}
+
 template <typename T>
 __device__ __forceinline__ void put4(T* p, const float* x) {
     Vec<T, 4> w;
@@ -253,10 +267,14 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_grad_q_kernel(artread_atten
             spread.fit(s, acc);
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks) {
-                const V8 ds = weights8<T>(s, ks);
+                V8 hi, lo;
+                terms8<T>(s, ks, hi, lo);
 #pragma unroll
-                for (int db = 0; db < DP / 32; ++db)
-                    acc[db] = Mma<T>::mul(lds_columns<T, DP>(kcol, 32 * kb + 16 * ks, db), ds, acc[db]);
+                for (int db = 0; db < DP / 32; ++db) {
+                    const V8 a = lds_columns<T, DP>(kcol, 32 * kb + 16 * ks, db);
+                    acc[db] = Mma<T>::mul(a, hi, acc[db]);
+                    acc[db] = Mma<T>::mul(a, lo, acc[db]);
+                }
             }
         }
         stage ^= 1;
@@ -467,7 +485,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_grad_stream_kernel(artread_
                                                                         AttendPlan P, const RowStat* __restrict__ stats,
                                                                         float* __restrict__ part) {
     constexpr int TILE = 32 * DP, CH = DP / 8;
-    constexpr int SHARED = 2 * RB * TILE, OWN = 2 * TILE + 2 * 1024;   // elements: Q and dO; K, V, P and dS of a wave
+    constexpr int SHARED = 2 * RB * TILE, OWN = 2 * TILE + 3 * 1024;   // elements: Q and dO; K, V, P and both terms of dS of a wave
     constexpr int BYTES = (SHARED + NW * OWN) * 2, SUMS = NW * 32 * RB * DP * 4;
     __shared__ __attribute__((aligned(1024))) char lds[BYTES > SUMS ? BYTES : SUMS];
     typedef typename Mma<T>::V8 V8;
@@ -554,9 +572,9 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_grad_stream_kernel(artread_
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // they are written: LDS keeps a wave's order
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
-            V8 pk[2];
+            V8 pk[3];
 #pragma unroll
-            for (int a = 0; a < 2; ++a) {
+            for (int a = 0; a < 3; ++a) {
                 union {
                     s16x4 h[2];
                     V8 v;
@@ -570,7 +588,9 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_grad_stream_kernel(artread_
 #pragma unroll
             for (int db = 0; db < DP / 32; ++db) {
                 dv[db] = Mma<T>::mul(lds_columns<T, DP>(qcol, 32 * (RB + x) + 16 * ks, db), pk[0], dv[db]);
-                dk[db] = Mma<T>::mul(lds_columns<T, DP>(qcol, 32 * x + 16 * ks, db), pk[1], dk[db]);
+                const V8 a = lds_columns<T, DP>(qcol, 32 * x + 16 * ks, db);
+                dk[db] = Mma<T>::mul(a, pk[1], dk[db]);
+                dk[db] = Mma<T>::mul(a, pk[2], dk[db]);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
@@ -629,15 +649,27 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_grad_stream_kernel(artread_
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     *(lds_u32x2*)(uintptr_t)(pw ^ (16 * i)) = pack4<T>(s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]);
-                    *(lds_u32x2*)(uintptr_t)((pw ^ (16 * i)) + 2048) = pack4<T>(spread_k.times(dp[4 * i]), spread_k.times(dp[4 * i + 1]), spread_k.times(dp[4 * i + 2]), spread_k.times(dp[4 * i + 3]));
+                    float y[4], z[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        y[e] = spread_k.times(dp[4 * i + e]);
+                        z[e] = y[e] - (float)(T)y[e];
+                    }
+                    *(lds_u32x2*)(uintptr_t)((pw ^ (16 * i)) + 2048) = pack4<T>(y[0], y[1], y[2], y[3]);
+                    *(lds_u32x2*)(uintptr_t)((pw ^ (16 * i)) + 4096) = pack4<T>(z[0], z[1], z[2], z[3]);
                 }
                 spread_q[x].fit(dp, dq[x]);
                 const uint32_t kcol = opaque(mine + columns_base<DP>(lane));
 #pragma unroll
                 for (int ks = 0; ks < 2; ++ks) {
-                    const V8 ds = weights8<T>(dp, ks);
+                    V8 hi, lo;
+                    terms8<T>(dp, ks, hi, lo);
 #pragma unroll
-                    for (int db = 0; db < DP / 32; ++db) dq[x][db] = Mma<T>::mul(lds_columns<T, DP>(kcol, 16 * ks, db), ds, dq[x][db]);
+                    for (int db = 0; db < DP / 32; ++db) {
+                        const V8 a = lds_columns<T, DP>(kcol, 16 * ks, db);
+                        dq[x][db] = Mma<T>::mul(a, hi, dq[x][db]);
+                        dq[x][db] = Mma<T>::mul(a, lo, dq[x][db]);
+                    }
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
