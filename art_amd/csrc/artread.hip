@@ -39,6 +39,7 @@ struct ReadDeviceGuard {
     explicit ReadDeviceGuard(int d) : dev(d) {
         err = hipGetDevice(&prev);
         if (err == hipSuccess && prev != dev) err = hipSetDevice(dev);
+        if (err != hipSuccess) (void)hipGetLastError();   // reported here, not by the next call
     }
     ~ReadDeviceGuard() {
         if (prev >= 0 && prev != dev) (void)hipSetDevice(prev);
@@ -60,6 +61,7 @@ static int check_tokens(const void* tokens, int token_bytes, const int32_t* leng
                         int64_t vocab, int64_t dim, int64_t vocab_base, Tokens* T) {
     READ_ARG(tokens, "tokens is NULL");
     READ_ARG(token_bytes == 4 || token_bytes == 8, "token_bytes must be 4 or 8 (got %d)", token_bytes);
+    READ_ARG(aligned(tokens, token_bytes) && aligned(lengths, 4), "misaligned tokens or lengths");
     READ_ARG(n >= 1 && len >= 1 && n < kLimit && len < kLimit && n * len < kLimit,
              "n %lld x len %lld must be in [1, 2^31)", (long long)n, (long long)len);
     READ_ARG(vocab >= 1 && vocab < kLimit, "vocab %lld must be in [1, 2^31)", (long long)vocab);
@@ -195,7 +197,8 @@ static void launch_grad_sums(const void* grad, const Pair* sorted, const SortMet
     S.workers = (T.positions + s.run - 1) / s.run;
     S.sum_groups = (S.workers + S.rpp - 1) / S.rpp;
     const int threads = S.cpr < 256 ? (int)round_up((int64_t)S.cpr * S.rpp, 64) : 256;
-    const int64_t clear = (T.vocab + kClearRows - 1) / kClearRows;
+    int64_t clear = (T.vocab + kClearRows - 1) / kClearRows;
+    if (clear > (1 << 20)) clear = 1 << 20;
     hipLaunchKernelGGL((grad_sum_kernel<GT, OT, EPV>), dim3((unsigned)(S.sum_groups + clear)), dim3(threads), 0, st,
                        (const GT*)grad, sorted, meta, T.vocab, scale, (OT*)table, dim, S, partial, chain_end);
     if (S.workers > 1)
@@ -309,6 +312,7 @@ static int check_attend_call(const artread_attend_t* a) {
     if (rc) return rc;
     READ_ARG(a->q && a->k && a->v && a->out, "q, k, v or out is NULL");
     READ_ARG(aligned(a->rest, 16), "rest must be 16-byte aligned");
+    READ_ARG(aligned(a->lse, 4) && aligned(a->lengths, 4), "misaligned lse or lengths");
     READ_ARG(aligned(a->q, 16) && aligned(a->k, 16) && aligned(a->v, 16) && aligned(a->out, 16),
              "q, k, v and out must be 16-byte aligned");
     return 0;

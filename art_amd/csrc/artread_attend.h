@@ -660,15 +660,15 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(artread_attend_t A,
         f32x16 s[KB];
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) s[kb] = f32x16{};
-        constexpr int NK = KB * DP / 16, NV = 2 * KB * DP / 32, EARLY = NV < 8 ? NV : 8, AHEAD = NK < 6 ? NK : 6;
+        constexpr int NK = KB * DP / 16, NV = 2 * KB * DP / 32, AHEAD = NK < 8 ? NK : 8;
 #pragma unroll
         for (int k = 0; k < DP / 16; ++k)
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) s[kb] = Mma<T>::mul(lds_rows<T, DP>(krow, kb, k), q[k], s[kb]);
-        // the first operands of the second product are on their way while the softmax runs
+        // the operands of the second product are on their way while the softmax runs
         V8 vt[NV];
 #pragma unroll
-        for (int i = 0; i < EARLY; ++i) vt[i] = lds_columns<T, DP>(vcol, 16 * (i / (DP / 32)), i % (DP / 32));
+        for (int i = 0; i < NV; ++i) vt[i] = lds_columns<T, DP>(vcol, 16 * (i / (DP / 32)), i % (DP / 32));
         __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);   // LDS reads ahead, then one per product
 #pragma unroll
         for (int i = 0; i < NK - AHEAD; ++i) {
@@ -680,9 +680,9 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(artread_attend_t A,
             __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
             __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
         }
+        __builtin_amdgcn_s_setprio(0);   // the other wave of the SIMD may have its products first
         softmax_tile<T, KB, DP / 32>(s, P.c, mask, half, m, l, o);
-#pragma unroll
-        for (int i = EARLY; i < NV; ++i) vt[i] = lds_columns<T, DP>(vcol, 16 * (i / (DP / 32)), i % (DP / 32));
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int ks = 0; ks < 2 * KB; ++ks) {
             const V8 pw = weights8<T>(s[ks >> 1], ks & 1);

@@ -283,23 +283,26 @@ __global__ __launch_bounds__(256) void grad_sum_kernel(const GT* __restrict__ gr
     const int64_t valid = meta->valid;
     if ((int64_t)blockIdx.x >= S.sum_groups) {
         __shared__ uint64_t empty_rows;
-        const int64_t v0 = ((int64_t)blockIdx.x - S.sum_groups) * kClearRows;
-        if (threadIdx.x < 64) {
-            const int64_t v = v0 + threadIdx.x;
-            int64_t lo = 0, hi = valid;   // the first position whose key is not below v
-            while (lo < hi) {
-                const int64_t mid = (lo + hi) >> 1;
-                if ((int64_t)sorted[mid].key < v) lo = mid + 1;
-                else hi = mid;
-            }
-            const uint64_t found = __ballot(v < vocab && (lo >= valid || (int64_t)sorted[lo].key != v));
-            if (threadIdx.x == 0) empty_rows = found;
-        }
-        __syncthreads();
         const float zero[EPV] = {};
-        for (uint64_t rows = empty_rows; rows; rows &= rows - 1)
-            for (int c = threadIdx.x; c < S.cpr; c += blockDim.x)
-                put_row<OT, EPV>(table, v0 + __ffsll((unsigned long long)rows) - 1, dim, c, zero, 1.0f);
+        for (int64_t v0 = ((int64_t)blockIdx.x - S.sum_groups) * kClearRows; v0 < vocab;
+             v0 += ((int64_t)gridDim.x - S.sum_groups) * kClearRows) {
+            if (threadIdx.x < 64) {
+                const int64_t v = v0 + threadIdx.x;
+                int64_t lo = 0, hi = valid;   // the first position whose key is not below v
+                while (lo < hi) {
+                    const int64_t mid = (lo + hi) >> 1;
+                    if ((int64_t)sorted[mid].key < v) lo = mid + 1;
+                    else hi = mid;
+                }
+                const uint64_t found = __ballot(v < vocab && (lo >= valid || (int64_t)sorted[lo].key != v));
+                if (threadIdx.x == 0) empty_rows = found;
+            }
+            __syncthreads();
+            for (uint64_t rows = empty_rows; rows; rows &= rows - 1)
+                for (int c = threadIdx.x; c < S.cpr; c += blockDim.x)
+                    put_row<OT, EPV>(table, v0 + __ffsll((unsigned long long)rows) - 1, dim, c, zero, 1.0f);
+            __syncthreads();
+        }
         return;
     }
     const int r = S.cpr < 256 ? (int)threadIdx.x / S.cpr : 0;

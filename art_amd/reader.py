@@ -114,6 +114,13 @@ def _scale_value(scale):
     return scale
 
 
+def _base_value(base):
+    base = int(base)
+    if not -(1 << 63) <= base < 1 << 63:
+        raise ValueError("vocab_base must fit 64 bits, got %d" % base)
+    return base
+
+
 # ---- embedding lookup -----------------------------------------------------------------------------
 def _check_tokens(tokens, lengths):
     if tokens.dtype not in (torch.int32, torch.int64) or tokens.dim() < 1:
@@ -192,11 +199,11 @@ def embed_tokens(tokens, table, lengths=None, scale=1.0, vocab_base=0, out_dtype
     out_dtype = table.dtype if out_dtype is None else out_dtype
     if out_dtype != table.dtype and (table.dtype != torch.float32 or out_dtype not in _ABI):
         raise ValueError("out_dtype must be the table's type, or float16 / bfloat16 of a float32 table")
-    scale = _scale_value(scale)
+    scale, vocab_base = _scale_value(scale), _base_value(vocab_base)
     _one_device(table, tokens, lengths)
     if table.requires_grad and torch.is_grad_enabled():
-        return _EmbedTokens.apply(table, tokens, lengths, scale, int(vocab_base), out_dtype)
-    return _embed(tokens, table, lengths, scale, int(vocab_base), out_dtype)
+        return _EmbedTokens.apply(table, tokens, lengths, scale, vocab_base, out_dtype)
+    return _embed(tokens, table, lengths, scale, vocab_base, out_dtype)
 
 
 def embed_tokens_grad(grad_out, tokens, vocab, lengths=None, scale=1.0, vocab_base=0, dtype=None):
@@ -214,9 +221,9 @@ def embed_tokens_grad(grad_out, tokens, vocab, lengths=None, scale=1.0, vocab_ba
     dtype = grad_out.dtype if dtype is None else dtype
     if dtype != grad_out.dtype and dtype != torch.float32:
         raise ValueError("dtype must be grad_out's type or float32")
-    scale = _scale_value(scale)
+    scale, vocab_base = _scale_value(scale), _base_value(vocab_base)
     _one_device(grad_out, tokens, lengths)
-    return _embed_grad(grad_out, tokens, lengths, vocab, scale, int(vocab_base), dtype)
+    return _embed_grad(grad_out, tokens, lengths, vocab, scale, vocab_base, dtype)
 
 
 # ---- cross attention ------------------------------------------------------------------------------

@@ -12,6 +12,8 @@
  * to the caller: calls that may overlap need one each.  Arguments are checked before anything is
  * launched; lengths, tokens and the other contents of device memory are bounded by the kernels.
  *
+ * Outputs and workspaces overlap neither each other nor any input.
+ *
  * `lengths` is what arttok_gather writes: the number of valid entries of a padded row, negative for
  * a passage that is not there (read as 0); a value above the padded length is read as that length.
  */

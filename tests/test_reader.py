@@ -55,6 +55,7 @@ LENS = torch.full((3,), 5, dtype=torch.int32)
     dict(scale=float("nan")),
     dict(scale=float("inf")),
     dict(scale=1e39),
+    dict(vocab_base=1 << 63),
     dict(),  # all fine, but not on a GPU
 ], ids=str)
 def test_embed_tokens_refuses(kwargs):
@@ -154,7 +155,7 @@ def _embed_args(**change):
     dict(table=None), dict(out=None), dict(tokens=None), dict(token_bytes=2), dict(n=0), dict(len=0), dict(n=-1),
     dict(n=1 << 20, len=1 << 11), dict(n=1 << 40, len=1 << 40), dict(vocab=0), dict(vocab=1 << 31), dict(dim=0),
     dict(dim=(1 << 20) + 1), dict(stride=7), dict(table_dtype=3), dict(out_dtype=2), dict(out_dtype=-1),
-    dict(table_dtype=1, out_dtype=0), dict(table=SOME + 1), dict(scale=float("nan")),
+    dict(table_dtype=1, out_dtype=0), dict(table=SOME + 1), dict(tokens=SOME + 2), dict(lengths=SOME + 2), dict(scale=float("nan")),
 ], ids=str)
 def test_c_embed_refuses(change):
     assert rd._read().artread_embed(*_embed_args(**change)) == -1
@@ -203,7 +204,7 @@ BAD_ATTEND = [
 
 
 @pytest.mark.parametrize("change", BAD_ATTEND + [dict(q=None), dict(k=None), dict(v=None), dict(out=None),
-                                                 dict(q=SOME + 8), dict(out=SOME + 2), dict(rest=SOME + 8)], ids=str)
+                                                 dict(q=SOME + 8), dict(lse=SOME + 2), dict(lengths=SOME + 1), dict(out=SOME + 2), dict(rest=SOME + 8)], ids=str)
 def test_c_attend_refuses(change):
     lib, a = rd._read(), _attend(**change)
     if change in BAD_ATTEND:
