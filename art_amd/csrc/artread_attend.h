@@ -588,20 +588,21 @@ struct TileFetch {
     // src: state 0 of the tile; mask: which of its states are valid; stride below 2^24
     typedef typename std::conditional<KB == 1, uint32_t, uint64_t>::type Mask;
     __device__ __forceinline__ void fetch(const T* src, int64_t stride, Mask mask, int dim, uint32_t tile) const {
-        const bool full = whole_tile<KB>(mask);   // uniform
-        // from the lane's number anew each time: the offsets of all pieces would not fit beside the accumulators
-        const int lane = (int)opaque(threadIdx.x & 63), row = lane / CH, col = lane % CH;
+        const bool full = whole_tile<KB>(mask) && dim == DP;   // uniform
+        // from the lane's number anew each time: the offsets of all pieces would not fit beside the accumulators.  Of a
+        // row's place in the order of chunks its piece changes two bits at most.
+        const int lane = (int)opaque(threadIdx.x & 63), row = lane / CH, chunk = tile_chunk<DP>(row, lane % CH);
         const uint32_t bytes = (uint32_t)row * (uint32_t)stride * 2;
 #pragma unroll
         for (int x = 0; x < PW; ++x) {
-            const int piece = wave * PW + x, r = piece * PR + row, c = tile_chunk<DP>(r, col) * 8;
+            const int piece = wave * PW + x, c = chunk ^ (DP == 128 ? piece & 3 : (piece & 1) << 1);
             const uint32_t dst = tile + (uint32_t)piece * 1024;
             const T* base = src + (int64_t)(piece * PR) * stride;
             if (full) {
-                if (c < dim) dma16(base, bytes + c * 2, dst);
-            } else if (c < dim && (mask >> r & 1)) {
-                dma16(base, bytes + c * 2, dst);
-            } else {
+                dma16(base, bytes + c * 16, dst);
+            } else if (c * 8 < dim && (mask >> (piece * PR + row) & 1)) {
+                dma16(base, bytes + c * 16, dst);
+            } else if (!whole_tile<KB>(mask)) {
                 *(__attribute__((address_space(3))) u32x4*)(uintptr_t)(dst + lane * 16) = u32x4{0, 0, 0, 0};
             }
         }
