@@ -232,6 +232,27 @@ __device__ __forceinline__ void dma16(const void* base, uint32_t lane_bytes, uin
     asm volatile("s_nop 4\n\ts_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %3, %2\n\ts_mov_b32 m0, %0"
                  : "=&s"(keep) : "s"(dst), "s"(uniform_ptr(base)), "v"(lane_bytes) : "memory");
 }
+// N pieces `step` bytes apart in memory and STEP in LDS, those of piece x from lane offsets off[x]
+template <int N, int STEP>
+__device__ __forceinline__ void dma_pieces(const void* base, uint32_t step, const uint32_t* off, uint32_t dst) {
+    static_assert(N == 1 || N == 2 || N == 4, "");
+    const char* at = (const char*)uniform_ptr(base);
+    uint32_t keep;
+    if constexpr (N == 1) {
+        dma16(at, off[0], dst);
+    } else if constexpr (N == 2) {
+        asm volatile("s_nop 4\n\ts_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %5, %3\n\t"
+                     "s_add_u32 m0, m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %6, %4\n\ts_mov_b32 m0, %0"
+                     : "=&s"(keep) : "s"(dst), "n"(STEP), "s"(at), "s"(at + step), "v"(off[0]), "v"(off[1]) : "memory", "scc");
+    } else {
+        asm volatile("s_nop 4\n\ts_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %7, %3\n\t"
+                     "s_add_u32 m0, m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %8, %4\n\t"
+                     "s_add_u32 m0, m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %9, %5\n\t"
+                     "s_add_u32 m0, m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %10, %6\n\ts_mov_b32 m0, %0"
+                     : "=&s"(keep) : "s"(dst), "n"(STEP), "s"(at), "s"(at + step), "s"(at + 2 * (uint64_t)step),
+                       "s"(at + 3 * (uint64_t)step), "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]) : "memory", "scc");
+    }
+}
 __device__ __forceinline__ void dma4(const void* base, uint32_t lane_bytes, uint32_t dst) {
     uint32_t keep;
     asm volatile("s_nop 4\n\ts_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %3, %2\n\ts_mov_b32 m0, %0"
@@ -578,30 +599,41 @@ __device__ __forceinline__ int64_t xcd_item(int64_t id, int64_t items) {
     return (id >> 3) < per ? (id & 7) * per + (id >> 3) : items;
 }
 
-// Brings tiles of KB x 32 states into a ring of LDS: 1 KiB pieces, PW of a tile for each of NW waves.  States that are
-// not valid and columns behind dim become zeros: the states are written, the columns cleared once.
+// Brings tiles of KB x 32 states into a ring of LDS: 1 KiB pieces, every NW-th of a tile by one of NW waves.  States
+// that are not valid and columns behind dim become zeros: the states are written, the columns cleared once.
 template <typename T, int DP, int KB, int NW>
 struct TileFetch {
     static constexpr int CH = DP / 8, PR = 64 / CH, PW = 32 * KB / PR / NW;   // chunks per row, rows per piece
+    static constexpr int FOLD = DP == 128 ? 3 : 1;    // of a row's place in the order of chunks its piece changes two bits
+    static_assert(NW == 1 || NW % 4 == 0, "");
+    typedef typename std::conditional<KB == 1, uint32_t, uint64_t>::type Mask;
     int wave;
     __device__ __forceinline__ void start(int w) { wave = w; }
     // src: state 0 of the tile; mask: which of its states are valid; stride below 2^24
-    typedef typename std::conditional<KB == 1, uint32_t, uint64_t>::type Mask;
     __device__ __forceinline__ void fetch(const T* src, int64_t stride, Mask mask, int dim, uint32_t tile) const {
-        const bool full = whole_tile<KB>(mask) && dim == DP;   // uniform
-        // from the lane's number anew each time: the offsets of all pieces would not fit beside the accumulators.  Of a
-        // row's place in the order of chunks its piece changes two bits at most.
-        const int lane = (int)opaque(threadIdx.x & 63), row = lane / CH, chunk = tile_chunk<DP>(row, lane % CH);
+        const int lane = (int)opaque(threadIdx.x & 63), row = lane / CH;   // anew each time: registers are few
+        const int chunk = tile_chunk<DP>(row, lane % CH) ^ ((wave & FOLD) << (DP == 128 ? 0 : 1));
         const uint32_t bytes = (uint32_t)row * (uint32_t)stride * 2;
+        uint32_t off[PW];
+#pragma unroll
+        for (int x = 0; x < PW; ++x) off[x] = bytes + (uint32_t)(chunk ^ ((x * NW & FOLD) << (DP == 128 ? 0 : 1))) * 16;
+        src += (int64_t)(wave * PR) * stride;
+        tile += (uint32_t)wave * 1024;
+        const uint32_t step = (uint32_t)stride * (NW * PR * 2);
+        if (whole_tile<KB>(mask)) {   // uniform
+            constexpr int N = PW < 4 ? PW : 4;
+            if (dim == DP) {
+#pragma unroll
+                for (int x = 0; x < PW; x += N) dma_pieces<N, NW * 1024>((const char*)src + x * (uint64_t)step, step, off + x, tile + x * (NW * 1024));
+                return;
+            }
+        }
 #pragma unroll
         for (int x = 0; x < PW; ++x) {
-            const int piece = wave * PW + x, c = chunk ^ (DP == 128 ? piece & 3 : (piece & 1) << 1);
-            const uint32_t dst = tile + (uint32_t)piece * 1024;
-            const T* base = src + (int64_t)(piece * PR) * stride;
-            if (full) {
-                dma16(base, bytes + c * 16, dst);
-            } else if (c * 8 < dim && (mask >> (piece * PR + row) & 1)) {
-                dma16(base, bytes + c * 16, dst);
+            const int piece = x * NW + wave, c = chunk ^ ((x * NW & FOLD) << (DP == 128 ? 0 : 1));
+            const uint32_t dst = tile + (uint32_t)x * (NW * 1024);
+            if (c * 8 < dim && (mask >> (piece * PR + row) & 1)) {
+                dma16((const char*)src + x * (uint64_t)step, off[x], dst);
             } else if (!whole_tile<KB>(mask)) {
                 *(__attribute__((address_space(3))) u32x4*)(uintptr_t)(dst + lane * 16) = u32x4{0, 0, 0, 0};
             }
