@@ -142,7 +142,8 @@ struct Walk {
     __device__ __forceinline__ bool settle() {
         while (j0 >= n) {
             j0 -= (n + KT - 1) / KT * KT;
-            if (++p >= passages) return false;
+            p = uniform(p + 1);
+            if (p >= passages) return false;
             if ((p & 63) == 0) hold();
             n = __builtin_amdgcn_readlane(held, p & 63);
         }
@@ -611,8 +612,8 @@ struct TileFetch {
     __device__ __forceinline__ void start(int w) { wave = w; }
     // src: state 0 of the tile; mask: which of its states are valid; stride below 2^24
     __device__ __forceinline__ void fetch(const T* src, int64_t stride, Mask mask, int dim, uint32_t tile) const {
-        const int lane = (int)opaque(threadIdx.x & 63), row = lane / CH;   // anew each time: registers are few
-        const int chunk = tile_chunk<DP>(row, lane % CH) ^ ((wave & FOLD) << (DP == 128 ? 0 : 1));
+        const uint32_t lane = opaque(threadIdx.x & 63), row = lane / CH;   // anew each time: registers are few
+        const uint32_t chunk = tile_chunk<DP>(row, lane % CH) ^ ((wave & FOLD) << (DP == 128 ? 0 : 1));
         const uint32_t bytes = (uint32_t)row * (uint32_t)stride * 2;
         uint32_t off[PW];
 #pragma unroll
@@ -630,9 +631,9 @@ struct TileFetch {
         }
 #pragma unroll
         for (int x = 0; x < PW; ++x) {
-            const int piece = x * NW + wave, c = chunk ^ ((x * NW & FOLD) << (DP == 128 ? 0 : 1));
+            const uint32_t piece = x * NW + wave, c = chunk ^ ((x * NW & FOLD) << (DP == 128 ? 0 : 1));
             const uint32_t dst = tile + (uint32_t)x * (NW * 1024);
-            if (c * 8 < dim && (mask >> (piece * PR + row) & 1)) {
+            if (c * 8 < (uint32_t)dim && (mask >> (piece * PR + row) & 1)) {
                 dma16((const char*)src + x * (uint64_t)step, off[x], dst);
             } else if (!whole_tile<KB>(mask)) {
                 *(__attribute__((address_space(3))) u32x4*)(uintptr_t)(dst + lane * 16) = u32x4{0, 0, 0, 0};
