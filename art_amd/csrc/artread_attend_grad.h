@@ -214,7 +214,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_grad_q_kernel(artread_atten
     if (w >= total) return;
     const int64_t rb = w % P.row_blocks, other = w / P.row_blocks;
     const int split = (int)(other % P.splits);
-    const int64_t bk = other / P.splits, kh = bk % A.kv_heads, b = bk / A.kv_heads;
+    const int64_t hb = other / P.splits, kh = hb / A.batch, b = hb % A.batch;
     const int64_t r = (rb * NW + wave) * 32 + (lane & 31);
     const T* kbase = (const T*)A.k + b * A.k_batch + kh * A.k_head;
     const T* vbase = (const T*)A.v + b * A.v_batch + kh * A.v_head;
@@ -234,7 +234,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_grad_q_kernel(artread_atten
     load_q<T, DP>(A, P, (const T*)A.q, A.q_batch, A.q_row, A.q_head, b, kh, r, half, P.q_and, P.q_xor, q);
     load_q<T, DP>(A, P, (const T*)G.grad_out, G.g_batch, G.g_row, G.g_head, b, kh, r, half, 0xffffffffu, 0u, g);
     RowStat st{INFINITY, 0.0f};
-    if (r < P.row_count) st = stats[bk * P.pad_rows + r];
+    if (r < P.row_count) st = stats[(b * A.kv_heads + kh) * P.pad_rows + r];
     f32x16 acc[DP / 32];
     Spread<T> spread;
 #pragma unroll
