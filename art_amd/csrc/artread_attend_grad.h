@@ -361,33 +361,49 @@ __global__ __launch_bounds__(256, 2) void attend_grad_kv_kernel(artread_attend_t
             kf[s] = load8<T>(kp + 16 * s, ok);
             vf[s] = load8<T>(vp + 16 * s, ok);
         }
-        // pieces of 1 KiB: PR rows each, PW of a tile for each wave; rows that are not there repeat the last one
-        // (their weight is zero), columns behind dim the first (they meet zeros of K and V)
+        // pieces of 1 KiB, PR rows each, every fourth of a tile by one wave: 4 * PR rows from one to the next.  Where that
+        // is whole query positions, a lane's pieces of all whole tiles lie at one offset from uniform addresses.
         constexpr int CH = DP / 8, PR = 64 / CH, PW = 32 * RT / PR / 4;
         const int tiles = (int)((P.row_count + 32 * RT - 1) / (32 * RT));
         const RowStat* sp = stats + (b * A.kv_heads + kh) * P.pad_rows;
         const T* qb = (const T*)A.q + b * A.q_batch + kh * P.share * A.q_head;
         const T* gb = (const T*)G.grad_out + b * G.g_batch + kh * P.share * G.g_head;
+        const uint32_t positions = 4 * PR / P.share;
+        const bool even = positions * P.share == 4 * PR && dim == DP;
         auto fetch = [&](int tile, int stage) {
-            int64_t t0, h0;
+            int64_t t0, h0, t, h;
             split_row(P, 0, (uint32_t)tile * 32 * RT, &t0, &h0);
-            const int ln = (int)opaque(lane), prow = ln / CH;
+            const uint32_t ln = opaque(lane), prow = ln / CH;
+            const uint32_t dst = lds_offset(&qtile[stage][wave * 512]), chunk = tile_chunk<DP>(prow, ln % CH) ^ (DP == 128 ? wave : (wave & 1) << 1);
+            const T *qt = qb + t0 * A.q_row, *gt = gb + t0 * G.g_row;
+            if (even && (int64_t)(tile + 1) * 32 * RT <= P.row_count) {   // uniform
+                split_row(P, 0, wave * PR + prow, &t, &h);
+                uint32_t qo[PW], go[PW];
 #pragma unroll
-            for (int x = 0; x < PW; ++x) {
-                const int piece = wave * PW + x, row = piece * PR + prow;
-                int64_t r = (int64_t)tile * 32 * RT + row, t, h;
-                r = r < P.row_count ? r : P.row_count - 1;
-                split_row(P, 0, (uint32_t)r, &t, &h);
-                int col = tile_chunk<DP>(row, ln % CH) * 8;
-                col = col < dim ? col : 0;
-                // bytes from the tile's first query position: a tile spans at most as many of them as rows
-                const uint32_t dt = (uint32_t)t - (uint32_t)t0;
-                dma16(qb + t0 * A.q_row, (dt * (uint32_t)A.q_row + (uint32_t)(h * A.q_head) + col) * 2, lds_offset(&qtile[stage][piece * 512]));
-                dma16(gb + t0 * G.g_row, (dt * (uint32_t)G.g_row + (uint32_t)(h * G.g_head) + col) * 2, lds_offset(&qtile[2 + stage][piece * 512]));
+                for (int x = 0; x < PW; ++x) {
+                    qo[x] = ((uint32_t)t * (uint32_t)A.q_row + (uint32_t)(h * A.q_head) + chunk * 8) * 2;
+                    go[x] = ((uint32_t)t * (uint32_t)G.g_row + (uint32_t)(h * G.g_head) + chunk * 8) * 2;
+                }
+                dma_pieces<PW, 4096>(qt, positions * (uint32_t)A.q_row * 2, qo, dst);
+                dma_pieces<PW, 4096>(gt, positions * (uint32_t)G.g_row * 2, go, dst + 2 * TILE * 2);
+            } else {
+                // rows that are not there repeat the last one (their weight is zero), columns behind dim the first (they
+                // meet zeros of K and V)
+                const uint32_t col = chunk * 8 < (uint32_t)dim ? chunk * 8 : 0;
+#pragma unroll
+                for (int x = 0; x < PW; ++x) {
+                    int64_t r = (int64_t)tile * 32 * RT + (x * 4 + wave) * PR + prow;
+                    r = r < P.row_count ? r : P.row_count - 1;
+                    split_row(P, 0, (uint32_t)r, &t, &h);
+                    // bytes from the tile's first query position: a tile spans at most as many of them as rows
+                    const uint32_t dt = (uint32_t)t - (uint32_t)t0;
+                    dma16(qt, (dt * (uint32_t)A.q_row + (uint32_t)(h * A.q_head) + col) * 2, dst + x * 4096);
+                    dma16(gt, (dt * (uint32_t)G.g_row + (uint32_t)(h * G.g_head) + col) * 2, dst + 2 * TILE * 2 + x * 4096);
+                }
             }
 #pragma unroll
             for (int x = 0; x < RT; ++x)   // the statistics are padded to whole tiles
-                dma4(sp + tile * 32 * RT + 32 * x, (uint32_t)lane * 4, lds_offset(&stile[stage][wave][32 * x]));
+                dma4(sp + tile * 32 * RT + 32 * x, ln * 4, lds_offset(&stile[stage][wave][32 * x]));
         };
         if (split < tiles) fetch(split, 0);
         // one loop for waves with keys and one for those without: both load and meet at the barriers
