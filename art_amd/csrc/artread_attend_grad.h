@@ -216,16 +216,24 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_grad_q_kernel(artread_atten
     const int split = (int)(other % P.splits);
     const int64_t hb = other / P.splits, kh = hb / A.batch, b = hb % A.batch;
     const int64_t r = (rb * NW + wave) * 32 + (lane & 31);
-    const T* kbase = (const T*)A.k + b * A.k_batch + kh * A.k_head;
-    const T* vbase = (const T*)A.v + b * A.v_batch + kh * A.v_head;
+    const T* kbase = (const T*)A.k + b * A.k_batch + kh * A.k_head + fetcher.first(A.k_row);
+    const T* vbase = (const T*)A.v + b * A.v_batch + kh * A.v_head + fetcher.first(A.v_row);
     Walk<32 * KB> walk;   // of the tiles fetched
     walk.start(A, P, b, split, P.splits);
     uint64_t mask = 0, next_mask = 0;   // of the tile worked on, and of the one being fetched
+    const T *kp = kbase, *vp = vbase;   // of the tile to fetch
+    const int64_t kstep = walk.step * A.k_row, vstep = walk.step * A.v_row;
     auto fetch = [&](int stage) {
         if (!walk.settle()) return false;
+        if (walk.moved) {
+            kp = kbase + walk.p * A.k_passage + walk.j0 * A.k_row;
+            vp = vbase + walk.p * A.v_passage + walk.j0 * A.v_row;
+        }
         next_mask = walk.mask;
-        fetcher.fetch(kbase + walk.p * A.k_passage + walk.j0 * A.k_row, A.k_row, next_mask, dim, lds_offset(ring[stage]));
-        fetcher.fetch(vbase + walk.p * A.v_passage + walk.j0 * A.v_row, A.v_row, next_mask, dim, lds_offset(ring[2 + stage]));
+        fetcher.fetch(kp, A.k_row, next_mask, dim, lds_offset(ring[stage]));
+        fetcher.fetch(vp, A.v_row, next_mask, dim, lds_offset(ring[2 + stage]));
+        kp += kstep;
+        vp += vstep;
         walk.advance();
         return true;
     };
