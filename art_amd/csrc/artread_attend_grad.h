@@ -191,6 +191,20 @@ __device__ __forceinline__ void store_turned(T* first, int64_t stride, int rows,
     }
 }
 
+// The order of N products whose operands take R LDS reads each: the reads of A products ahead, of which the scheduler by
+// itself keeps one.  Nothing else moves in or out: registers for more are not there.
+template <int N, int R, int A>
+__device__ __forceinline__ void ahead() {
+    __builtin_amdgcn_sched_group_barrier(0x100, R * A, 0);
+#pragma unroll
+    for (int k = 0; k < N - A; ++k) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, A, 0);
+    __builtin_amdgcn_sched_barrier(0);
+}
+
 // ---- dQ: the row walk -----------------------------------------------------------------------------------
 // NW waves of 32 rows share tiles of 32 * KB keys; while a tile is worked on the next one arrives in LDS.  With P.splits > 1 each split leaves
 // its f32 part of dQ at part + split * (all of dQ).
@@ -432,6 +446,7 @@ __global__ __launch_bounds__(256, 2) void attend_grad_kv_kernel(artread_attend_t
                             s = Mma<T>::mul(lds_rows<T, DP>(qrow, x, k), kf[k], s);
                             dp = Mma<T>::mul(lds_rows<T, DP>(qrow, 2 * RT + x, k), vf[k], dp);
                         }
+                        ahead<DP / 8, 1, DP == 128 ? 2 : 4>();
 #pragma unroll
                         for (int y = 0; y < 4; ++y) {
                             const float4 a = *(const float4*)&stile[stage][wave][32 * x + 8 * y + 4 * half];
@@ -445,16 +460,21 @@ __global__ __launch_bounds__(256, 2) void attend_grad_kv_kernel(artread_attend_t
                             }
                         }
                         spread.fit(dp, dk);
+                        V8 pw[2], ds[2];
 #pragma unroll
                         for (int ks = 0; ks < 2; ++ks) {
-                            const V8 pw = weights8<T>(s, ks), ds = weights8<T>(dp, ks);
+                            pw[ks] = weights8<T>(s, ks);
+                            ds[ks] = weights8<T>(dp, ks);
+                        }
+                        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                        for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
                             for (int db = 0; db < DP / 32; ++db) {
-                                dv[db] = Mma<T>::mul(lds_columns<T, DP>(qcol, 32 * (2 * RT + x) + 16 * ks, db), pw, dv[db]);
-                                dk[db] = Mma<T>::mul(lds_columns<T, DP>(qcol, 32 * x + 16 * ks, db), ds, dk[db]);
+                                dv[db] = Mma<T>::mul(lds_columns<T, DP>(qcol, 32 * (2 * RT + x) + 16 * ks, db), pw[ks], dv[db]);
+                                dk[db] = Mma<T>::mul(lds_columns<T, DP>(qcol, 32 * x + 16 * ks, db), ds[ks], dk[db]);
                             }
-                        }
-                        __builtin_amdgcn_sched_barrier(0);   // the next rows' operands would not fit beside these
+                        ahead<DP / 8, 2, 4>();
                     }
                 }
                 stage ^= 1;
