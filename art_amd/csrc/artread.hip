@@ -549,10 +549,9 @@ static void launch_attend_grad(const artread_attend_t* a, const artread_attend_g
         return;
     }
     const dim3 gq = grid2(S.q.items * S.q.splits);
-    if (S.narrow)
-        hipLaunchKernelGGL((attend_grad_q_kernel<T, DP, 1, 1>), gq, dim3(64), 0, st, *a, *g, S.q, stats, part);
-    else
-        hipLaunchKernelGGL((attend_grad_q_kernel<T, DP, 4, 2>), gq, dim3(256), 0, st, *a, *g, S.q, stats, part);
+    if constexpr (DP == 128)   // 33 to 64 rows; at 64 columns they are the one walk's
+        if (S.narrow) hipLaunchKernelGGL((attend_grad_q_kernel<T, DP, 1, 1>), gq, dim3(64), 0, st, *a, *g, S.q, stats, part);
+    if (!S.narrow) hipLaunchKernelGGL((attend_grad_q_kernel<T, DP, 4, 2>), gq, dim3(256), 0, st, *a, *g, S.q, stats, part);
     if (S.q.splits > 1) launch_sum<T>(part, S.all_q, S.q.splits, g->grad_q, S.all_q, st);
     hipLaunchKernelGGL((attend_grad_kv_kernel<T, DP>), grid2(S.kv.items * S.kv.splits), dim3(256), 0, st, *a, *g,
                        S.kv, stats, part);
