@@ -240,7 +240,10 @@ def attend_ref(q, k, v, lengths, grad=None, scale=None):
     ds = (dim + 4) * U32 * abs(scale) * torch.matmul(Q.abs(), K.abs().transpose(2, 3)).amax(3, keepdim=True)
     ds = ds + 520 * U32
     n_keys = inside.sum(3, keepdim=True)
-    floor = TINY[t] * 2.0 ** -9  # weights keep a power of two beside them: what a subnormal one loses
+    # weights keep a power of two beside them: what a subnormal one loses; exp2 gives zero for what 32 bits hold as a
+    # subnormal, below 2^-126, and a product takes subnormal operands as zero
+    flush = 2.0 ** -126
+    floor = max(TINY[t] * 2.0 ** -9, flush)
     pv = torch.matmul(p, V.abs())
     v_max = V.abs().amax((2, 3), keepdim=True)
     # weights: u, their scores' error in numerator and sum: 2 ds, the 32-bit sums of numerator and weights
@@ -262,7 +265,8 @@ def attend_ref(q, k, v, lengths, grad=None, scale=None):
     # of out and rest leave u * u
     gv = torch.matmul(G.abs(), V.abs().transpose(2, 3))
     delta_off = (G.abs() * (out_bound - u * out.abs() + (u * u + (dim + 1) * U32) * out.abs())).sum(3, keepdim=True)
-    dS_off = dS.abs() * (u + p_off) + p * (dim * U32 * gv + delta_off) * (1 + u + p_off)
+    # a weight that was flushed is off by flush times its factor, a dS that was by flush
+    dS_off = dS.abs() * (u + p_off) + p * (dim * U32 * gv + delta_off) * (1 + u + p_off) + flush * ((dp - delta).abs() + 1) * inside
     n_rows = rows * share
     small = TINY[t] * 2.0 ** -9 * dS.abs().amax((2, 3), keepdim=True) / max(torch.finfo(t).smallest_normal, 2.0 ** -14)
     a = abs(scale)
@@ -373,6 +377,47 @@ def test_attention_layouts(dtype):
     wide = torch.zeros((4, 6), device="cuda", dtype=torch.int32)
     wide[::2, ::2] = lengths
     same(q, k, v, wide[::2, ::2], grad)
+
+
+# heads that share a key head in numbers that divide a tile's rows and in others; the last tile of rows is short
+SHARED = [(2, 50, 3, 70, 6, 2, 128), (1, 40, 2, 130, 16, 1, 64), (1, 12, 2, 100, 32, 1, 128), (2, 30, 3, 70, 8, 1, 128),
+          (1, 70, 2, 90, 10, 2, 64), (1, 192, 2, 64, 4, 4, 128)]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("shape", SHARED, ids=str)
+def test_attention_shared_heads_in_strided_rows(shape, dtype):
+    """Many rows of shared heads, whose queries and gradients lie in wider tensors."""
+    q, k, v, lengths, grad = attend_case(*shape, dtype, seed=37)
+    check_attend(q, k, v, lengths, grad)
+    out, saved = rd.cross_attention(q, k, v, lengths, return_saved=True)
+    want = rd.cross_attention_grad(grad, q, k, v, out, saved, lengths)
+    batch, rows, passages, length, heads, kv_heads, dim = shape
+
+    def inside(x, pad):
+        wide = torch.full((*x.shape[:-2], x.shape[-2] + pad, dim + 8 * pad), float("nan"), device="cuda", dtype=dtype)
+        wide[..., 1:1 + x.shape[-2], 8:8 + dim] = x
+        return wide[..., 1:1 + x.shape[-2], 8:8 + dim]
+
+    qs, ks, vs, gs = inside(q, 2), inside(k, 3), inside(v, 4), inside(grad, 5)
+    o, l = rd.cross_attention(qs, ks, vs, lengths, return_saved=True)
+    assert torch.equal(o, out) and torch.equal(l[0], saved[0])
+    got = rd.cross_attention_grad(gs, qs, ks, vs, o, l, lengths)
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("rows", [1, 40, 200])
+@pytest.mark.parametrize("step", [0.002, 0.03, -0.03, 2.0])
+def test_attention_scores_that_rise_along_the_keys(step, rows, dtype):
+    """Maxima that creep up by less than a factor of two a tile, by some, by many, and that fall."""
+    q, k, v, lengths, grad = attend_case(2, rows, 3, 230, 2, 1, 64, dtype, 39, q_std=0.5)
+    q[..., 0] = 8.0
+    k[..., 0] = (torch.arange(690, device="cuda").view(3, 230, 1) * step).to(dtype)
+    check_attend(q, k, v, lengths, grad)
+    alone = rd.cross_attention(q[:, :1], k, v, lengths)
+    if rows == 1:
+        assert torch.equal(alone, rd.cross_attention(q, k, v, lengths))
 
 
 def test_attention_broadcast_states():
