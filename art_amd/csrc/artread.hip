@@ -187,8 +187,9 @@ extern "C" int64_t artread_embed_grad_workspace(int64_t vocab, int64_t dim, int6
 }
 
 template <typename GT, typename OT, int EPV>
-static void launch_grad_sums(const void* grad, const Pair* sorted, const SortMeta* meta, const Tokens& T, float scale, void* table, int dim, const GradSpace& s, float* partial,
-                             int32_t* chain_end, hipStream_t st) {
+static void launch_grad_sums(const void* grad, const Pair* sorted, const SortMeta* meta, const Tokens& T, float scale,
+                             void* table, int dim, const GradSpace& s, float* partial, int32_t* chain_end,
+                             hipStream_t st) {
     SumPlan S;
     S.run = s.run;
     S.cpr = dim / EPV;
@@ -202,7 +203,8 @@ static void launch_grad_sums(const void* grad, const Pair* sorted, const SortMet
     hipLaunchKernelGGL((grad_sum_kernel<GT, OT, EPV>), dim3((unsigned)(S.sum_groups + clear)), dim3(threads), 0, st,
                        (const GT*)grad, sorted, meta, T.vocab, scale, (OT*)table, dim, S, partial, chain_end);
     if (S.workers > 1)
-        hipLaunchKernelGGL((grad_join_kernel<OT>), dim3((unsigned)((S.workers + kJoinWaves - 1) / kJoinWaves), (unsigned)((dim + 255) / 256)),
+        hipLaunchKernelGGL((grad_join_kernel<OT>),
+                           dim3((unsigned)((S.workers + kJoinWaves - 1) / kJoinWaves), (unsigned)((dim + 255) / 256)),
                            dim3(64 * kJoinWaves), 0, st, sorted, meta, scale, (OT*)table, dim, S, partial, chain_end);
 }
 
@@ -387,13 +389,13 @@ static AttendShape attend_shape(const artread_attend_t* given) {
     if (S.stream) {
         // Workgroups that fill the chip.  By registers two waves share a SIMD, three at 64 columns and 32 rows;
         // a round more evens out the lengths, while each more leaves partial results to join (us, kernel + join,
-        // for 2048, 3072, 4096 waves: 64 questions x 32 passages x 64 columns 222, 203, 195; 2 x 100 x 128 columns
+        // for 8, 12, 16 waves a compute unit: 64 questions x 32 passages x 64 columns 222, 203, 195; 2 x 100 x 128 columns
         // 76, 87, 89; 48 rows 161, 151, 159).
-        const int64_t waves = a->dim > 64 ? 2048 : (S.qb == 2 ? 3072 : 4096);
+        const int64_t waves = 256 * (a->dim > 64 ? 8 : (S.qb == 2 ? 12 : 16));
         int64_t want = (waves / 4 + P.items - 1) / P.items;
         if (P.items < waves && tiles >= 4) P.walkers = 4;
         else want = 1;
-        const int64_t most = tiles / 16;   // a part of fewer than four tiles a wave costs less than its join
+        const int64_t most = tiles / 16;   // parts of at least four tiles a wave: shorter ones cost more in the join than they save
         want = want < most ? want : most;
         P.splits = (int)(want < 1 ? 1 : (want < 256 ? want : 256));
     } else {

@@ -15,7 +15,8 @@ struct RowStat {
     float x, delta;
 };
 
-// 16 lanes per row, eight columns each.  The rows of a key head are padded to whole tiles of 64.
+// 16 lanes per row, eight columns each.  The rows of a key head are padded to whole tiles of 64.  Bound by reading
+// grad_out, out and rest: 8 x 1,024 rows of 16 x 128 bf16 in 19 us, 5.3 TB/s.
 template <typename T>
 __global__ __launch_bounds__(256) void attend_delta_kernel(artread_attend_t A, artread_attend_grads_t G, AttendPlan P,
                                                            int64_t all_rows, RowStat* __restrict__ stats) {
@@ -53,7 +54,6 @@ __global__ __launch_bounds__(256) void attend_delta_kernel(artread_attend_t A, a
 // accumulators follow.  bf16 has the exponents of f32 and needs none.
 template <typename T>
 struct Spread {
-    float f = 1.0f;
     __device__ __forceinline__ float inverse() const { return 1.0f; }
     template <int N>
     __device__ __forceinline__ void fit(f32x16&, f32x16 (&)[N]) {}
@@ -122,9 +122,9 @@ struct SpreadAll<f16> {
 
 // dS as two terms, the rounded value and what the rounding took, for products that share the other operand's LDS read.
 // With one term the error of dQ is up to 1.5 times that of its own rounding, where a row's sum hangs on few keys; with
-// two it is that rounding (train_top100: 2.08e-4 instead of 3.1e-4 of f16 dQ, row walk of train_long 480 us instead of
-// 407).  The key walk takes one: its sums run over more than 32 rows, 1.4 times, and the registers of a second term
-// would spill V.  P takes one everywhere.
+// two it is that rounding (48 rows, 100 x 250 states of 64 f16: 2.08e-4 instead of 3.1e-4).  It costs the row walk an
+// eighth to a sixth of its time.  The key walk takes one: its sums run over more than 32 rows, 1.4 times, and the
+// registers of a second term would spill (640 us instead of 510).  P takes one everywhere.
 template <typename T>
 __device__ __forceinline__ void terms8(const f32x16& s, int ks, typename Mma<T>::V8& hi, typename Mma<T>::V8& lo) {
 #pragma unroll
@@ -152,7 +152,7 @@ __device__ __forceinline__ u32x2 pack4(float a, float b, float c, float d) {
 
 // Accumulators of 32 keys (lane: key, elements: columns), times f, rounded, as rows: through 4 KiB of LDS of the
 // wave's own, 64 columns at a time, so that eight lanes hold 128 bytes of a row.  Stores of 8 bytes by 64 rows would
-// ask the L2 for eight times as many writes, which bound the gradient of few rows (456 us against 292).
+// ask the L2 for eight times as many writes, which bound the gradient of few rows (456 us against 292 for 48 rows of 100 x 250 states).
 // w[4 * c + x]: row 8 * x + (lane >> 3), columns 64 * c + 8 * (lane & 7)..
 template <typename T, int DP>
 __device__ __forceinline__ void turn_keys(const f32x16 (&acc)[DP / 32], float f, bool key, uint32_t lds, int lane,
@@ -206,8 +206,11 @@ __device__ __forceinline__ void ahead() {
 }
 
 // ---- dQ: the row walk -----------------------------------------------------------------------------------
-// NW waves of 32 rows share tiles of 32 * KB keys; while a tile is worked on the next one arrives in LDS.  With P.splits > 1 each split leaves
-// its f32 part of dQ at part + split * (all of dQ).
+// NW waves of 32 rows share tiles of 32 * KB keys; while a tile is worked on the next one arrives in LDS.  With
+// P.splits > 1 each split leaves its f32 part of dQ at part + split * (all of dQ).  Bound by the matrix units and what
+// stands between their products: 8 x 8 x 512 states of 128 bf16 columns, 75 % valid, 4,096 rows a key head in 437-470 us,
+// 880-940 TFLOP/s with the second term's products, which run in 54 % of the cycles.  Four waves; for up to 64 rows one
+// wave a workgroup, since the others would have none.
 template <typename T, int DP, int NW, int KB>
 __global__ __launch_bounds__(64 * NW, 2) void attend_grad_q_kernel(artread_attend_t A, artread_attend_grads_t G,
                                                                     AttendPlan P, const RowStat* __restrict__ stats,
@@ -322,7 +325,9 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_grad_q_kernel(artread_atten
 // ---- dK and dV: the key walk ------------------------------------------------------------------------------
 // Four waves of 32 keys of one passage share tiles of 64 rows of Q and dO; while a tile is worked on the next one
 // arrives in LDS.  Each is read as rows for S and dP and transposed for dK and dV.  With P.splits > 1 the rows are dealt
-// to splits, which leave f32 parts of dK and dV.
+// to splits, which leave f32 parts of dK and dV.  K, V, dK and dV of 32 keys are 192 registers of 256, so operands are few
+// ahead, and the wait for LDS is what a wave mostly does besides products (48 % of the cycles): 480-500 us for 8 x 8 x 512
+// states of 128 bf16 columns, 75 % valid, 4,096 rows a key head, 820 TFLOP/s.
 template <typename T, int DP>
 __global__ __launch_bounds__(256, 2) void attend_grad_kv_kernel(artread_attend_t A, artread_attend_grads_t G,
                                                                   AttendPlan P, const RowStat* __restrict__ stats,
@@ -519,11 +524,14 @@ __global__ __launch_bounds__(256, 2) void attend_grad_kv_kernel(artread_attend_t
 // ---- all three gradients at once: few rows -----------------------------------------------------------------
 // Up to 32 * RB rows per key head.  A wave walks tiles of 32 keys, those behind the lengths among them (they get their
 // zeros here), and finishes dK and dV of a tile before the next: every state is read once and every gradient written
-// once, which is what bounds this, where the two walks would read the states twice.  S^T and dP^T leave P^T and dS^T
-// as B operands over the keys, for dQ; dV and dK want them over the rows, so both go through a 32 x 32 tile of LDS and
-// come back by the transposing read.  A tile's results are stored once the next tile has arrived: waiting for that
-// tile then never waits for the stores.  The waves of a workgroup add their dQ in LDS, in order.  PACK: passages too
-// short to fill tiles of their own are packed; a kernel of its own, for the registers.
+// once, which is what bounds this, where the two walks would read the states twice (16 rows of 8 x 12 heads, 100 x 250
+// states of 64 bf16, 75 % valid: 246 us, 4.4 TB/s; of 128 columns 470 us, 4.6 TB/s; 48 rows of 64 f16, 62 % valid: 270 us,
+// 3.7 TB/s, where 1,100 vector instructions a tile stand beside the bytes).  Two tiles of K in LDS, the next one on its way
+// from the start of a tile, cost more workgroups than they save waiting (325 us against 294, fewer rows 2 % more).  S^T
+// and dP^T leave P^T and dS^T as B operands over the keys, for dQ; dV and dK want them over the rows, so both go through a
+// 32 x 32 tile of LDS and come back by the transposing read.  A tile's results are stored once the next tile has arrived:
+// waiting for that tile then never waits for the stores.  The waves of a workgroup add their dQ in LDS, in order.  PACK:
+// passages too short to fill tiles of their own are packed; a kernel of its own, for the registers.
 template <typename T, int DP, int RB, int NW, bool PACK>
 __global__ __launch_bounds__(64 * NW, 2) void attend_grad_stream_kernel(artread_attend_t A, artread_attend_grads_t G,
                                                                         AttendPlan P, const RowStat* __restrict__ stats,
@@ -762,7 +770,8 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_grad_stream_kernel(artread_
     }
 }
 
-// out = sum of `splits` f32 parts `stride` apart, in order, rounded once; n is a multiple of 8
+// out = sum of `splits` f32 parts `stride` apart, in order, rounded once; n is a multiple of 8.  Five parts of 8 x 48 x 12
+// rows of 64: 5 us, mostly a launch.
 template <typename T>
 __global__ __launch_bounds__(256) void attend_sum_kernel(const float* __restrict__ part, int64_t stride, int splits,
                                                          T* __restrict__ out, int64_t n) {

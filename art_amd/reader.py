@@ -303,19 +303,24 @@ def _attend(query, key, value, lengths, sizes, scale, want_lse, want_rest):
 
 class _CrossAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, query, key, value, lengths, sizes, scale):
+    def forward(ctx, query, key, value, lengths, sizes, scale, want_saved):
         out, lse, rest = _attend(query, key, value, lengths, sizes, scale, True, True)
         ctx.save_for_backward(query, key, value, lengths, out, lse, rest)
         ctx.of = sizes, scale
+        if not want_saved:   # each further result costs the call some microseconds
+            return out
         ctx.mark_non_differentiable(lse, rest)
+        ctx.set_materialize_grads(False)   # no zeros for lse and rest
         return out, lse, rest
 
     @staticmethod
     @once_differentiable
-    def backward(ctx, grad_out, _lse, _rest):
+    def backward(ctx, grad_out, *_):
+        if grad_out is None:
+            return (None,) * 7
         query, key, value, lengths, out, lse, rest = ctx.saved_tensors
         _one_device(query, grad_out)
-        return _attend_grad(grad_out, query, key, value, lengths, out, lse, rest, *ctx.of) + (None, None, None)
+        return _attend_grad(grad_out, query, key, value, lengths, out, lse, rest, *ctx.of) + (None, None, None, None)
 
 
 def cross_attention(query, key, value, lengths=None, scale=None, return_lse=False, return_saved=False):
@@ -336,7 +341,9 @@ def cross_attention(query, key, value, lengths=None, scale=None, return_lse=Fals
     sizes, scale = _plan(query, key, value, lengths, scale)
     _one_device(query, key, value, lengths)
     if (query.requires_grad or key.requires_grad or value.requires_grad) and torch.is_grad_enabled():
-        out, lse, rest = _CrossAttention.apply(query, key, value, lengths, sizes, scale)
+        if not (return_lse or return_saved):
+            return _CrossAttention.apply(query, key, value, lengths, sizes, scale, False)
+        out, lse, rest = _CrossAttention.apply(query, key, value, lengths, sizes, scale, True)
     else:
         out, lse, rest = _attend(query, key, value, lengths, sizes, scale, return_lse or return_saved, return_saved)
     if return_saved:
