@@ -323,11 +323,68 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_grad_q_kernel(artread_atten
 }
 
 // ---- dK and dV: the key walk ------------------------------------------------------------------------------
-// Four waves of 32 keys of one passage share tiles of 64 rows of Q and dO; while a tile is worked on the next one
+// Four waves of 32 keys each share tiles of 64 rows of Q and dO; while a tile is worked on the next one
 // arrives in LDS.  Each is read as rows for S and dP and transposed for dK and dV.  With P.splits > 1 the rows are dealt
 // to splits, which leave f32 parts of dK and dV.  K, V, dK and dV of 32 keys are 192 registers of 256, so operands are few
 // ahead, and the wait for LDS is what a wave mostly does besides products (48 % of the cycles): 480-500 us for 8 x 8 x 512
 // states of 128 bf16 columns, 75 % valid, 4,096 rows a key head, 820 TFLOP/s.
+// Tile `first` + wave of a batch entry's tiles of 32 keys.  At 128 columns those with valid keys come first, so that the
+// waves of a workgroup have keys whatever the lengths are: there two waves share a SIMD, and one without keys leaves half
+// of it idle (128 rows, 100 x 150 states, 62 % valid: dQ, dK and dV 640 us instead of 797).  At 64, where three to four
+// do, a workgroup takes 128 keys of one passage: finding a tile would cost more than the idle waves (258 us instead of
+// 245 for 100 x 100 states).
+constexpr bool deal_tiles(int64_t dim) { return dim > 64; }
+template <bool DEAL>
+__host__ __device__ __forceinline__ int key_tiles(int64_t len) { return (int)(DEAL ? (len + 31) / 32 : (len + 127) / 128 * 4); }
+struct KeyTile {
+    int p, j, n;   // passage (A.passages: none left), tile of it, its length
+    bool some;     // a wave of the workgroup has valid keys
+};
+template <bool DEAL>
+__device__ __forceinline__ KeyTile find_tile(const artread_attend_t& A, const AttendPlan& P, int64_t b, int per_passage,
+                                             int first, int wave) {
+    const int slot = first + wave, passages = (int)A.passages, len = (int)A.len;
+    const int32_t* lengths = A.lengths && !P.pack ? A.lengths + b * A.passages : nullptr;
+    if (!DEAL || !lengths) {
+        const int p = slot / per_passage, j = slot - p * per_passage;
+        int n = p < passages ? len : 0;
+        if (lengths && n) {
+            n = uniform(lengths[p]);
+            n = n < 0 ? 0 : (n < len ? n : len);
+        }
+        return KeyTile{p, j, n, lengths ? 32 * (j - wave) < n : true};
+    }
+    const int lane = threadIdx.x & 63;
+    int valid = 0, before = 0;
+#pragma unroll 1
+    for (int pass = 0; pass < 2; ++pass) {   // tiles with valid keys, then those without
+        before = pass ? valid : 0;
+        for (int p0 = 0; p0 < passages; p0 += 64) {
+            const int p = p0 + lane;
+            int n = p < passages ? lengths[p] : 0;
+            n = n < 0 ? 0 : (n < len ? n : len);
+            int c = (n + 31) >> 5;
+            if (pass) c = p < passages ? per_passage - c : 0;
+            int sum = c;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const int x = __shfl_up(sum, o);
+                if (lane >= o) sum += x;
+            }
+            const uint64_t behind = __ballot(before + sum > slot);
+            if (behind) {
+                const int l = __ffsll((unsigned long long)behind) - 1;
+                const int j = slot - (before + __builtin_amdgcn_readlane(sum - c, l));
+                const int m = __builtin_amdgcn_readlane(n, l);
+                return KeyTile{p0 + l, pass ? j + (per_passage - __builtin_amdgcn_readlane(c, l)) : j, m, !pass || first < valid};
+            }
+            before += __builtin_amdgcn_readlane(sum, 63);
+        }
+        if (!pass) valid = before;
+    }
+    return KeyTile{passages, 0, 0, first < valid};
+}
+
 template <typename T, int DP>
 __global__ __launch_bounds__(256, 2) void attend_grad_kv_kernel(artread_attend_t A, artread_attend_grads_t G,
                                                                   AttendPlan P, const RowStat* __restrict__ stats,
@@ -338,8 +395,10 @@ __global__ __launch_bounds__(256, 2) void attend_grad_kv_kernel(artread_attend_t
     typedef typename Mma<T>::V8 V8;
     const int lane = threadIdx.x & 63, half = lane >> 5, wave = uniform(threadIdx.x >> 6);
     const int dim = (int)A.dim;
-    const int64_t key_blocks = (A.len + 127) / 128;
-    const int64_t total = P.items * P.splits;   // batch x passages x key_blocks x kv_heads x splits
+    constexpr bool DEAL = deal_tiles(DP);
+    const int per_passage = key_tiles<DEAL>(A.len);
+    const int64_t groups = (A.passages * per_passage + 3) / 4;
+    const int64_t total = P.items * P.splits;   // batch x kv_heads x groups x splits
     const int64_t id = block_id();
     // Many rows: the workgroups of one key head stand together on an XCD, whose L2 then serves its rows.  Few:
     // the key heads of a state, neighbours in memory, are read side by side.
@@ -352,33 +411,27 @@ __global__ __launch_bounds__(256, 2) void attend_grad_kv_kernel(artread_attend_t
         kh = item % A.kv_heads;
         item /= A.kv_heads;
     }
-    const int64_t j0 = item % key_blocks * 128;
-    item /= key_blocks;
-    const int64_t p = item % A.passages;
-    item /= A.passages;
+    const int first = (int)(item % groups) * 4;
+    item /= groups;
     if (P.by_head) {
         kh = item % A.kv_heads;
         item /= A.kv_heads;
     }
     const int64_t b = item;
-    const int64_t j = j0 + 32 * wave + (lane & 31);
-    int n = (int)A.len;
-    bool key = j < n;   // this lane's
-    if (P.pack) {
+    const KeyTile at_tile = find_tile<DEAL>(A, P, b, per_passage, first, wave);
+    const int64_t p = at_tile.p, j1 = 32 * at_tile.j, j = j1 + (lane & 31);   // this lane's key
+    bool key = j < at_tile.n;   // never where no tile is left
+    if (P.pack && key) {
         Packed packed;
         packed.start(A, P, b);
         packed.ask((int)j);
         key = packed.valid();
-    } else if (A.lengths) {
-        const int x = uniform(A.lengths[b * A.passages + p]);
-        n = x < n ? x : n;
-        key = j < n;
     }
     f32x16 dk[DP / 32], dv[DP / 32];
     Spread<T> spread;
 #pragma unroll
     for (int db = 0; db < DP / 32; ++db) dk[db] = dv[db] = f32x16{};
-    if (j0 < n) {   // uniform over the workgroup
+    if (at_tile.some) {   // uniform over the workgroup
         V8 kf[DP / 16], vf[DP / 16];
         const T* kp = (const T*)A.k + b * A.k_batch + p * A.k_passage + j * A.k_row + kh * A.k_head + 8 * half;
         const T* vp = (const T*)A.v + b * A.v_batch + p * A.v_passage + j * A.v_row + kh * A.v_head + 8 * half;
@@ -493,8 +546,8 @@ __global__ __launch_bounds__(256, 2) void attend_grad_kv_kernel(artread_attend_t
     if (P.splits == 1) {
         __syncthreads();   // the tiles are read
         const uint32_t own = lds_offset(&qtile[0][0]) + (uint32_t)wave * 4096;
-        const int64_t j1 = j0 + 32 * wave, at = (((b * A.passages + p) * A.len + j1) * A.kv_heads + kh) * dim;
-        const int rows = A.len - j1 < 32 ? (int)(A.len - j1) : 32;
+        const int64_t at = (((b * A.passages + p) * A.len + j1) * A.kv_heads + kh) * dim;
+        const int rows = p >= A.passages ? 0 : (A.len - j1 < 32 ? (int)(A.len - j1) : 32);
         u32x4 w[DP / 16];
         turn_keys<T, DP>(dv, fv, key, own, lane, w);
         store_turned<T, DP>((T*)G.grad_v + at, A.kv_heads * dim, rows, dim, lane, w);
@@ -502,7 +555,7 @@ __global__ __launch_bounds__(256, 2) void attend_grad_kv_kernel(artread_attend_t
         store_turned<T, DP>((T*)G.grad_k + at, A.kv_heads * dim, rows, dim, lane, w);
         return;
     }
-    if (j >= A.len) return;
+    if (p >= A.passages || j >= A.len) return;
     const int64_t at = (((b * A.passages + p) * A.len + j) * A.kv_heads + kh) * dim;
 #pragma unroll
     for (int db = 0; db < DP / 32; ++db)

@@ -406,6 +406,22 @@ def test_attention_shared_heads_in_strided_rows(shape, dtype):
     assert all(torch.equal(x, y) for x, y in zip(got, want))
 
 
+@pytest.mark.parametrize("rows,dim", [(1, 128), (20, 64), (70, 128), (130, 64), (40, 128)])
+@pytest.mark.parametrize("passages,length", [(150, 40), (129, 63), (70, 70), (200, 33)])
+def test_attention_many_passages(passages, length, rows, dim):
+    """More passages than are looked at together, most of them empty for one batch entry, one behind the other and with
+    gaps between them."""
+    q, k, v, lengths, grad = attend_case(3, rows, passages, length, 2, 1, dim, BF16, seed=passages + rows)
+    lengths[0, 3:passages - 2] = 0
+    lengths[1] = 0
+    lengths[1, -1] = 1
+    check_attend(q, k, v, lengths, grad)
+    gaps = [torch.full((3, passages, length + 2, 1, dim), float("nan"), device="cuda", dtype=BF16) for _ in range(2)]
+    for wide, x in zip(gaps, (k, v)):
+        wide[:, :, 1:-1] = x
+    check_attend(q, gaps[0][:, :, 1:-1], gaps[1][:, :, 1:-1], lengths, grad)
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("rows", [1, 40, 200])
 @pytest.mark.parametrize("step", [0.002, 0.03, -0.03, 2.0])
