@@ -212,7 +212,7 @@ __device__ __forceinline__ void ahead() {
 // 880-940 TFLOP/s with the second term's products, which run in 54 % of the cycles.  Four waves; for up to 64 rows one
 // wave a workgroup, since the others would have none.
 template <typename T, int DP, int NW, int KB>
-__global__ __launch_bounds__(64 * NW, 2) void attend_grad_q_kernel(artread_attend_t A, artread_attend_grads_t G,
+__global__ __launch_bounds__(64 * NW, DP == 64 ? 3 : 2) void attend_grad_q_kernel(artread_attend_t A, artread_attend_grads_t G,
                                                                     AttendPlan P, const RowStat* __restrict__ stats,
                                                                     float* __restrict__ part) {
     constexpr int TILE = 32 * KB * DP;
