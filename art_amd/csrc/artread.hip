@@ -503,8 +503,7 @@ static GradShape grad_shape(const artread_attend_t* given) {
     AttendPlan& K = S.kv;
     K.row_blocks = 1;
     K.by_head = K.row_count > 64;
-    const int64_t key_tiles_each = deal_tiles(a->dim) ? key_tiles<true>(a->len) : key_tiles<false>(a->len);
-    K.items = a->batch * a->kv_heads * ((a->passages * key_tiles_each + 3) / 4);
+    K.items = a->batch * a->kv_heads * ((a->passages * ((a->len + 31) / 32) + 3) / 4);
     want = (512 + K.items - 1) / K.items;
     most = (K.row_count + 63) / 64 / 2;
     want = want < most ? want : most;

@@ -330,12 +330,9 @@ __global__ __launch_bounds__(64 * NW, DP == 64 ? 3 : 2) void attend_grad_q_kerne
 // states of 128 bf16 columns, 75 % valid, 4,096 rows a key head, 820 TFLOP/s.
 // Tile `first` + wave of a batch entry's tiles of 32 keys.  At 128 columns those with valid keys come first, so that the
 // waves of a workgroup have keys whatever the lengths are: there two waves share a SIMD, and one without keys leaves half
-// of it idle (128 rows, 100 x 150 states, 62 % valid: dQ, dK and dV 640 us instead of 797).  At 64, where three to four
-// do, a workgroup takes 128 keys of one passage: finding a tile would cost more than the idle waves (258 us instead of
-// 245 for 100 x 100 states).
-constexpr bool deal_tiles(int64_t dim) { return dim > 64; }
-template <bool DEAL>
-__host__ __device__ __forceinline__ int key_tiles(int64_t len) { return (int)(DEAL ? (len + 31) / 32 : (len + 127) / 128 * 4); }
+// of it idle (128 rows, 100 x 150 states, 62 % valid: dQ, dK and dV 640 us instead of 797 with four tiles of one passage a
+// workgroup).  At 64, where three do, finding such a tile costs as much as the idle waves (244 us instead of 239 for 128
+// rows, 100 x 100 states): they are taken in the order they have in memory.
 struct KeyTile {
     int p, j, n;   // passage (A.passages: none left), tile of it, its length
     bool some;     // a wave of the workgroup has valid keys
@@ -345,16 +342,15 @@ __device__ __forceinline__ KeyTile find_tile(const artread_attend_t& A, const At
                                              int first, int wave) {
     const int slot = first + wave, passages = (int)A.passages, len = (int)A.len;
     const int32_t* lengths = A.lengths && !P.pack ? A.lengths + b * A.passages : nullptr;
-    if (!DEAL || !lengths) {
-        const int p = slot / per_passage, j = slot - p * per_passage;
-        int n = p < passages ? len : 0;
-        if (lengths && n) {
-            n = uniform(lengths[p]);
-            n = n < 0 ? 0 : (n < len ? n : len);
-        }
-        return KeyTile{p, j, n, lengths ? 32 * (j - wave) < n : true};
-    }
     const int lane = threadIdx.x & 63;
+    if (!DEAL || !lengths) {   // the lanes look at one tile each
+        const int p = (first + (lane & 3)) / per_passage, j = first + (lane & 3) - p * per_passage;
+        int n = p < passages ? len : 0;
+        if (lengths && p < passages) n = lengths[p];
+        n = n < 0 ? 0 : (n < len ? n : len);
+        const bool some = __any(32 * j < n);
+        return KeyTile{__builtin_amdgcn_readlane(p, wave), __builtin_amdgcn_readlane(j, wave), __builtin_amdgcn_readlane(n, wave), some};
+    }
     int valid = 0, before = 0;
 #pragma unroll 1
     for (int pass = 0; pass < 2; ++pass) {   // tiles with valid keys, then those without
@@ -395,8 +391,7 @@ __global__ __launch_bounds__(256, 2) void attend_grad_kv_kernel(artread_attend_t
     typedef typename Mma<T>::V8 V8;
     const int lane = threadIdx.x & 63, half = lane >> 5, wave = uniform(threadIdx.x >> 6);
     const int dim = (int)A.dim;
-    constexpr bool DEAL = deal_tiles(DP);
-    const int per_passage = key_tiles<DEAL>(A.len);
+    const int per_passage = (int)((A.len + 31) / 32);
     const int64_t groups = (A.passages * per_passage + 3) / 4;
     const int64_t total = P.items * P.splits;   // batch x kv_heads x groups x splits
     const int64_t id = block_id();
@@ -418,7 +413,7 @@ __global__ __launch_bounds__(256, 2) void attend_grad_kv_kernel(artread_attend_t
         item /= A.kv_heads;
     }
     const int64_t b = item;
-    const KeyTile at_tile = find_tile<DEAL>(A, P, b, per_passage, first, wave);
+    const KeyTile at_tile = find_tile<DP == 128>(A, P, b, per_passage, first, wave);
     const int64_t p = at_tile.p, j1 = 32 * at_tile.j, j = j1 + (lane & 31);   // this lane's key
     bool key = j < at_tile.n;   // never where no tile is left
     if (P.pack && key) {
