@@ -208,8 +208,8 @@ __device__ __forceinline__ void ahead() {
 // ---- dQ: the row walk -----------------------------------------------------------------------------------
 // NW waves of 32 rows share tiles of 32 * KB keys; while a tile is worked on the next one arrives in LDS.  With
 // P.splits > 1 each split leaves its f32 part of dQ at part + split * (all of dQ).  Bound by the matrix units and what
-// stands between their products: 8 x 8 x 512 states of 128 bf16 columns, 75 % valid, 4,096 rows a key head in 437-470 us,
-// 880-940 TFLOP/s with the second term's products, which run in 54 % of the cycles.  Four waves; for up to 64 rows one
+// stands between their products: 8 x 8 x 512 states of 128 bf16 columns, 75 % valid, 4,096 rows a key head in 440-460 us,
+// 900-940 TFLOP/s with the second term's products; a product runs in 52 % of the cycles.  Four waves; for up to 64 rows one
 // wave a workgroup, since the others would have none.
 template <typename T, int DP, int NW, int KB>
 __global__ __launch_bounds__(64 * NW, DP == 64 ? 3 : 2) void attend_grad_q_kernel(artread_attend_t A, artread_attend_grads_t G,
@@ -280,6 +280,16 @@ __global__ __launch_bounds__(64 * NW, DP == 64 ? 3 : 2) void attend_grad_q_kerne
                 s = Mma<T>::mul(lds_rows<T, DP>(krow, kb, k), q[k], s);
                 dp = Mma<T>::mul(lds_rows<T, DP>(krow, 2 * KB + kb, k), g[k], dp);
             }
+            if constexpr (DP == 128) {   // LDS reads eight products ahead: 1 to 3 % at 4,096 rows
+                __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
+#pragma unroll
+                for (int k = 0; k < DP / 8 - 8; ++k) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                }
+                __builtin_amdgcn_sched_group_barrier(0x008, 8, 0);
+                __builtin_amdgcn_sched_barrier(0);
+            }
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], P.c, -st.x)) * (dp[i] - st.delta);
             if (!whole_tile<KB>(mask)) {
@@ -326,8 +336,8 @@ __global__ __launch_bounds__(64 * NW, DP == 64 ? 3 : 2) void attend_grad_q_kerne
 // Four waves of 32 keys each share tiles of 64 rows of Q and dO; while a tile is worked on the next one
 // arrives in LDS.  Each is read as rows for S and dP and transposed for dK and dV.  With P.splits > 1 the rows are dealt
 // to splits, which leave f32 parts of dK and dV.  K, V, dK and dV of 32 keys are 192 registers of 256, so operands are few
-// ahead, and the wait for LDS is what a wave mostly does besides products (48 % of the cycles): 480-500 us for 8 x 8 x 512
-// states of 128 bf16 columns, 75 % valid, 4,096 rows a key head, 820 TFLOP/s.
+// ahead, and the wait for LDS is what a wave mostly does besides products (48 % of the cycles): 455-490 us for 8 x 8 x 512
+// states of 128 bf16 columns, 75 % valid, 4,096 rows a key head, 840-910 TFLOP/s.
 // Tile `first` + wave of a batch entry's tiles of 32 keys.  At 128 columns those with valid keys come first, so that the
 // waves of a workgroup have keys whatever the lengths are: there two waves share a SIMD, and one without keys leaves half
 // of it idle (128 rows, 100 x 150 states, 62 % valid: dQ, dK and dV 640 us instead of 797 with four tiles of one passage a
