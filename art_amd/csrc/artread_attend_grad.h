@@ -342,7 +342,9 @@ __global__ __launch_bounds__(64 * NW, DP == 64 ? 3 : 2) void attend_grad_q_kerne
 // waves of a workgroup have keys whatever the lengths are: there two waves share a SIMD, and one without keys leaves half
 // of it idle (128 rows, 100 x 150 states, 62 % valid: dQ, dK and dV 640 us instead of 797 with four tiles of one passage a
 // workgroup).  At 64, where three do, finding such a tile costs as much as the idle waves (244 us instead of 239 for 128
-// rows, 100 x 100 states): they are taken in the order they have in memory.
+// rows, 100 x 100 states): they are taken in the order they have in memory, as they are where a batch entry has more than
+// kDealPassages of them, since every workgroup looks at their lengths.
+constexpr int kDealPassages = 1024;
 struct KeyTile {
     int p, j, n;   // passage (A.passages: none left), tile of it, its length
     bool some;     // a wave of the workgroup has valid keys
@@ -353,7 +355,7 @@ __device__ __forceinline__ KeyTile find_tile(const artread_attend_t& A, const At
     const int slot = first + wave, passages = (int)A.passages, len = (int)A.len;
     const int32_t* lengths = A.lengths && !P.pack ? A.lengths + b * A.passages : nullptr;
     const int lane = threadIdx.x & 63;
-    if (!DEAL || !lengths) {   // the lanes look at one tile each
+    if (!DEAL || !lengths || passages > kDealPassages) {   // the lanes look at one tile each
         const int p = (first + (lane & 3)) / per_passage, j = first + (lane & 3) - p * per_passage;
         int n = p < passages ? len : 0;
         if (lengths && p < passages) n = lengths[p];

@@ -407,7 +407,7 @@ def test_attention_shared_heads_in_strided_rows(shape, dtype):
 
 
 @pytest.mark.parametrize("rows,dim", [(1, 128), (20, 64), (70, 128), (130, 64), (40, 128)])
-@pytest.mark.parametrize("passages,length", [(150, 40), (129, 63), (70, 70), (200, 33)])
+@pytest.mark.parametrize("passages,length", [(150, 40), (129, 63), (70, 70), (200, 33), (1100, 33)])
 def test_attention_many_passages(passages, length, rows, dim):
     """More passages than are looked at together, most of them empty for one batch entry, one behind the other and with
     gaps between them."""
