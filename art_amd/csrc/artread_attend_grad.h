@@ -624,9 +624,12 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_grad_stream_kernel(artread_
         *(V8*)(qtile + at) = load8<T>((const T*)A.q + b * A.q_batch + t * A.q_row + h * A.q_head + 8 * chunk, ok);
         *(V8*)(gtile + at) = load8<T>((const T*)G.grad_out + b * G.g_batch + t * G.g_row + h * G.g_head + 8 * chunk, ok);
     }
-    if (dim < DP)   // the columns behind dim of the wave's own tiles
+    if (dim < DP) {   // the columns behind dim of the wave's own tiles
         for (int i = lane; i < 2 * TILE / 8; i += 64)
             *(__attribute__((address_space(3))) u32x4*)(uintptr_t)(mine + i * 16) = u32x4{0, 0, 0, 0};
+        // loads from memory to LDS do not wait for the wave's LDS stores: the first tile's come to the same places
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
     RowStat st[RB];
     f32x16 dq[RB][DP / 32];
     Spread<T> spread_q[RB];

@@ -3,6 +3,8 @@ reach a GPU."""
 import ctypes
 import os
 import re
+import struct
+import subprocess
 
 import pytest
 import torch
@@ -231,3 +233,47 @@ def test_c_attend_grad_refuses():
     assert lib.artread_attend_grad(0, ctypes.byref(no_lse), ctypes.byref(g), SOME, need, None) == -1
     assert lib.artread_attend(0, None, None, 0, None) == -1
     assert lib.artread_attend_workspace(None) == -1
+
+
+# ---- what was compiled ------------------------------------------------------------------------------
+OBJDUMP = "/opt/rocm/llvm/bin/llvm-objdump"
+
+
+def _gpu_code(tmp_path):
+    """{kernel: instructions} of the built library's gfx950 code."""
+    with open(rd.READ_LIB_PATH, "rb") as f:
+        data = f.read()
+    at = data.index(b"__CLANG_OFFLOAD_BUNDLE__")
+    (count,), place = struct.unpack_from("<Q", data, at + 24), at + 32
+    for _ in range(count):
+        offset, size, chars = struct.unpack_from("<QQQ", data, place)
+        target = data[place + 24:place + 24 + chars]
+        place += 24 + chars
+        if target.endswith(b"gfx950"):
+            code = tmp_path / "artread.co"
+            code.write_bytes(data[at + offset:at + offset + size])
+    text = subprocess.run([OBJDUMP, "-d", str(code)], check=True, capture_output=True, text=True).stdout
+    kernels, name = {}, None
+    for line in text.splitlines():
+        head = re.match(r"[0-9a-f]+ <(.*)>:", line)
+        if head:
+            name = head.group(1)
+            kernels[name] = []
+        elif name and line.startswith("\t"):
+            kernels[name].append(line.split("//")[0].strip())
+    return kernels
+
+
+@pytest.mark.skipif(not os.path.exists(OBJDUMP), reason="no disassembler")
+def test_cleared_tiles_are_settled_before_memory_is_loaded_into_them(tmp_path):
+    """The few-row gradient clears the wave's own tiles by LDS stores and then loads memory into them: loads to LDS do
+    not wait for LDS stores by themselves, so a wait for all of these stands between the two."""
+    seen = 0
+    for name, code in _gpu_code(tmp_path).items():
+        if "attend_grad_stream_kernel" not in name:
+            continue
+        seen += 1
+        load = next(i for i, x in enumerate(code) if x.startswith("global_load_lds"))
+        store = max(i for i, x in enumerate(code[:load]) if x.startswith("ds_write"))
+        assert any(re.match(r"s_waitcnt lgkmcnt\(0\)$", x) for x in code[store:load]), name
+    assert seen == 12

@@ -692,3 +692,15 @@ def test_gpu_refusals():
         rd.embed_tokens(tokens, table, lens.cpu())
     with pytest.raises(ValueError):
         rd.embed_tokens_grad(torch.zeros((2, 3, 8), device="cuda", dtype=F16), tokens.cpu(), 5)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("rows", [2, 25, 60])
+@pytest.mark.parametrize("dim", range(8, 129, 8))
+def test_attention_gradient_of_few_rows_at_every_head_size(dim, rows, dtype):
+    """Columns behind the head size are cleared in LDS before the first tile comes to it, which is whole for one batch
+    entry, part of a tile for another and empty for a third."""
+    q, k, v, lengths, grad = attend_case(3, rows, 6, 70, 2, 2, dim, dtype, seed=dim + rows)
+    lengths[0], lengths[1, ::2], lengths[2, 0] = 70, 5, 0
+    check_attend(q, k, v, lengths, grad)
+    check_attend(q, k, v, None, grad)
