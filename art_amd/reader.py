@@ -12,6 +12,8 @@ call allocates its outputs and workspace from torch's allocator on that stream, 
 next call and never waits for the host, so it may be captured into a graph.  To capture gradients, use
 ``cross_attention_grad`` and ``embed_tokens_grad``: autograd's own bookkeeping of leaves that are
 shared with an eager graph does not survive a capture.
+
+Derivatives are reverse-mode only: tensors with a forward-mode tangent are refused, since the call would drop it.
 """
 import ctypes
 import math
@@ -19,6 +21,7 @@ import os
 import struct
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from .engine import _on_device
@@ -94,7 +97,12 @@ def _rcheck(rc):
 
 
 def _one_device(first, *others):
-    """Every tensor of a call lives on one GPU: the kernels read them all by address."""
+    """Every tensor of a call lives on one GPU: the kernels read them all by address.  What torch would keep
+    beside a tensor's values, and a call by address would lose, is refused first."""
+    if forward_ad._current_level >= 0:   # inside a dual level
+        for t in (first, *others):
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError("forward-mode derivatives are not implemented: a tensor has a tangent")
     if not first.is_cuda:
         raise ValueError("tensors must be on a GPU, got %s" % first.device)
     for t in others:
@@ -179,6 +187,7 @@ class _EmbedTokens(torch.autograd.Function):
     def backward(ctx, grad_out):
         tokens, lengths = ctx.saved_tensors
         vocab, scale, vocab_base, dtype = ctx.of
+        _one_device(grad_out, tokens, lengths)
         return _embed_grad(grad_out, tokens, lengths, vocab, scale, vocab_base, dtype), None, None, None, None, None
 
 

@@ -141,6 +141,30 @@ def test_cross_attention_grad_refuses(kwargs):
         rd.cross_attention_grad(**args)
 
 
+@pytest.mark.parametrize("which", ["table", "query", "key", "value", "grad_out", "embed grad_out", "out", "rest"])
+def test_forward_mode_tangents_are_refused(which):
+    """A call by address sees a dual tensor's values only: its tangent would be gone from the result."""
+    forward_ad = torch.autograd.forward_ad
+
+    def call(dual):
+        if which == "table":
+            return rd.embed_tokens(TOKENS, dual(TABLE), LENS)
+        if which == "embed grad_out":
+            return rd.embed_tokens_grad(dual(torch.zeros((3, 5, 8), dtype=torch.float16)), TOKENS, 7, LENS)
+        args = dict(query=Q, key=K, value=K, lengths=KL)
+        if which in args:
+            args[which] = dual(args[which])
+            return rd.cross_attention(**args)
+        return rd.cross_attention_grad(dual(Q) if which == "grad_out" else Q, out=dual(Q) if which == "out" else Q,
+                                       saved=(LSE, dual(Q) if which == "rest" else Q), **args)
+
+    with forward_ad.dual_level():
+        with pytest.raises(NotImplementedError):
+            call(lambda t: forward_ad.make_dual(t, torch.ones_like(t)))
+        with pytest.raises(ValueError):   # without a tangent: on past it, to the tensors' place
+            call(lambda t: t)
+
+
 # ---- the C entry points: refused before the device is even looked at -------------------------------
 SOME = 4096  # an address that is never followed
 

@@ -704,3 +704,22 @@ def test_attention_gradient_of_few_rows_at_every_head_size(dim, rows, dtype):
     lengths[0], lengths[1, ::2], lengths[2, 0] = 70, 5, 0
     check_attend(q, k, v, lengths, grad)
     check_attend(q, k, v, None, grad)
+
+
+def test_forward_mode_is_refused_in_the_backward_pass_too():
+    """Forward over reverse: the tangent of the result's gradient."""
+    q, k, v, lengths, grad = attend_case(2, 3, 2, 5, 2, 2, 16, F16, 55)
+    tokens, lens, table = embed_case(3, 5, 11, 8, F32, 56)
+    forward_ad = torch.autograd.forward_ad
+    calls = [(lambda x: rd.cross_attention(x, k, v, lengths), q, grad),
+             (lambda x: rd.embed_tokens(tokens, x, lens), table, torch.ones((3, 5, 8), device="cuda"))]
+    for call, leaf, weight in calls:
+        leaf.requires_grad_()
+        y = call(leaf)
+        with forward_ad.dual_level():
+            dual = forward_ad.make_dual(weight, torch.ones_like(weight))
+            with pytest.raises(NotImplementedError):
+                torch.autograd.grad(y, leaf, dual)
+            with pytest.raises(NotImplementedError):
+                call(forward_ad.make_dual(leaf, torch.ones_like(leaf)))
+        assert torch.autograd.grad(call(leaf), leaf, weight)[0].shape == leaf.shape
