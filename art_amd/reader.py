@@ -14,6 +14,7 @@ next call and never waits for the host, so it may be captured into a graph.  To 
 shared with an eager graph does not survive a capture.
 
 Derivatives are reverse-mode only: tensors with a forward-mode tangent are refused, since the call would drop it.
+So are calls under ``torch.jit.trace`` and ``make_fx``, which would record the outputs and not what fills them.
 """
 import ctypes
 import math
@@ -23,6 +24,7 @@ import struct
 import torch
 from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
+from torch.fx.experimental.proxy_tensor import get_proxy_mode
 
 from .engine import _on_device
 
@@ -103,6 +105,8 @@ def _one_device(first, *others):
         for t in (first, *others):
             if t is not None and forward_ad.unpack_dual(t).tangent is not None:
                 raise NotImplementedError("forward-mode derivatives are not implemented: a tensor has a tangent")
+    if torch.jit.is_tracing() or torch._C._len_torch_dispatch_stack() and get_proxy_mode() is not None:
+        raise NotImplementedError("a traced graph would hold the outputs' allocation but not the call that fills them")
     if not first.is_cuda:
         raise ValueError("tensors must be on a GPU, got %s" % first.device)
     for t in others:

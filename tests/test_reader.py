@@ -8,6 +8,7 @@ import subprocess
 
 import pytest
 import torch
+from torch.fx.experimental.proxy_tensor import make_fx
 
 from art_amd import reader as rd
 
@@ -163,6 +164,26 @@ def test_forward_mode_tangents_are_refused(which):
             call(lambda t: forward_ad.make_dual(t, torch.ones_like(t)))
         with pytest.raises(ValueError):   # without a tangent: on past it, to the tensors' place
             call(lambda t: t)
+
+
+CALLS = {
+    "embed_tokens": (lambda t, w: rd.embed_tokens(t, w), (TOKENS, TABLE)),
+    "embed_tokens_grad": (lambda g, t: rd.embed_tokens_grad(g, t, 7), (torch.zeros((3, 5, 8)), TOKENS)),
+    "cross_attention": (lambda q, k: rd.cross_attention(q, k, k), (Q, K)),
+    "cross_attention_grad": (lambda q, k: rd.cross_attention_grad(q, q, k, k, q, (LSE, q)), (Q, K)),
+}
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_tracing_is_refused(name):
+    """A recorded graph would hold the allocation of the outputs and no call: its replay would return what is in memory."""
+    call, args = CALLS[name]
+    with pytest.raises(NotImplementedError):
+        torch.jit.trace(call, args, check_trace=False)
+    with pytest.raises(NotImplementedError):
+        make_fx(call)(*args)
+    with pytest.raises(ValueError):   # not traced: on past it, to the tensors' place
+        call(*args)
 
 
 # ---- the C entry points: refused before the device is even looked at -------------------------------
