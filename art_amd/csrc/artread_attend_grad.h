@@ -617,12 +617,14 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_grad_stream_kernel(artread_
     const int64_t bk = id / P.splits, kh = bk % A.kv_heads, b = bk / A.kv_heads;
     for (int i = threadIdx.x; i < RB * 32 * CH; i += 64 * NW) {
         const int row = i / CH, chunk = i % CH;
+        // rows that are not there have no weight and no gradient; their scores repeat the last row's, since those of zeros
+        // would be NaN for an infinite key that every row does without
+        const bool there = row < P.row_count;
         int64_t t, h;
-        split_row(P, kh, (uint32_t)row, &t, &h);
-        const bool ok = row < P.row_count && 8 * chunk < dim;
+        split_row(P, kh, there ? (uint32_t)row : (uint32_t)(P.row_count - 1), &t, &h);
         const int at = row * DP + tile_chunk<DP>(row, chunk) * 8;
-        *(V8*)(qtile + at) = load8<T>((const T*)A.q + b * A.q_batch + t * A.q_row + h * A.q_head + 8 * chunk, ok);
-        *(V8*)(gtile + at) = load8<T>((const T*)G.grad_out + b * G.g_batch + t * G.g_row + h * G.g_head + 8 * chunk, ok);
+        *(V8*)(qtile + at) = load8<T>((const T*)A.q + b * A.q_batch + t * A.q_row + h * A.q_head + 8 * chunk, 8 * chunk < dim);
+        *(V8*)(gtile + at) = load8<T>((const T*)G.grad_out + b * G.g_batch + t * G.g_row + h * G.g_head + 8 * chunk, there && 8 * chunk < dim);
     }
     if (dim < DP) {   // the columns behind dim of the wave's own tiles
         for (int i = lane; i < 2 * TILE / 8; i += 64)

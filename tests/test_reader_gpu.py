@@ -723,3 +723,28 @@ def test_forward_mode_is_refused_in_the_backward_pass_too():
             with pytest.raises(NotImplementedError):
                 call(forward_ad.make_dual(leaf, torch.ones_like(leaf)))
         assert torch.autograd.grad(call(leaf), leaf, weight)[0].shape == leaf.shape
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("rows", [1, 40, 200])
+def test_attention_infinities_among_valid_keys(rows, dtype):
+    """An infinite element of a key: rows whose score it makes -inf do without that key, those it makes inf have NaN."""
+    q, k, v, _, grad = attend_case(3, rows, 2, 70, 2, 1, 64, dtype, 61, q_std=0.5)
+    lengths = torch.tensor([[70, 34], [70, 34], [70, 34]], device="cuda", dtype=torch.int32)
+    q[0, ..., 3], q[1, ..., 3], q[2, ..., 3] = -1.0, 1.0, 0.5
+    k[:2, 1, 33, 0, 3] = float("inf")
+    shorter = torch.tensor([[70, 33], [70, 33], [70, 34]], device="cuda", dtype=torch.int32)
+    want = attend_ref(q, torch.where(torch.isinf(k), 0.0, k), v, shorter, grad)   # that key is behind the length there
+    out, saved = rd.cross_attention(q, k, v, lengths, return_saved=True)
+    got = rd.cross_attention_grad(grad, q, k, v, out, saved, lengths)
+    fine = [0, 2]
+    within(out[fine], *(x[fine] for x in want["out"]))
+    within(saved[0][fine], *(x[fine] for x in want["lse"]))
+    assert bool(torch.isnan(out[1]).all()) and bool(torch.isnan(saved[0][1]).all())
+    assert all(bool(torch.isnan(x[1]).all()) for x in (got[0], got[1][:, :1, :34], got[2][:, :1, :34]))
+    within(got[1][fine], *(x[fine] for x in want["dk"]))
+    within(got[2][fine], *(x[fine] for x in want["dv"]))
+    others = [d for d in range(64) if d != 3]   # 0 * inf in that column of the rows' gradients
+    assert bool(torch.isnan(got[0][0, ..., 3]).all())
+    within(got[0][fine][..., others], *(x[fine][..., others] for x in want["dq"]))
+    within(got[0][2], *(x[2] for x in want["dq"]))
