@@ -725,6 +725,91 @@ def test_forward_mode_is_refused_in_the_backward_pass_too():
         assert torch.autograd.grad(call(leaf), leaf, weight)[0].shape == leaf.shape
 
 
+# ---- rows, layouts, values and sizes that stand alone ---------------------------------------------------
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("rows", [2, 40, 200])
+def test_attention_a_row_depends_on_itself_alone(rows, dtype):
+    """One row kept while its neighbours, their maxima and their gradients change: its bits stay."""
+    q, k, v, lengths, grad = attend_case(2, rows, 3, 90, 2, 1, 64, dtype, 57)
+    k[..., 0] = (torch.arange(270, device="cuda").view(3, 90, 1) * 0.03).to(dtype)   # maxima that rise along the keys
+    keep = rows // 2
+    results = []
+    for seed, std in ((1, 0.1), (2, 4.0)):
+        other = (torch.randn(q.shape, device="cuda", generator=gen(seed)) * std).to(dtype)
+        other[:, keep] = q[:, keep]
+        g = (torch.randn(q.shape, device="cuda", generator=gen(seed + 10)) * std).to(dtype)
+        g[:, keep] = grad[:, keep]
+        out, saved = rd.cross_attention(other, k, v, lengths, return_saved=True)
+        results.append((out[:, keep], saved[0][:, :, keep], saved[1][:, keep],
+                        rd.cross_attention_grad(g, other, k, v, out, saved, lengths)[0][:, keep]))
+    assert all(torch.equal(x, y) for x, y in zip(*results))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("rows,dim", [(1, 64), (40, 64), (200, 64), (20, 128), (50, 128), (200, 128), (70, 40)])
+@pytest.mark.parametrize("length,with_lengths", [(1, True), (7, True), (31, True), (32, True), (7, False), (50, False)])
+def test_attention_short_passages_one_behind_the_other_and_with_gaps(length, with_lengths, rows, dim, dtype):
+    """Passages that lie one behind the other may share tiles, those with gaps between them cannot: the same results
+    within the same bounds, though not the same bits."""
+    q, k, v, lengths, grad = attend_case(2, rows, 20, length, 2, 1, dim, dtype, seed=58 + length)
+    lengths = lengths if with_lengths else None
+    check_attend(q, k, v, lengths, grad)
+    gaps = [torch.full((2, 20, length + 3, 1, dim), float("nan"), device="cuda", dtype=dtype) for _ in range(2)]
+    for wide, x in zip(gaps, (k, v)):
+        wide[:, :, 1:1 + length] = x
+    k, v = gaps[0][:, :, 1:1 + length], gaps[1][:, :, 1:1 + length]
+    ref = attend_ref(q, k, v, lengths, grad)
+    leaves = [x.detach().requires_grad_() for x in (q, k, v)]   # no copies: those would close the gaps
+    out = rd.cross_attention(*leaves, lengths)
+    within(out, *ref["out"])
+    within(rd.cross_attention(q, k, v, lengths, return_lse=True)[1], *ref["lse"])
+    got = torch.autograd.grad(out, leaves, grad)
+    for name, x in zip(("dq", "dk", "dv"), got):
+        within(x, *ref[name])
+    held, saved = rd.cross_attention(q, k, v, lengths, return_saved=True)
+    assert torch.equal(held, out)
+    again = rd.cross_attention_grad(grad, q, k, v, held, saved, lengths)
+    assert all(torch.equal(x, y) for x, y in zip(got, again))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("std", [30.0, 120.0])
+@pytest.mark.parametrize("rows", [1, 40, 200])
+def test_attention_gradients_of_large_scores(rows, std, dtype):
+    """Weights made anew from a log-sum of hundreds: its 32 bits are what their precision hangs on."""
+    q, k, v, lengths, grad = attend_case(2, rows, 2, 90, 2, 2, 64, dtype, 59, q_std=std)
+    check_attend(q, k, v, lengths, grad)
+    check_attend(q, k, v, None, grad)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("rows", [1, 40, 200])
+@pytest.mark.parametrize("value", [float("inf"), -float("inf"), float("nan")])
+def test_attention_infinities_and_nan_among_valid_values(value, rows, dtype):
+    """One element of one valid state's value: its column of its key head's rows has it, nothing else changes, and the
+    gradients that need it have none for that head."""
+    q, k, v, _, grad = attend_case(3, rows, 4, 70, 4, 2, 64, dtype, 60, q_std=0.3)
+    lengths = torch.tensor([[70, 9, 0, 33], [70, 9, 0, 33], [1, 2, 3, 64]], device="cuda", dtype=torch.int32)
+    clean, saved = rd.cross_attention(q, k, v, lengths, return_saved=True)
+    grads = rd.cross_attention_grad(grad, q, k, v, clean, saved, lengths)
+    v[1, 3, 20, 1, 5] = value   # read by heads 2 and 3
+    out, saved2 = rd.cross_attention(q, k, v, lengths, return_saved=True)
+    got = rd.cross_attention_grad(grad, q, k, v, out, saved2, lengths)
+    hit = torch.zeros(q.shape, dtype=torch.bool, device="cuda")
+    hit[1, :, 2:, 5] = True
+    same = torch.isnan(out[hit]) if math.isnan(value) else out[hit] == value
+    assert bool(same.all()) and torch.equal(out[~hit], clean[~hit]) and torch.equal(saved2[0], saved[0])
+    rows_hit = torch.zeros(q.shape, dtype=torch.bool, device="cuda")
+    rows_hit[1, :, 2:] = True
+    inside = (torch.arange(70, device="cuda") < lengths[..., None])[..., None, None].expand(k.shape)
+    states_hit = torch.zeros(k.shape, dtype=torch.bool, device="cuda")
+    states_hit[1, :, :, 1] = True
+    states_hit &= inside
+    assert bool(torch.isnan(got[0][rows_hit]).all()) and torch.equal(got[0][~rows_hit], grads[0][~rows_hit])
+    assert bool(torch.isnan(got[1][states_hit]).all()) and torch.equal(got[1][~states_hit], grads[1][~states_hit])
+    assert torch.equal(got[2], grads[2])
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("rows", [1, 40, 200])
 def test_attention_infinities_among_valid_keys(rows, dtype):
@@ -748,3 +833,67 @@ def test_attention_infinities_among_valid_keys(rows, dtype):
     assert bool(torch.isnan(got[0][0, ..., 3]).all())
     within(got[0][fine][..., others], *(x[fine][..., others] for x in want["dq"]))
     within(got[0][2], *(x[2] for x in want["dq"]))
+
+
+@pytest.mark.parametrize("rows", [1, 70])
+def test_attention_gradient_offsets_past_32_bits(rows):
+    """States and gradients of more than 2^31 elements, a few of them valid at both ends."""
+    passages, length, heads, dim = 33, 1 << 16, 8, 128
+    g = gen(62)
+    states = torch.zeros((1, passages, length, heads, dim), device="cuda", dtype=BF16)
+    assert states.numel() > 1 << 31
+    q, grad = (torch.randn((1, rows, heads, dim), device="cuda", generator=g).to(BF16) for _ in range(2))
+    lengths = torch.zeros((1, passages), device="cuda", dtype=torch.int32)
+    ends = ((0, 3), (passages - 1, 100))
+    small = torch.zeros((1, 2, 100, heads, dim), device="cuda", dtype=BF16)
+    for i, (p, n) in enumerate(ends):
+        lengths[0, p] = n
+        states[0, p, :n] = small[0, i, :n] = torch.randn((n, heads, dim), device="cuda", generator=g).to(BF16)
+    ref = attend_ref(q, small, small, torch.tensor([[3, 100]], device="cuda", dtype=torch.int32), grad)
+    out, saved = rd.cross_attention(q, states, states, lengths, return_saved=True)
+    got = rd.cross_attention_grad(grad, q, states, states, out, saved, lengths)
+    within(out, *ref["out"])
+    within(got[0], *ref["dq"])
+    for x, name in zip(got[1:], ("dk", "dv")):
+        for i, (p, n) in enumerate(ends):
+            within(x[0, p, :n], *(y[0, i, :n] for y in ref[name]))
+            x[0, p, :n] = 0
+        assert int(x.count_nonzero()) == 0
+
+
+def test_embed_and_gradient_past_32_bits():
+    """Results and gradients of more than 2^31 elements, and a table of as many."""
+    n, length, dim, vocab = 2100, 1000, 1024, 50
+    tokens, lengths, table = embed_case(n, length, vocab, dim, BF16, 63)
+    lengths[-1] = length
+    out = rd.embed_tokens(tokens, table, lengths)
+    assert out.numel() > 1 << 31
+    for i in (0, n // 2, n - 1):
+        assert torch.equal(out[i], embed_ref(tokens[i:i + 1], lengths[i:i + 1], table, 1.0)[0].to(BF16))
+    few = torch.where(torch.arange(n, device="cuda") % 300 == 299, lengths, 0).int()   # the last row is one of them
+    assert int(few[-1]) == length
+    d = rd.embed_tokens_grad(out, tokens, vocab, few)
+    some = torch.arange(299, n, 300, device="cuda")
+    ref = grad_ref(out[some], tokens[some], few[some], vocab, 1.0)
+    within(d, ref[0], grad_bound(*ref, BF16))
+    del out
+    vocab = 2_200_000
+    big = torch.zeros((vocab, dim), device="cuda", dtype=BF16)
+    big[-1], big[7] = 3.0, 2.0
+    ids = torch.tensor([[vocab - 1, 7, 0, vocab - 2]], device="cuda", dtype=torch.int64)
+    assert rd.embed_tokens(ids, big)[0, :, -1].tolist() == [3.0, 2.0, 0.0, 0.0]
+    d = rd.embed_tokens_grad(torch.ones((1, 4, dim), device="cuda", dtype=BF16), ids, vocab)
+    assert int(d.count_nonzero()) == 4 * dim and bool((d[ids[0]] == 1.0).all())
+
+
+@pytest.mark.parametrize("out", [F32, BF16])
+def test_embed_large_batches_of_a_32_bit_table(out):
+    tokens, lengths, table = embed_case(1200, 256, 30522, 768, F32, 64)
+    got = rd.embed_tokens(tokens, table, lengths, out_dtype=out)
+    step = 200
+    for i in range(0, 1200, step):
+        want = embed_ref(tokens[i:i + step], lengths[i:i + step], table, 1.0).to(out)
+        assert torch.equal(got[i:i + step], want)
+    d = rd.embed_tokens_grad(got, tokens, 30522, lengths, dtype=F32)
+    ref = grad_ref(got, tokens, lengths, 30522, 1.0)
+    within(d, ref[0], grad_bound(*ref, F32))
