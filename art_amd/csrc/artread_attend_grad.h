@@ -593,7 +593,7 @@ __global__ __launch_bounds__(256, 2) void attend_grad_kv_kernel(artread_attend_t
 // waiting for that tile then never waits for the stores.  The waves of a workgroup add their dQ in LDS, in order.  PACK:
 // passages too short to fill tiles of their own are packed; a kernel of its own, for the registers.
 template <typename T, int DP, int RB, int NW, bool PACK>
-__global__ __launch_bounds__(64 * NW, 2) void attend_grad_stream_kernel(artread_attend_t A, artread_attend_grads_t G,
+__global__ __launch_bounds__(64 * NW, DP == 64 ? 2 : 1) void attend_grad_stream_kernel(artread_attend_t A, artread_attend_grads_t G,
                                                                         AttendPlan P, const RowStat* __restrict__ stats,
                                                                         float* __restrict__ part) {
     constexpr int TILE = 32 * DP, CH = DP / 8;
