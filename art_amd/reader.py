@@ -34,6 +34,7 @@ READ_SYMBOLS = ("artread_embed", "artread_embed_grad_workspace", "artread_embed_
                 "artread_attend_workspace", "artread_attend", "artread_attend_grad_workspace",
                 "artread_attend_grad", "artread_last_error")
 MAX_HEAD_DIM = 128
+MAX_ROW = 1 << 20   # elements of an embedding
 _ABI = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}  # ARTREAD_F16, ARTREAD_BF16, ARTREAD_F32
 _lib = None
 
@@ -144,6 +145,11 @@ def _check_tokens(tokens, lengths):
         raise ValueError("tokens holds %d positions, the limit is 2**31 - 1" % tokens.numel())
 
 
+def _check_row(dim):
+    if dim > MAX_ROW:
+        raise ValueError("an embedding holds at most %d elements, got %d" % (MAX_ROW, dim))
+
+
 def _embed(tokens, table, lengths, scale, vocab_base, out_dtype):
     dev, shape = table.device, tokens.shape
     vocab, dim = table.shape
@@ -209,6 +215,7 @@ def embed_tokens(tokens, table, lengths=None, scale=1.0, vocab_base=0, out_dtype
         raise ValueError("table must be a float16, bfloat16 or float32 tensor [vocab, dim]")
     if table.shape[1] > 1 and table.stride(1) != 1 or table.stride(0) < table.shape[1] and table.shape[0] > 1:
         raise ValueError("the rows of table must be contiguous and must not overlap")
+    _check_row(table.shape[1])
     out_dtype = table.dtype if out_dtype is None else out_dtype
     if out_dtype != table.dtype and (table.dtype != torch.float32 or out_dtype not in _ABI):
         raise ValueError("out_dtype must be the table's type, or float16 / bfloat16 of a float32 table")
@@ -228,6 +235,7 @@ def embed_tokens_grad(grad_out, tokens, vocab, lengths=None, scale=1.0, vocab_ba
     if grad_out.dtype not in _ABI or grad_out.dim() < 2 or grad_out.shape[:-1] != tokens.shape:
         raise ValueError("grad_out must be a float16, bfloat16 or float32 tensor %s"
                          % (tuple(tokens.shape) + ("dim",),))
+    _check_row(grad_out.shape[-1])
     vocab = int(vocab)
     if not 1 <= vocab < 1 << 31:
         raise ValueError("vocab must be in [1, 2**31), got %d" % vocab)

@@ -86,6 +86,15 @@ def test_embed_tokens_grad_refuses(kwargs):
         rd.embed_tokens_grad(**args)
 
 
+def test_rows_of_more_than_the_limit_are_refused_by_name():
+    wide = torch.zeros((1, rd.MAX_ROW + 8), dtype=torch.float16)
+    tokens = torch.zeros((1, 1), dtype=torch.int32)
+    with pytest.raises(ValueError, match="at most"):
+        rd.embed_tokens(tokens, wide)
+    with pytest.raises(ValueError, match="at most"):
+        rd.embed_tokens_grad(wide[None], tokens, 1)
+
+
 Q = torch.zeros((2, 3, 4, 16), dtype=torch.float16)
 K = torch.zeros((2, 5, 6, 2, 16), dtype=torch.float16)
 KL = torch.zeros((2, 5), dtype=torch.int32)
