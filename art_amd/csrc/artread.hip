@@ -357,9 +357,10 @@ static void plan_share(AttendPlan* P, const artread_attend_t* a) {
 }
 // Passages that lie one behind the other are one long passage where every entry is valid, and one with holes where they
 // are short: of a tile of keys a passage of 7 would fill 7 (32 x 100 rows, 100 passages of 7 of 64 columns: forward 39 us
-// instead of 164, gradients 81 instead of 620).  Longer ones keep tiles of their own, which end with them; up to 63 packing
-// would still gain where rows are many (1,000 passages of 40, 400 rows: 75 us instead of 107), but there a call's last bits
-// would hang on its layout.
+// instead of 164, gradients 81 instead of 620).  Longer ones with lengths keep tiles of their own, which end with them; up
+// to 63 packing measured faster where rows are many (1,000 passages of 40, 400 rows: 75 us instead of 107) and is not taken.
+// Where passages are packed or one long one, sums run over other tiles than where gaps lie between them: a call's last bits
+// depend on its layout there.
 constexpr int64_t kPackLength = 32;
 static bool few_rows(int64_t row_count, int64_t dim) { return row_count <= (dim <= 64 ? 64 : 32); }
 static artread_attend_t pack_passages(const artread_attend_t* given, AttendPlan* P) {

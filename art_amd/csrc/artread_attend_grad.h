@@ -86,7 +86,9 @@ struct Spread<f16> {
     }
 };
 
-// The same with one power of two for a whole wave's dS, where its columns are not the accumulators' ones.
+// The same with one power of two for a whole wave's dS, where its columns are not the accumulators' ones.  Beside the
+// largest dS of the wave's walk so far, entries down to 2^-23 of it keep f16's bits in their two terms; what lies 2^-35
+// below it is lost.
 template <typename T>
 struct SpreadAll {
     __device__ __forceinline__ float inverse() const { return 1.0f; }
@@ -333,11 +335,13 @@ __global__ __launch_bounds__(64 * NW, DP == 64 ? 3 : 2) void attend_grad_q_kerne
 }
 
 // ---- dK and dV: the key walk ------------------------------------------------------------------------------
-// Four waves of 32 keys each share tiles of 64 rows of Q and dO; while a tile is worked on the next one
-// arrives in LDS.  Each is read as rows for S and dP and transposed for dK and dV.  With P.splits > 1 the rows are dealt
+// Four waves of 32 keys each share tiles of 64 rows of Q and dO; the next tile's loads to LDS are sent before a tile is
+// worked on.  Each is read as rows for S and dP and transposed for dK and dV.  With P.splits > 1 the rows are dealt
 // to splits, which leave f32 parts of dK and dV.  K, V, dK and dV of 32 keys are 192 registers of 256, so operands are few
-// ahead, and the wait for LDS is what a wave mostly does besides products (48 % of the cycles): 455-490 us for 8 x 8 x 512
-// states of 128 bf16 columns, 75 % valid, 4,096 rows a key head, 840-910 TFLOP/s.
+// ahead: 455-490 us for 8 x 8 x 512 states of 128 bf16 columns, 75 % valid, 4,096 rows a key head, 840-910 TFLOP/s, a
+// product in 48 % of the cycles.  The rest is waits, for LDS and for the next tile: the compiler, which does not count the
+// loads to LDS, waits for the wave's own K and V at their first use in the loop (vmcnt(1) and vmcnt(0) for f16), behind
+// the next tile's ten loads, so that a tile's first products wait for nearly all of the next one.
 // Tile `first` + wave of a batch entry's tiles of 32 keys.  At 128 columns those with valid keys come first, so that the
 // waves of a workgroup have keys whatever the lengths are: there two waves share a SIMD, and one without keys leaves half
 // of it idle (128 rows, 100 x 150 states, 62 % valid: dQ, dK and dV 640 us instead of 797 with four tiles of one passage a
@@ -585,13 +589,17 @@ __global__ __launch_bounds__(256, 2) void attend_grad_kv_kernel(artread_attend_t
 // Up to 32 * RB rows per key head.  A wave walks tiles of 32 keys, those behind the lengths among them (they get their
 // zeros here), and finishes dK and dV of a tile before the next: every state is read once and every gradient written
 // once, which is what bounds this, where the two walks would read the states twice (16 rows of 8 x 12 heads, 100 x 250
-// states of 64 bf16, 75 % valid: 246 us, 4.4 TB/s; of 128 columns 470 us, 4.6 TB/s; 48 rows of 64 f16, 62 % valid: 270 us,
-// 3.7 TB/s, where 1,100 vector instructions a tile stand beside the bytes).  Two tiles of K in LDS, the next one on its way
-// from the start of a tile, cost more workgroups than they save waiting (325 us against 294, fewer rows 2 % more).  S^T
+// states of 64 bf16, 75 % valid: 246 us, 4.4 TB/s; of 128 columns 470 us, 4.6 TB/s; 48 rows of 64 f16, 62 % valid: 275 to
+// 310 us, 3.3 to 3.7 TB/s).  Two tiles of K in LDS, the next one on its way from the start of a tile, cost more workgroups
+// than they save waiting (325 us against 294, fewer rows 2 % more).  S^T
 // and dP^T leave P^T and dS^T as B operands over the keys, for dQ; dV and dK want them over the rows, so both go through a
-// 32 x 32 tile of LDS and come back by the transposing read.  A tile's results are stored once the next tile has arrived:
-// waiting for that tile then never waits for the stores.  The waves of a workgroup add their dQ in LDS, in order.  PACK:
-// passages too short to fill tiles of their own are packed; a kernel of its own, for the registers.
+// 32 x 32 tile of LDS and come back by the transposing read.  A tile's results are stored once the next tile has arrived,
+// so that waiting for that tile does not wait for the stores; the compiler's own waits still do, at the first use of the
+// row statistics and where a passage's length is read, and for 48 rows a wave waits in 46 % of its cycles.  Two row blocks
+// in f16, and in bf16 where packed, fill the 256 registers: 4 to 10 of them are kept in scratch, and their loads, the zeros
+// of a partly valid tile among them, wait for the stores and the pieces before them too.  The waves of a workgroup add
+// their dQ in LDS, in order.  PACK: passages too short to fill tiles of their own are packed; a kernel of its own, for the
+// registers.  At 64 columns two waves share a SIMD; at 128 LDS leaves one, with up to 436 registers.
 template <typename T, int DP, int RB, int NW, bool PACK>
 __global__ __launch_bounds__(64 * NW, DP == 64 ? 2 : 1) void attend_grad_stream_kernel(artread_attend_t A, artread_attend_grads_t G,
                                                                         AttendPlan P, const RowStat* __restrict__ stats,

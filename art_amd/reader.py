@@ -230,7 +230,7 @@ def embed_tokens_grad(grad_out, tokens, vocab, lengths=None, scale=1.0, vocab_ba
     """Gradient of ``embed_tokens`` in its table: [vocab, dim], every row written (zeros where no valid
     position holds the token).  The tokens are sorted and each row is the 32-bit sum of its positions in a
     fixed order, rounded once: equal inputs give equal bits.  ``dtype`` is grad_out's type (default) or
-    float32."""
+    float32.  Not differentiable itself."""
     _check_tokens(tokens, lengths)
     if grad_out.dtype not in _ABI or grad_out.dim() < 2 or grad_out.shape[:-1] != tokens.shape:
         raise ValueError("grad_out must be a float16, bfloat16 or float32 tensor %s"
@@ -358,7 +358,10 @@ def cross_attention(query, key, value, lengths=None, scale=None, return_lse=Fals
 
     Returns [batch, rows, heads, dim], with ``return_lse`` also the float32 [batch, heads, rows] log of the
     softmax's sum (not differentiable), with ``return_saved`` instead what ``cross_attention_grad`` takes: that
-    log and what rounding took from the result.  Differentiable in query, key and value."""
+    log and what rounding took from the result.  Differentiable in query, key and value.
+
+    Statistics and sums are 32 bits, the weights are rounded once to the inputs' type.  Equal inputs give equal
+    bits; the last ones may depend on whether passages lie one behind the other in memory or with gaps."""
     sizes, scale = _plan(query, key, value, lengths, scale)
     _one_device(query, key, value, lengths)
     if (query.requires_grad or key.requires_grad or value.requires_grad) and torch.is_grad_enabled():
@@ -392,7 +395,8 @@ def _attend_grad(grad_out, query, key, value, lengths, out, lse, rest, sizes, sc
 
 def cross_attention_grad(grad_out, query, key, value, out, saved, lengths=None, scale=None):
     """Gradients (query, key, value) of ``cross_attention`` from its result ``out`` and what it ``saved``.
-    Written whole, zeros behind each passage's length; equal inputs give equal bits."""
+    Written whole, zeros behind each passage's length; equal inputs in equal layouts give equal bits.  Not
+    differentiable itself."""
     sizes, scale = _plan(query, key, value, lengths, scale)
     if grad_out.shape != query.shape or grad_out.dtype != query.dtype:
         raise ValueError("grad_out must have query's shape and type")

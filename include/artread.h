@@ -69,7 +69,10 @@ int artread_embed_grad(int device, const void* grad_out, int grad_dtype, const v
  *   heads is a multiple of kv_heads: query head h reads key head h / (heads / kv_heads)
  * f16 or bf16, dim a multiple of 8 up to 128.  Strides count elements; the innermost one is 1, the
  * others are >= 0 and multiples of 8, those of rows below 2^24, the query heads that share a key head
- * within 2^29 elements, the rest below 2^40.  Pointers are 16-byte aligned; out is contiguous. */
+ * within 2^29 elements, the rest below 2^40.  Pointers are 16-byte aligned; out is contiguous.
+ * Scores, softmax statistics and sums are f32; weights are rounded once to the states' type before they meet v.
+ * Passages that lie one behind the other in memory may share tiles, those with gaps between them do not: equal
+ * inputs with equal strides give equal bits, with other strides the last ones may differ. */
 typedef struct {
     const void* q;
     const void* k;
@@ -93,7 +96,8 @@ int artread_attend(int device, const artread_attend_t* a, void* workspace, int64
  * (rest may be NULL: the row sums of grad_out * out then take out as it was rounded).
  * grad_out is [batch, rows, heads, dim] with the given strides; grad_q, grad_k and grad_v are contiguous
  * of q's, k's and v's shapes and written whole, zeros behind each passage's length.  No atomics: equal
- * inputs give equal bits. */
+ * inputs with equal strides give equal bits.  Weights and their gradients are rounded to the states' type
+ * before the products that make grad_q, grad_k and grad_v, which add in f32. */
 typedef struct {
     const void* grad_out;
     int64_t g_batch, g_row, g_head;
