@@ -443,6 +443,10 @@ __global__ __launch_bounds__(256, 2) void attend_grad_kv_kernel(artread_attend_t
 #pragma unroll
     for (int db = 0; db < DP / 32; ++db) dk[db] = dv[db] = f32x16{};
     if (at_tile.some) {   // uniform over the workgroup
+        if (dim < DP) {
+            for (int i = threadIdx.x; i < 4 * TILE / 8; i += 256) ((u32x4*)&qtile[0][0])[i] = u32x4{0, 0, 0, 0};
+            __syncthreads();
+        }
         V8 kf[DP / 16], vf[DP / 16];
         const T* kp = (const T*)A.k + b * A.k_batch + p * A.k_passage + j * A.k_row + kh * A.k_head + 8 * half;
         const T* vp = (const T*)A.v + b * A.v_batch + p * A.v_passage + j * A.v_row + kh * A.v_head + 8 * half;
@@ -478,9 +482,8 @@ __global__ __launch_bounds__(256, 2) void attend_grad_kv_kernel(artread_attend_t
                 dma_pieces<PW, 4096>(qt, positions * (uint32_t)A.q_row * 2, qo, dst);
                 dma_pieces<PW, 4096>(gt, positions * (uint32_t)G.g_row * 2, go, dst + 2 * TILE * 2);
             } else {
-                // rows that are not there repeat the last one (their weight is zero), columns behind dim the first (they
-                // meet zeros of K and V)
-                const uint32_t col = chunk * 8 < (uint32_t)dim ? chunk * 8 : 0;
+                // rows that are not there repeat the last one (their weight is zero); columns behind dim stay cleared
+                const bool there = dim == DP || chunk * 8 < (uint32_t)dim;
 #pragma unroll
                 for (int x = 0; x < PW; ++x) {
                     int64_t r = (int64_t)tile * 32 * RT + (x * 4 + wave) * PR + prow;
@@ -488,8 +491,10 @@ __global__ __launch_bounds__(256, 2) void attend_grad_kv_kernel(artread_attend_t
                     split_row(P, 0, (uint32_t)r, &t, &h);
                     // bytes from the tile's first query position: a tile spans at most as many of them as rows
                     const uint32_t dt = (uint32_t)t - (uint32_t)t0;
-                    dma16(qt, (dt * (uint32_t)A.q_row + (uint32_t)(h * A.q_head) + col) * 2, dst + x * 4096);
-                    dma16(gt, (dt * (uint32_t)G.g_row + (uint32_t)(h * G.g_head) + col) * 2, dst + 2 * TILE * 2 + x * 4096);
+                    if (there) {
+                        dma16(qt, (dt * (uint32_t)A.q_row + (uint32_t)(h * A.q_head) + chunk * 8) * 2, dst + x * 4096);
+                        dma16(gt, (dt * (uint32_t)G.g_row + (uint32_t)(h * G.g_head) + chunk * 8) * 2, dst + 2 * TILE * 2 + x * 4096);
+                    }
                 }
             }
 #pragma unroll

@@ -897,3 +897,35 @@ def test_embed_large_batches_of_a_32_bit_table(out):
     d = rd.embed_tokens_grad(got, tokens, 30522, lengths, dtype=F32)
     ref = grad_ref(got, tokens, lengths, 30522, 1.0)
     within(d, ref[0], grad_bound(*ref, F32))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("rows", [1, 40, 200])
+@pytest.mark.parametrize("dim", [40, 64, 80, 128])
+def test_attention_a_row_whose_scores_are_all_minus_infinity(dim, rows, dtype):
+    """An infinite element of one query that meets negative elements alone: its row has no weight, and the others'
+    gradients stay what they are (but for dK's column of that element, 0 * inf)."""
+    q, k, v, lengths, grad = attend_case(2, rows, 3, 70, 2, 2, dim, dtype, 65)
+    k[..., 3] = -k[..., 3].abs() - 0.5
+    lengths[0] = torch.tensor([70, 33, 0], device="cuda", dtype=torch.int32)
+    row = rows - 1
+    alone = q.clone()
+    alone[0, row, 1] = 0
+    weight = grad.clone()
+    weight[0, row, 1] = 0
+    ref = attend_ref(alone, k, v, lengths, weight)   # a row of zeros with no gradient adds nothing to dK and dV
+    q[0, row, 1, 3] = float("inf")
+    out, saved = rd.cross_attention(q, k, v, lengths, return_saved=True)
+    got = rd.cross_attention_grad(grad, q, k, v, out, saved, lengths)
+    assert int(out[0, row, 1].count_nonzero()) == 0 and float(saved[0][0, 1, row]) == -math.inf
+    assert int(got[0][0, row, 1].count_nonzero()) == 0
+    others = torch.ones((2, rows, 2), dtype=torch.bool, device="cuda")
+    others[0, row, 1] = False
+    within(out[others], *(x[others] for x in ref["out"]))
+    within(got[0][others], *(x[others] for x in ref["dq"]))
+    within(got[2], *ref["dv"])
+    columns = torch.ones(k.shape, dtype=torch.bool, device="cuda")
+    columns[0, :, :, 1, 3] = False
+    within(got[1][columns], *(x[columns] for x in ref["dk"]))
+    inside = torch.arange(70, device="cuda") < lengths[0][:, None]
+    assert bool(torch.isnan(got[1][0, :, :, 1, 3][inside]).all()) and int(got[1][0, :, :, 1, 3][~inside].count_nonzero()) == 0
