@@ -482,19 +482,31 @@ __global__ __launch_bounds__(256, 2) void attend_grad_kv_kernel(artread_attend_t
                 dma_pieces<PW, 4096>(qt, positions * (uint32_t)A.q_row * 2, qo, dst);
                 dma_pieces<PW, 4096>(gt, positions * (uint32_t)G.g_row * 2, go, dst + 2 * TILE * 2);
             } else {
-                // rows that are not there repeat the last one (their weight is zero); columns behind dim stay cleared
-                const bool there = dim == DP || chunk * 8 < (uint32_t)dim;
+                const bool there = dim == DP || chunk * 8 < (uint32_t)dim;   // columns behind dim stay cleared
 #pragma unroll
                 for (int x = 0; x < PW; ++x) {
-                    int64_t r = (int64_t)tile * 32 * RT + (x * 4 + wave) * PR + prow;
-                    r = r < P.row_count ? r : P.row_count - 1;
+                    const int64_t r = (int64_t)tile * 32 * RT + (x * 4 + wave) * PR + prow;
                     split_row(P, 0, (uint32_t)r, &t, &h);
                     // bytes from the tile's first query position: a tile spans at most as many of them as rows
                     const uint32_t dt = (uint32_t)t - (uint32_t)t0;
-                    if (there) {
+                    if (there && r < P.row_count) {
                         dma16(qt, (dt * (uint32_t)A.q_row + (uint32_t)(h * A.q_head) + chunk * 8) * 2, dst + x * 4096);
                         dma16(gt, (dt * (uint32_t)G.g_row + (uint32_t)(h * G.g_head) + chunk * 8) * 2, dst + 2 * TILE * 2 + x * 4096);
                     }
+                }
+                if ((int64_t)(tile + 1) * 32 * RT > P.row_count) {   // uniform
+                    // rows that are not there: the last one's query, whose weight is zero, and a gradient of zeros, since no
+                    // weight times an infinite one would be NaN
+                    const uint32_t l2 = opaque(lane), z = opaque(0);   // made here: no register holds them over the loop
+                    const int left = (int)(P.row_count - (int64_t)tile * 32 * RT) - (int)(wave * PR + l2 / CH);
+                    split_row(P, 0, (uint32_t)(P.row_count - 1), &t, &h);
+                    const uint32_t last = (((uint32_t)t - (uint32_t)t0) * (uint32_t)A.q_row + (uint32_t)(h * A.q_head) + chunk * 8) * 2;
+#pragma unroll
+                    for (int x = 0; x < PW; ++x)
+                        if (x * 4 * PR >= left) {
+                            if (there) dma16(qt, last, dst + x * 4096);
+                            *(__attribute__((address_space(3))) u32x4*)(uintptr_t)(dst + 2 * TILE * 2 + x * 4096 + l2 * 16) = u32x4{z, z, z, z};
+                        }
                 }
             }
 #pragma unroll

@@ -929,3 +929,28 @@ def test_attention_a_row_whose_scores_are_all_minus_infinity(dim, rows, dtype):
     within(got[1][columns], *(x[columns] for x in ref["dk"]))
     inside = torch.arange(70, device="cuda") < lengths[0][:, None]
     assert bool(torch.isnan(got[1][0, :, :, 1, 3][inside]).all()) and int(got[1][0, :, :, 1, 3][~inside].count_nonzero()) == 0
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("rows", [1, 20, 40, 64, 200])
+@pytest.mark.parametrize("dim", [64, 80, 128])
+def test_attention_an_infinite_gradient_of_the_last_row(dim, rows, dtype):
+    """dV takes the infinity in its column, with its sign, and keeps the others; rows that are not there add nothing."""
+    q, k, v, lengths, grad = attend_case(2, rows, 3, 70, 4, 2, dim, dtype, 66, q_std=0.3)
+    lengths[0] = torch.tensor([70, 33, 0], device="cuda", dtype=torch.int32)
+    ref = attend_ref(q, k, v, lengths, grad)
+    out, saved = rd.cross_attention(q, k, v, lengths, return_saved=True)
+    clean = rd.cross_attention_grad(grad, q, k, v, out, saved, lengths)
+    inside = torch.arange(70, device="cuda") < lengths[0][:, None]
+    for value in (math.inf, -math.inf):
+        grad[0, -1, 3, 9] = value
+        got = rd.cross_attention_grad(grad, q, k, v, out, saved, lengths)
+        assert bool((got[2][0, :, :, 1, 9][inside] == value).all())
+        others = torch.ones(k.shape, dtype=torch.bool, device="cuda")
+        others[0, :, :, 1, 9] = False
+        assert torch.equal(got[2][others], clean[2][others])
+        within(got[2][others], *(x[others] for x in ref["dv"]))
+        rows_left = torch.ones(q.shape, dtype=torch.bool, device="cuda")
+        rows_left[0, -1, 3] = False
+        assert torch.equal(got[0][rows_left], clean[0][rows_left]) and not bool(torch.isfinite(got[0][~rows_left]).any())
+        assert torch.equal(got[1][:, :, :, 0], clean[1][:, :, :, 0]) and torch.equal(got[1][1], clean[1][1])
