@@ -99,14 +99,21 @@ def _rcheck(rc):
         raise ArtreadError(rc, _read().artread_last_error().decode("utf-8", "replace"))
 
 
+_tracing_state, _dispatch_modes = torch._C._get_tracing_state, torch._C._len_torch_dispatch_stack
+
+
+def _refuse_tangents(*tensors):
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError("forward-mode derivatives are not implemented: a tensor has a tangent")
+
+
 def _one_device(first, *others):
     """Every tensor of a call lives on one GPU: the kernels read them all by address.  What torch would keep
     beside a tensor's values, and a call by address would lose, is refused first."""
     if forward_ad._current_level >= 0:   # inside a dual level
-        for t in (first, *others):
-            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
-                raise NotImplementedError("forward-mode derivatives are not implemented: a tensor has a tangent")
-    if torch.jit.is_tracing() or torch._C._len_torch_dispatch_stack() and get_proxy_mode() is not None:
+        _refuse_tangents(first, *others)
+    if _tracing_state() is not None or _dispatch_modes() and get_proxy_mode() is not None:
         raise NotImplementedError("a traced graph would hold the outputs' allocation but not the call that fills them")
     if not first.is_cuda:
         raise ValueError("tensors must be on a GPU, got %s" % first.device)
@@ -197,7 +204,8 @@ class _EmbedTokens(torch.autograd.Function):
     def backward(ctx, grad_out):
         tokens, lengths = ctx.saved_tensors
         vocab, scale, vocab_base, dtype = ctx.of
-        _one_device(grad_out, tokens, lengths)
+        if forward_ad._current_level >= 0:
+            _refuse_tangents(grad_out)
         return _embed_grad(grad_out, tokens, lengths, vocab, scale, vocab_base, dtype), None, None, None, None, None
 
 
